@@ -385,6 +385,43 @@ int moe_decode_noalloc(const moe_layer_desc* desc, const moe_weights* w, const u
                        int64_t* topk_ids_dev, uint16_t* topk_weights_dev, int32_t* status_dev,
                        void* stream, char* err, size_t err_len);
 
+/* ---- Dense (unquantised) projections ----
+ * The products of the reference's bf16 nn.Linear modules (dense decoder
+ * layers, GPU-resident experts, router: nano_ktrans/layers/expert_mlp.py:9-25,
+ * nano_ktrans/models/mixtral.py:127, :180-189) with what follows them in the
+ * same kernel.  Stateless: no handle and no workspace, nothing is kept between
+ * calls, so calls on several streams or in several graphs are independent.
+ *   w_up_dev NULL:  out = round(act(x . w^T + bias) + residual)
+ *   w_up_dev set:   out = round(act(x . w^T) * (x . w_up^T))
+ * x [m][k], w and w_up [n][k], bias [n], residual and out [m][n]: 16-bit
+ * elements of `dtype` (one type for all), unit stride along a row, the ld*
+ * elements from row to row; bias and residual may be NULL.  Sums are fp32,
+ * the result is rounded once.  residual_dev == out_dev (same ldr) adds in
+ * place; any other overlap of out with an input is refused.  m == 0 is a
+ * no-op.  Any alignment of 2 bytes is accepted; rows on 16-byte boundaries
+ * with k a multiple of 8 take the fast kernels. */
+enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_FP16 = 1 };
+enum moe_activation {
+  MOE_ACT_NONE = 0,
+  MOE_ACT_SILU = 1,
+  MOE_ACT_GELU = 2,      /* v/2 (1 + erf(v / sqrt 2)) */
+  MOE_ACT_GELU_TANH = 3, /* its tanh approximation */
+  MOE_ACT_RELU = 4
+};
+typedef struct moe_linear_desc {
+  const void* x_dev;
+  const void* w_dev;
+  const void* w_up_dev;
+  const void* bias_dev;
+  const void* residual_dev;
+  void* out_dev;
+  int64_t ldx, ldw, ldw_up, ldr, ldo;
+  int32_t m, n, k;
+  int32_t dtype;
+  int32_t activation;
+} moe_linear_desc;
+int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

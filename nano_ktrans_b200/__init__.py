@@ -7,6 +7,8 @@ Public API (mirrors the reference's names):
 * ``CudaMoEBackend`` — the ``"cuda"`` expert backend
 * ``HybridMoE`` — the MoE layer using it
 * ``MoeLayer`` — direct access to the C-ABI handle (route / experts / fused forward)
+* ``linear``, ``gated_linear``, ``DenseMLP`` — unquantised (bf16 / fp16) projections with their
+  bias, activation, gating and residual in the same kernel
 * ``EpMoeLayer``, ``plan_placement``, ``shard_layer``, ``TorchDistComm``,
   ``PeerExchange`` — expert parallelism over the ranks of a process group (NCCL
   all-to-alls, or the library's kernels over peer memory)
@@ -18,6 +20,7 @@ __all__ = [
     "ExpertOffloadBackend", "normalize_offload_backend_name", "GPTQLinearWeight", "LayerWeights",
     "quantize_symmetric", "stack_layer", "CudaMoEBackend", "HybridMoE", "MoeLayer",
     "EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange",
+    "linear", "gated_linear", "DenseMLP",
 ]
 
 
@@ -34,4 +37,7 @@ def __getattr__(name):
     if name in ("EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange"):
         from . import expert_parallel
         return getattr(expert_parallel, name)
+    if name in ("linear", "gated_linear", "DenseMLP"):
+        from . import dense
+        return getattr(dense, name)
     raise AttributeError(name)

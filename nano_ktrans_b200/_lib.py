@@ -15,6 +15,8 @@ HEADER_PATH = os.path.join(os.path.dirname(PKG_DIR), "include", "moe_b200.h")
 
 MOE_OK, MOE_EINVAL, MOE_ECUDA, MOE_ENOWEIGHTS, MOE_ERANGE, MOE_EDEVICE = range(6)
 K_ROUTE, K_PERMUTE, K_GATEUP, K_DOWN, K_COMBINE, K_DECODE_FUSED = range(1, 7)
+DTYPE_BF16, DTYPE_FP16 = 0, 1
+ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 OPT_DECODE_FUSED, OPT_TRACE, OPT_GEMM, OPT_GEMM_TILE, OPT_STREAM, OPT_HOST_IO = 1, 2, 3, 4, 5, 6
 
 _DESC_FIELDS = ("num_experts", "top_k", "hidden_size", "inter_size", "bits", "group_size",
@@ -30,6 +32,12 @@ class MoeLayerDesc(ctypes.Structure):
 
 class MoeWeights(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in _WEIGHT_FIELDS]
+
+
+class MoeLinearDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x_dev", "w_dev", "w_up_dev", "bias_dev", "residual_dev", "out_dev")]
+                + [(n, ctypes.c_int64) for n in ("ldx", "ldw", "ldw_up", "ldr", "ldo")]
+                + [(n, ctypes.c_int32) for n in ("m", "n", "k", "dtype", "activation")])
 
 
 class MoeError(RuntimeError):
@@ -79,6 +87,7 @@ SIGNATURES = {
     "moe_ep_group_last_error": (_i32, [_vp, _cp, _sz]),
     "moe_ep_group_close_peers": (_i32, [_vp]),
     "moe_ep_group_destroy": (_i32, [_vp]),
+    "moe_linear": (_i32, [ctypes.POINTER(MoeLinearDesc), _vp, _cp, _sz]),
 }
 
 EP_IPC_HANDLE_BYTES = 64
