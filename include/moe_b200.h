@@ -422,6 +422,71 @@ typedef struct moe_linear_desc {
 } moe_linear_desc;
 int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_len);
 
+/* ---- A whole expert layer on unquantised weights, for a few tokens ----
+ * The reference's MoE block (nano_ktrans/models/mixtral.py:212-218) with
+ * GPU-resident bf16 / fp16 experts (layers/hybrid_moe.py:3321-3329, :3442-3533)
+ * and the decoder layer's residual add, in two kernel launches:
+ *   out[t] = round(residual[t] + sum_e w[t][e] * down_e(silu(gate_e(x[t])) * up_e(x[t]))
+ *                  + sigmoid(x[t] . shared_gate_vec) * shared(x[t]))
+ * in fp32, e over the experts that token t is routed to (and offload_mask
+ * keeps).  Weights of one type: gate, up [num_experts][inter][hidden], down
+ * [num_experts][hidden][inter], shared likewise with shared_inter, router_w
+ * [num_experts][hidden], all contiguous.  All weights have to be finite.
+ * Routing, one of:
+ *   router_w_dev set             logits = round(x . router_w^T), then top-k;
+ *                                logits_dev, when set, receives them
+ *   logits_dev set               top-k of the given logits
+ *   ids_dev and weights_dev set  given: ids [tokens][top_k] int64, negative
+ *                                ones mean no expert (ids >= num_experts too,
+ *                                flagged in the status word), weights of the
+ *                                layer's type; an expert given twice for a
+ *                                token counts with both weights
+ * with the ranking and rounding of moe_route, in the layer's type.
+ * ids_out_dev / weights_out_dev (may be NULL) receive the routing in the first
+ * two forms.
+ * 0 <= num_tokens <= MOE_DENSE_MAX_TOKENS (above: MOE_ERANGE), num_experts in
+ * [1, 1024], top_k in [1, min(16, num_experts)], hidden and inter multiples of
+ * 16, x rows and all weights on 32-byte boundaries.  out may be x or residual
+ * itself, and overlaps nothing else.
+ * workspace_dev: moe_dense_workspace bytes, 256-byte aligned, for this call
+ * alone until its kernels have run (calls in flight at once, and graphs
+ * replayed at once, each need their own).  Its contents need no preparation.
+ * Nothing else is kept between calls. */
+#define MOE_DENSE_MAX_TOKENS 16
+typedef struct moe_dense_desc {
+  const void* gate_dev;
+  const void* up_dev;
+  const void* down_dev;
+  const void* shared_gate_dev; /* with shared_inter > 0 */
+  const void* shared_up_dev;
+  const void* shared_down_dev;
+  const void* shared_gate_vec_dev;
+  int32_t num_experts, top_k, hidden_size, inter_size, shared_inter;
+  int32_t router_use_softmax, normalize_topk_prob;
+  int32_t dtype;
+  /* per call */
+  const void* x_dev;
+  const void* router_w_dev;
+  void* logits_dev;
+  const int64_t* ids_dev;
+  const void* weights_dev;
+  const uint8_t* offload_mask_dev; /* [num_experts], 0 leaves an expert out; NULL: none */
+  const void* residual_dev;
+  void* out_dev;
+  int64_t* ids_out_dev;
+  void* weights_out_dev;
+  void* workspace_dev;
+  int64_t ldx, ldr, ldo; /* elements between rows of x, residual, out */
+  int64_t workspace_bytes;
+  int32_t num_tokens;
+  int32_t add_shared; /* 0 leaves the shared expert out of this call */
+} moe_dense_desc;
+int moe_dense_workspace(const moe_dense_desc* desc, int64_t* bytes, char* err, size_t err_len);
+int moe_dense_forward(const moe_dense_desc* desc, void* stream, char* err, size_t err_len);
+/* Copy the current device's status word of the dense calls (bits as
+ * moe_read_status) to *status and clear it; synchronises `stream`. */
+int moe_dense_read_status(int32_t* status, void* stream, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

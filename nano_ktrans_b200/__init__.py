@@ -9,6 +9,8 @@ Public API (mirrors the reference's names):
 * ``MoeLayer`` — direct access to the C-ABI handle (route / experts / fused forward)
 * ``linear``, ``gated_linear``, ``DenseMLP`` — unquantised (bf16 / fp16) projections with their
   bias, activation, gating and residual in the same kernel
+* ``DenseMoeLayer`` — a whole expert layer on unquantised weights for a few tokens: router
+  projection, routing, experts, shared expert and residual in two kernels
 * ``EpMoeLayer``, ``plan_placement``, ``shard_layer``, ``TorchDistComm``,
   ``PeerExchange`` — expert parallelism over the ranks of a process group (NCCL
   all-to-alls, or the library's kernels over peer memory)
@@ -20,7 +22,7 @@ __all__ = [
     "ExpertOffloadBackend", "normalize_offload_backend_name", "GPTQLinearWeight", "LayerWeights",
     "quantize_symmetric", "stack_layer", "CudaMoEBackend", "HybridMoE", "MoeLayer",
     "EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange",
-    "linear", "gated_linear", "DenseMLP",
+    "linear", "gated_linear", "DenseMLP", "DenseMoeLayer",
 ]
 
 
@@ -40,4 +42,7 @@ def __getattr__(name):
     if name in ("linear", "gated_linear", "DenseMLP"):
         from . import dense
         return getattr(dense, name)
+    if name == "DenseMoeLayer":
+        from .dense_moe import DenseMoeLayer
+        return DenseMoeLayer
     raise AttributeError(name)

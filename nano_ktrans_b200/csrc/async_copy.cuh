@@ -90,5 +90,25 @@ MOE_DEV bool grid_sync_epoch(unsigned long long* bar, unsigned long long seen, i
   return *ok_smem != 0;
 }
 
+// Grid-wide barrier on a counter that an earlier kernel of the stream zeroed
+// for this launch alone.
+MOE_DEV bool grid_sync_zeroed(unsigned long long* bar, int* ok_smem) {
+  __syncthreads();  // the CTA's writes are ordered before thread 0's release (cumulativity)
+  if (threadIdx.x == 0) {
+    asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(bar) : "memory");
+    cuda::atomic_ref<unsigned long long, cuda::thread_scope_device> count(*bar);
+    int ok = 1;
+    for (uint32_t i = 0; count.load(cuda::memory_order_acquire) < gridDim.x; ++i) {
+      if (i > kSpinLimit) {
+        ok = 0;
+        break;
+      }
+    }
+    *ok_smem = ok;
+  }
+  __syncthreads();
+  return *ok_smem != 0;
+}
+
 }  // namespace ac
 }  // namespace moe

@@ -26,5 +26,41 @@ struct LinearArgs {
 // Every shape, stride and alignment.
 cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st);
 
+// Elements of the widest load that every row of x and of the weights allows:
+// 16 (32 bytes), 8 (16 bytes), or 0 (none).
+int wide_elements(const LinearArgs& a);
+// Up to kStreamTokens tokens, wide_elements(a) != 0.
+constexpr int kStreamTokens = 32;
+cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaStream_t st);
+
+// A whole expert layer for up to kMoeTokens tokens.
+constexpr int kMoeTokens = 16;
+constexpr int kMoeTopK = 16;
+constexpr int kMoePairs = kMoeTokens * kMoeTopK;
+constexpr int kMoeExperts = 1024;
+struct MoeArgs {
+  const uint16_t* x;
+  const uint16_t* router_w;  // logits are computed when set, else read (or unused with ids_in)
+  uint16_t* logits;          // [tokens][experts]
+  const int64_t* ids_in;     // given routing [tokens][top_k], or null
+  const uint16_t* w_in;
+  const uint8_t* mask;       // [experts], null: all
+  const uint16_t *gate, *up, *down;  // [experts][inter][hidden] twice, [experts][hidden][inter]
+  const uint16_t *shared_gate, *shared_up, *shared_down, *shared_gate_vec;
+  const uint16_t* res;
+  uint16_t* out;
+  int64_t* ids_out;
+  uint16_t* w_out;
+  // workspace of the call
+  unsigned long long* bar;
+  float* shared_open;        // [tokens]
+  uint16_t* h;               // [tokens * top_k][hi, lo][inter]
+  uint16_t* h_shared;        // [tokens][hi, lo][shared_inter]
+  int64_t ldx, ldr, ldo;
+  int tokens, experts, top_k, hidden, inter, shared_inter, use_softmax, renorm;
+};
+cudaError_t launch_dense_moe(const MoeArgs& a, int dtype, int sms, cudaStream_t st);
+cudaError_t read_dense_status(int* status, cudaStream_t st);
+
 }  // namespace dense
 }  // namespace moe

@@ -33,6 +33,20 @@ Span span(const void* p, int64_t rows, int64_t cols, int64_t ld) {
 }
 bool meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
 
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  return cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? sms : 0;
+}
+
+cudaError_t launch_linear(const LinearArgs& a, int dtype, cudaStream_t st) {
+  const int sms = sm_count();
+  if (sms < 1) return cudaErrorInvalidDevice;
+  if (moe::dense::wide_elements(a) == 0) return moe::dense::launch_generic(a, dtype, st);
+  if (a.m <= moe::dense::kStreamTokens) return moe::dense::launch_stream_linear(a, dtype, sms, st);
+  return moe::dense::launch_generic(a, dtype, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -84,8 +98,172 @@ int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len
   a.n = d->n;
   a.k = d->k;
   a.act = d->activation;
-  const cudaError_t e = moe::dense::launch_generic(a, d->dtype, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_linear(a, d->dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "%s: %s", me, cudaGetErrorString(e));
+  return MOE_OK;
+}
+
+
+namespace {
+
+struct MoeSpace {
+  size_t bar, open, logits, h, h_shared, bytes;
+};
+MoeSpace moe_space(const moe_dense_desc& d) {
+  const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+  const size_t t = d.num_tokens;
+  MoeSpace s{};
+  s.bar = 0;
+  s.open = 256;
+  s.logits = s.open + up(4 * t);
+  s.h = s.logits + up(2 * t * d.num_experts);
+  s.h_shared = s.h + up(4 * t * d.top_k * d.inter_size);
+  s.bytes = s.h_shared + up(4 * t * d.shared_inter);
+  return s;
+}
+
+// nullptr, or what is wrong with the layer's description.
+const char* check_layer(const moe_dense_desc& d) {
+  if (d.dtype != MOE_DTYPE_BF16 && d.dtype != MOE_DTYPE_FP16) return "dtype must be MOE_DTYPE_BF16 or MOE_DTYPE_FP16";
+  if (d.num_experts < 1 || d.num_experts > moe::dense::kMoeExperts) return "num_experts must be in [1, 1024]";
+  if (d.top_k < 1 || d.top_k > moe::dense::kMoeTopK || d.top_k > d.num_experts)
+    return "top_k must be in [1, min(16, num_experts)]";
+  const int32_t big = 1 << 20;
+  if (d.hidden_size < 16 || d.hidden_size % 16 || d.hidden_size > big) return "hidden_size must be a positive multiple of 16";
+  if (d.inter_size < 16 || d.inter_size % 16 || d.inter_size > big) return "inter_size must be a positive multiple of 16";
+  if (d.shared_inter < 0 || d.shared_inter % 16 || d.shared_inter > big) return "shared_inter must be a multiple of 16";
+  if (d.num_tokens < 0) return "negative token count";
+  return nullptr;
+}
+
+}  // namespace
+
+int moe_dense_workspace(const moe_dense_desc* d, int64_t* bytes, char* err, size_t err_len) {
+  if (d == nullptr || bytes == nullptr) return refuse(err, err_len, MOE_EINVAL, "moe_dense_workspace: null argument");
+  if (const char* why = check_layer(*d)) return refuse(err, err_len, MOE_EINVAL, "moe_dense_workspace: %s", why);
+  if (d->num_tokens > MOE_DENSE_MAX_TOKENS)
+    return refuse(err, err_len, MOE_ERANGE, "moe_dense_workspace: %d tokens, at most %d", d->num_tokens, MOE_DENSE_MAX_TOKENS);
+  *bytes = static_cast<int64_t>(moe_space(*d).bytes);
+  return MOE_OK;
+}
+
+int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t err_len) {
+  const char* me = "moe_dense_forward";
+  if (d == nullptr) return refuse(err, err_len, MOE_EINVAL, "%s: null argument", me);
+  if (const char* why = check_layer(*d)) return refuse(err, err_len, MOE_EINVAL, "%s: %s", me, why);
+  if (d->num_tokens > MOE_DENSE_MAX_TOKENS)
+    return refuse(err, err_len, MOE_ERANGE, "%s: %d tokens, at most %d", me, d->num_tokens, MOE_DENSE_MAX_TOKENS);
+  if (d->num_tokens == 0) return MOE_OK;
+  const bool shared = d->shared_inter > 0 && d->add_shared;
+  const int64_t t = d->num_tokens, E = d->num_experts, H = d->hidden_size, I = d->inter_size;
+  const int64_t S = shared ? d->shared_inter : 0;
+  const void* need[] = {d->gate_dev, d->up_dev, d->down_dev, d->x_dev, d->out_dev, d->workspace_dev};
+  for (const void* p : need)
+    if (p == nullptr) return refuse(err, err_len, MOE_EINVAL, "%s: null device pointer", me);
+  if (shared && (!d->shared_gate_dev || !d->shared_up_dev || !d->shared_down_dev || !d->shared_gate_vec_dev))
+    return refuse(err, err_len, MOE_EINVAL, "%s: null shared-expert pointer", me);
+  const bool given = d->ids_dev != nullptr || d->weights_dev != nullptr;
+  if (given && (d->ids_dev == nullptr || d->weights_dev == nullptr || d->router_w_dev || d->logits_dev))
+    return refuse(err, err_len, MOE_EINVAL, "%s: given routing needs ids and weights, and no router or logits", me);
+  if (!given && d->router_w_dev == nullptr && d->logits_dev == nullptr)
+    return refuse(err, err_len, MOE_EINVAL, "%s: no routing: router weights, logits or ids", me);
+  if (given && (d->ids_out_dev || d->weights_out_dev))
+    return refuse(err, err_len, MOE_EINVAL, "%s: given routing is not written out again", me);
+  const void* wide[] = {d->gate_dev, d->up_dev, d->down_dev, d->x_dev, d->router_w_dev,
+                        shared ? d->shared_gate_dev : nullptr, shared ? d->shared_up_dev : nullptr,
+                        shared ? d->shared_down_dev : nullptr, shared ? d->shared_gate_vec_dev : nullptr};
+  for (const void* p : wide)
+    if (reinterpret_cast<uintptr_t>(p) % 32)
+      return refuse(err, err_len, MOE_EINVAL, "%s: x and the weights must start on 32-byte boundaries", me);
+  if (t > 1 && d->ldx % 16) return refuse(err, err_len, MOE_EINVAL, "%s: the rows of x must lie on 32-byte boundaries", me);
+  const void* even[] = {d->logits_dev, d->weights_dev, d->residual_dev, d->out_dev, d->weights_out_dev};
+  for (const void* p : even)
+    if (reinterpret_cast<uintptr_t>(p) % 2) return refuse(err, err_len, MOE_EINVAL, "%s: pointers must be 2-byte aligned", me);
+  if (reinterpret_cast<uintptr_t>(d->ids_dev) % 8 || reinterpret_cast<uintptr_t>(d->ids_out_dev) % 8)
+    return refuse(err, err_len, MOE_EINVAL, "%s: ids must be 8-byte aligned", me);
+  if (d->ldx < H || d->ldo < H || (d->residual_dev && d->ldr < H))
+    return refuse(err, err_len, MOE_EINVAL, "%s: the rows of x, residual and out must be at least hidden_size apart", me);
+  const MoeSpace ws = moe_space(*d);
+  if (reinterpret_cast<uintptr_t>(d->workspace_dev) % 256 || d->workspace_bytes < static_cast<int64_t>(ws.bytes))
+    return refuse(err, err_len, MOE_EINVAL, "%s: the workspace must be 256-byte aligned and hold %lld bytes", me,
+                  static_cast<long long>(ws.bytes));
+  // What is written: out, the routing, the logits, the workspace.  Nothing of
+  // it may meet anything that is read, nor each other; out may be x (which is
+  // read no more once the first output is stored) or residual.
+  const auto whole = [](const void* p, int64_t n, int64_t bytes_each) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+    return p ? Span{b, b + static_cast<uintptr_t>(n * bytes_each)} : Span{0, 0};
+  };
+  const Span x = span(d->x_dev, t, H, d->ldx), out = span(d->out_dev, t, H, d->ldo);
+  const Span res = d->residual_dev ? span(d->residual_dev, t, H, d->ldr) : Span{0, 0};
+  const Span lg = whole(d->logits_dev, t * E, 2);
+  const Span written[] = {out, whole(d->workspace_dev, ws.bytes, 1), whole(d->ids_out_dev, t * d->top_k, 8),
+                          whole(d->weights_out_dev, t * d->top_k, 2), d->router_w_dev ? lg : Span{0, 0}};
+  const Span read[] = {x, res, whole(d->gate_dev, E * I * H, 2), whole(d->up_dev, E * I * H, 2),
+                       whole(d->down_dev, E * I * H, 2), whole(shared ? d->shared_gate_dev : nullptr, S * H, 2),
+                       whole(shared ? d->shared_up_dev : nullptr, S * H, 2),
+                       whole(shared ? d->shared_down_dev : nullptr, S * H, 2),
+                       whole(shared ? d->shared_gate_vec_dev : nullptr, H, 2), whole(d->router_w_dev, E * H, 2),
+                       d->router_w_dev ? Span{0, 0} : lg, whole(d->ids_dev, t * d->top_k, 8),
+                       whole(d->weights_dev, t * d->top_k, 2), whole(d->offload_mask_dev, E, 1)};
+  const bool on_x = d->out_dev == d->x_dev && (t == 1 || d->ldo == d->ldx);
+  const bool on_res = d->out_dev == d->residual_dev && (t == 1 || d->ldo == d->ldr);
+  for (int i = 0; i < 5; ++i) {
+    for (int j = 0; j < 14; ++j)
+      if (meet(written[i], read[j]) && !(i == 0 && ((j == 0 && on_x) || (j == 1 && on_res))))
+        return refuse(err, err_len, MOE_EINVAL, "%s: an output overlaps an input (only x or residual may be out itself)", me);
+    for (int j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return refuse(err, err_len, MOE_EINVAL, "%s: two outputs overlap", me);
+  }
+  char* w = static_cast<char*>(d->workspace_dev);
+  moe::dense::MoeArgs a{};
+  a.x = static_cast<const uint16_t*>(d->x_dev);
+  a.router_w = static_cast<const uint16_t*>(d->router_w_dev);
+  a.logits = d->logits_dev ? static_cast<uint16_t*>(d->logits_dev) : reinterpret_cast<uint16_t*>(w + ws.logits);
+  a.ids_in = d->ids_dev;
+  a.w_in = static_cast<const uint16_t*>(d->weights_dev);
+  a.mask = d->offload_mask_dev;
+  a.gate = static_cast<const uint16_t*>(d->gate_dev);
+  a.up = static_cast<const uint16_t*>(d->up_dev);
+  a.down = static_cast<const uint16_t*>(d->down_dev);
+  if (shared) {
+    a.shared_gate = static_cast<const uint16_t*>(d->shared_gate_dev);
+    a.shared_up = static_cast<const uint16_t*>(d->shared_up_dev);
+    a.shared_down = static_cast<const uint16_t*>(d->shared_down_dev);
+    a.shared_gate_vec = static_cast<const uint16_t*>(d->shared_gate_vec_dev);
+  }
+  a.res = static_cast<const uint16_t*>(d->residual_dev);
+  a.out = static_cast<uint16_t*>(d->out_dev);
+  a.ids_out = d->ids_out_dev;
+  a.w_out = static_cast<uint16_t*>(d->weights_out_dev);
+  a.bar = reinterpret_cast<unsigned long long*>(w + ws.bar);
+  a.shared_open = reinterpret_cast<float*>(w + ws.open);
+  a.h = reinterpret_cast<uint16_t*>(w + ws.h);
+  a.h_shared = reinterpret_cast<uint16_t*>(w + ws.h_shared);
+  a.ldx = d->ldx;
+  a.ldr = d->ldr;
+  a.ldo = d->ldo;
+  a.tokens = d->num_tokens;
+  a.experts = d->num_experts;
+  a.top_k = d->top_k;
+  a.hidden = d->hidden_size;
+  a.inter = d->inter_size;
+  a.shared_inter = static_cast<int>(S);
+  a.use_softmax = d->router_use_softmax != 0;
+  a.renorm = d->normalize_topk_prob != 0;
+  const int sms = sm_count();
+  if (sms < 1) return refuse(err, err_len, MOE_ECUDA, "%s: no device", me);
+  const cudaError_t e = moe::dense::launch_dense_moe(a, d->dtype, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "%s: %s", me, cudaGetErrorString(e));
+  return MOE_OK;
+}
+
+int moe_dense_read_status(int32_t* status, void* stream, char* err, size_t err_len) {
+  if (status == nullptr) return refuse(err, err_len, MOE_EINVAL, "moe_dense_read_status: null argument");
+  int v = 0;
+  const cudaError_t e = moe::dense::read_dense_status(&v, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "moe_dense_read_status: %s", cudaGetErrorString(e));
+  *status = v;
   return MOE_OK;
 }
 

@@ -1,11 +1,13 @@
 // dense_linear.cu — dense projections out = act(x W^T + b) + r and the gated
-// product act(x Wg^T) * (x Wu^T): the kernel for every shape and alignment.
+// product act(x Wg^T) * (x Wu^T): the kernel for every shape and alignment,
+// and the weight-streaming kernel for a few tokens.
 //
 // The reference computes these with nn.Linear modules: the dense decoder
 // layer's and the GPU-resident experts' w2(silu(w1 x) * w3 x)
 // (nano_ktrans/layers/expert_mlp.py:9-25) and the router
 // (nano_ktrans/models/mixtral.py:127).
-#include "dense_common.cuh"
+#include "dense_stream.cuh"
+#include "kernels.h"
 
 namespace moe {
 namespace dense {
@@ -87,6 +89,123 @@ static cudaError_t generic(const LinearArgs& a, cudaStream_t st) {
 
 cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
   return dtype == MOE_DTYPE_FP16 ? generic<Fp16>(a, st) : generic<Bf16>(a, st);
+}
+
+// ---------------------------------------------------------------------------
+// A few tokens: weight rows streamed past the token columns (dense_stream.cuh).
+// One block per SM; block c owns features [n c / G, n (c + 1) / G), so the SMs
+// have the same number of rows to within one.  A plain tile is 16 features; a
+// gated tile is 8 gate rows (mma rows 0-7) and the same 8 up rows (mma rows
+// 8-15), so gate and up of a feature meet in one thread.
+// ---------------------------------------------------------------------------
+template <typename T, bool GATED, int NT, int VEC>
+struct LinearSrc {
+  const LinearArgs& a;
+  int r0, r1, g, t;
+  const uint16_t* xrow[NT];
+  MOE_DEV LinearSrc(const LinearArgs& args, int lo, int hi) : a(args), r0(lo), r1(hi) {
+    const int lane = threadIdx.x & 31;
+    g = lane >> 2;
+    t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.m ? a.x + (8 * j + g) * a.ldx : nullptr;
+  }
+  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[VEC / 2], uint32_t (&fb)[VEC / 2]) const {
+    const int k = unit * 4 * VEC + t * VEC;
+    if constexpr (GATED) {
+      const int r = r0 + 8 * tile + g;
+      if (r < r1 && k < a.k) {
+        ld_weights(fa, a.w + r * a.ldw + k);
+        ld_weights(fb, a.w_up + r * a.ldwu + k);
+      } else {
+        zero(fa);
+        zero(fb);
+      }
+    } else {
+      const int r = r0 + 16 * tile + g;
+      if (r < r1 && k < a.k) ld_weights(fa, a.w + r * a.ldw + k);
+      else zero(fa);
+      if (r + 8 < r1 && k < a.k) ld_weights(fb, a.w + (r + 8) * a.ldw + k);
+      else zero(fb);
+    }
+  }
+  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[VEC / 2]) const {
+    const int k = unit * 4 * VEC + t * VEC;
+    if (xrow[j] != nullptr && k < a.k) ld_tokens(x, xrow[j] + k);
+    else zero(x);
+  }
+};
+
+template <typename T, bool GATED, int NT, int VEC>
+__global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __grid_constant__ LinearArgs a) {
+  extern __shared__ float part[];
+  // A launch that may start early reads nothing before its predecessor is done
+  // (weights too: they may be that kernel's output), and lets none start early.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int r0 = static_cast<int>(static_cast<int64_t>(a.n) * blockIdx.x / gridDim.x);
+  const int r1 = static_cast<int>(static_cast<int64_t>(a.n) * (blockIdx.x + 1) / gridDim.x);
+  constexpr int kRows = GATED ? 8 : 16, kD = VEC == 16 ? 4 : 6;
+  const int tiles = (r1 - r0 + kRows - 1) / kRows, units = (a.k + 4 * VEC - 1) / (4 * VEC);
+  const LinearSrc<T, GATED, NT, VEC> src(a, r0, r1);
+  Streamer<T, NT, VEC, kD, kRows> s;
+  s.prologue(src, tiles, units);
+  s.run(src, tiles, units, a.m, [&](int tile, int row, int col, auto sum) {
+    const int n = r0 + kRows * tile + row;
+    if (n >= r1) return;
+    float v = sum(row, col);
+    if constexpr (GATED) {
+      v = activate_rt(a.act, v) * sum(row + 8, col);
+    } else {
+      if (a.bias) v += T::to_f32(a.bias[n]);
+      v = activate_rt(a.act, v);
+      if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
+    }
+    a.out[col * a.ldo + n] = T::from_f32(v);
+  }, part);
+}
+
+template <typename T, bool GATED, int NT, int VEC>
+static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) {
+  const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT, VEC>);
+  if (!ensure_dynamic_smem(kern, part_bytes<NT>(), kSThreads)) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.n < sms ? a.n : sms);
+  cfg.blockDim = dim3(kSThreads);
+  cfg.dynamicSmemBytes = part_bytes<NT>();
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, stream_linear_kernel<T, GATED, NT, VEC>, a);
+}
+
+template <typename T, bool GATED, int NT>
+static cudaError_t stream_vec(const LinearArgs& a, int vec, int sms, cudaStream_t st) {
+  return vec == 16 ? stream_launch<T, GATED, NT, 16>(a, sms, st) : stream_launch<T, GATED, NT, 8>(a, sms, st);
+}
+
+template <typename T, bool GATED>
+static cudaError_t stream_cols(const LinearArgs& a, int vec, int sms, cudaStream_t st) {
+  return a.m <= 8 ? stream_vec<T, GATED, 1>(a, vec, sms, st)
+         : a.m <= 16 ? stream_vec<T, GATED, 2>(a, vec, sms, st)
+                     : stream_vec<T, GATED, 4>(a, vec, sms, st);
+}
+
+int wide_elements(const LinearArgs& a) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) |
+                      reinterpret_cast<uintptr_t>(a.w_up);
+  // a single row has no stride to respect
+  const int64_t l = (a.m > 1 ? a.ldx : 0) | (a.n > 1 ? a.ldw : 0) | (a.n > 1 && a.w_up ? a.ldwu : 0) | a.k;
+  return p % 32 == 0 && l % 16 == 0 ? 16 : p % 16 == 0 && l % 8 == 0 ? 8 : 0;
+}
+
+cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaStream_t st) {
+  const int vec = wide_elements(a);
+  if (dtype == MOE_DTYPE_FP16)
+    return a.w_up ? stream_cols<Fp16, true>(a, vec, sms, st) : stream_cols<Fp16, false>(a, vec, sms, st);
+  return a.w_up ? stream_cols<Bf16, true>(a, vec, sms, st) : stream_cols<Bf16, false>(a, vec, sms, st);
 }
 
 }  // namespace dense

@@ -1,0 +1,440 @@
+// dense_moe.cu — a whole mixture-of-experts layer on unquantised bf16 / fp16
+// expert weights for a few tokens, in two kernels.
+//
+// The reference's MoE block (nano_ktrans/models/mixtral.py:212-218) with
+// GPU-resident experts: router nn.Linear, routing
+// (layers/hybrid_moe.py:3321-3329), the per-expert module loop with its host
+// reads of the routed ids (:3501-3533) or the batch-1 stacked bmm
+// (:3442-3500), weighted sum, shared expert, and the decoder layer's residual.
+//
+//   l     = round(x Wr^T);  ids, w = top-k of l as the router kernel ranks it
+//   h_te  = w_te * silu(x_t G_e^T) * (x_t U_e^T)            (fp32)
+//   out_t = round(r_t + sum_e D_e h_te + D_s h_ts),  h_ts weighted by sigmoid(x_t . g_s)
+//
+// With the weight inside h the weighted sum over experts is part of the down
+// projection's K loop: out = [D_e1 | D_e2 | ...] [h_e1; h_e2; ...], one
+// accumulator per output.  h is kept as hi + lo, two values of the layer's
+// type (hi = round(h), lo = round(h - hi): relative error 2^-16 for bf16,
+// 2^-22 for fp16), each a token column of its own: the tensor cores have room,
+// since the kernel is bound by reading each routed expert's weights once.
+//
+// dense_router_kernel: one block per expert, logits of all tokens; one more
+// block for the shared expert's gate; zeroes the grid barrier of the call.
+// dense_moe_kernel: one block per SM, cooperative.  Every block routes all
+// tokens by itself (one warp a token) and lists the routed experts in
+// ascending order; then the gate / up rows of all of them, and after one grid
+// barrier the output rows, are split evenly over the blocks by rows and
+// streamed (dense_stream.cuh).  The first down-projection steps are loaded
+// before the barrier, so its latency passes with 128 KB per SM in flight.
+#include "async_copy.cuh"
+#include "dense_stream.cuh"
+#include "kernels.h"
+
+namespace moe {
+namespace dense {
+
+__device__ int g_dense_status;  // kStatus* bits of this device's dense calls since the last read
+
+constexpr int kRouterThreads = 128;
+
+// Block e < num_experts: logits[t][e]; block num_experts: the shared gate.
+template <typename T>
+__global__ void __launch_bounds__(kRouterThreads) dense_router_kernel(const __grid_constant__ MoeArgs a) {
+  __shared__ float part[kRouterThreads / 32][kMoeTokens];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (blockIdx.x == 0 && tid == 0) *a.bar = 0;
+  const int e = a.router_w ? blockIdx.x : a.experts;  // without a projection the only block is the gate's
+  const uint16_t* w = e < a.experts ? a.router_w + static_cast<int64_t>(e) * a.hidden : a.shared_gate_vec;
+  if (w == nullptr) return;
+  float acc[kMoeTokens];
+#pragma unroll
+  for (int t = 0; t < kMoeTokens; ++t) acc[t] = 0.0f;
+  for (int k = tid * 16; k < a.hidden; k += kRouterThreads * 16) {
+    uint32_t wv[8];
+    ld_weights(wv, w + k);
+#pragma unroll
+    for (int t = 0; t < kMoeTokens; ++t)
+      if (t < a.tokens) {
+        uint32_t xv[8];
+        ld_tokens(xv, a.x + t * a.ldx + k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 p = T::unpack(wv[i]), q = T::unpack(xv[i]);
+          acc[t] = fmaf(p.x, q.x, acc[t]);
+          acc[t] = fmaf(p.y, q.y, acc[t]);
+        }
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < kMoeTokens; ++t)
+    if (t < a.tokens) {
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) acc[t] += __shfl_xor_sync(kFullMask, acc[t], off);
+      if (lane == 0) part[warp][t] = acc[t];
+    }
+  __syncthreads();
+  if (tid < a.tokens) {
+    const float v = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    if (e < a.experts) a.logits[tid * a.experts + e] = T::from_f32(v);
+    else a.shared_open[tid] = sigmoid_f32(v);
+  }
+}
+
+// Order-preserving 16-bit image of a 16-bit float: NaN on top, -0 equal to +0.
+template <typename T>
+MOE_DEV uint32_t key16(float v) {
+  if (isnan(v)) return 0xffffu;
+  uint32_t b = T::from_f32(v);
+  if (b == 0x8000u) b = 0;
+  return (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+}
+template <typename T>
+MOE_DEV float key16_value(uint32_t k) {
+  return T::to_f32(static_cast<uint16_t>((k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu)));
+}
+
+// One warp routes one token: lane j < top_k returns the j-th pick.  keys: this
+// warp's scratch of `E` words.  Values are rounded to the layer's type before
+// they are ranked, equal ones go to the lowest expert.
+template <typename T>
+MOE_DEV void route_warp(const uint16_t* row, const MoeArgs& a, uint32_t* keys, int& id, float& wt) {
+  const int lane = threadIdx.x & 31, E = a.experts;
+  float m = -INFINITY, s = 0.0f;
+  if (a.use_softmax) {
+    for (int e = lane; e < E; e += 32) {
+      const float v = T::to_f32(__ldcg(row + e));
+      keys[e] = __float_as_uint(v);
+      m = fmaxf(m, v);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
+    for (int e = lane; e < E; e += 32) {
+      const float p = expf(__uint_as_float(keys[e]) - m);
+      keys[e] = __float_as_uint(p);
+      s += p;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
+    for (int e = lane; e < E; e += 32)
+      keys[e] = (key16<T>(__uint_as_float(keys[e]) / s) << 16) | static_cast<uint32_t>(0xffff - e);
+  } else {
+    for (int e = lane; e < E; e += 32)
+      keys[e] = (key16<T>(T::to_f32(__ldcg(row + e))) << 16) | static_cast<uint32_t>(0xffff - e);
+  }
+  float val = 0.0f, sum = 0.0f, v0 = 0.0f, exsum = 0.0f;
+  id = -1;
+  for (int j = 0; j < a.top_k; ++j) {
+    uint32_t best = 0;
+    for (int e = lane; e < E; e += 32) best = max(best, keys[e]);
+    best = __reduce_max_sync(kFullMask, best);
+    const int e = 0xffff - static_cast<int>(best & 0xffffu);
+    if ((e & 31) == lane) keys[e] = 0;  // valid keys are never 0; each lane reads back only its own words
+    const float v = key16_value<T>(best >> 16);
+    if (lane == j) {
+      val = v;
+      id = e;
+    }
+    sum += v;
+    if (j == 0) v0 = v;
+    if (!a.use_softmax) exsum += expf(v - v0);
+  }
+  if (a.use_softmax)
+    wt = a.renorm ? val / T::to_f32(T::from_f32(sum)) : val;
+  else
+    wt = expf(val - v0) / exsum;
+  wt = T::to_f32(T::from_f32(wt));
+}
+
+// Routing tables of a call, in shared memory.
+struct Tables {
+  int16_t pair[kMoePairs][kMoeTokens];  // [active expert][token]: t * top_k + slot, -1 when not routed there
+  float weight[kMoePairs][kMoeTokens];
+  int active[kMoePairs];                // routed experts, ascending
+  int id[kMoeTokens][kMoeTopK];
+  float w[kMoeTokens][kMoeTopK];
+  int n_active;
+  int ok;
+};
+
+// Gate and up rows of the routed experts, then of the shared expert, as one
+// list of rows; `lo` to `hi` are this block's.  Tile i is the list's group of
+// 8 rows number lo / 8 + i (a group never spans two experts: their sizes are
+// multiples of 16), rows outside the block's range masked.
+template <typename T, int NT>
+struct GateUpSrc {
+  const MoeArgs& a;
+  const Tables& tb;
+  int lo, hi, routed, g, t;
+  const uint16_t* xrow[NT];
+  MOE_DEV GateUpSrc(const MoeArgs& args, const Tables& tables, int lo_, int hi_)
+      : a(args), tb(tables), lo(lo_), hi(hi_), routed(tables.n_active * args.inter) {
+    const int lane = threadIdx.x & 31;
+    g = lane >> 2;
+    t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx : nullptr;
+  }
+  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[8], uint32_t (&fb)[8]) const {
+    const int k = unit * 64 + t * 16, v0 = (lo / 8 + tile) * 8, v = v0 + g;
+    if (v < lo || v >= hi || k >= a.hidden) {
+      zero(fa);
+      zero(fb);
+      return;
+    }
+    if (v0 < routed) {
+      const int s = v0 / a.inter;
+      const int64_t row = static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter);
+      ld_weights(fa, a.gate + row * a.hidden + k);
+      ld_weights(fb, a.up + row * a.hidden + k);
+    } else {
+      const int64_t row = v - routed;
+      ld_weights(fa, a.shared_gate + row * a.hidden + k);
+      ld_weights(fb, a.shared_up + row * a.hidden + k);
+    }
+  }
+  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[8]) const {
+    const int k = unit * 64 + t * 16;
+    if (xrow[j] != nullptr && k < a.hidden) ld_tokens(x, xrow[j] + k);
+    else zero(x);
+  }
+};
+
+// Output rows [r0, r1); K runs over the routed experts' h, then the shared
+// expert's.  Columns: hi of token c for c < half, then lo of token c - half.
+template <typename T, int NT>
+struct DownSrc {
+  static constexpr int kHalf = 4 * NT;
+  const MoeArgs& a;
+  const Tables& tb;
+  int r0, r1, ue, routed_units, g, t;
+  MOE_DEV DownSrc(const MoeArgs& args, const Tables& tables, int lo, int hi) : a(args), tb(tables), r0(lo), r1(hi) {
+    const int lane = threadIdx.x & 31;
+    g = lane >> 2;
+    t = lane & 3;
+    ue = (a.inter + 63) / 64;
+    routed_units = tables.n_active * ue;
+  }
+  MOE_DEV int units() const { return routed_units + (a.shared_inter + 63) / 64; }
+  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[8], uint32_t (&fb)[8]) const {
+    const int r = r0 + 16 * tile + g;
+    const uint16_t* base;
+    int k, len;
+    if (unit < routed_units) {
+      const int s = unit / ue;
+      k = (unit - s * ue) * 64 + t * 16;
+      len = a.inter;
+      base = a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter;
+    } else {
+      k = (unit - routed_units) * 64 + t * 16;
+      len = a.shared_inter;
+      base = a.shared_down;
+    }
+    if (r < r1 && k < len) ld_weights(fa, base + static_cast<int64_t>(r) * len + k);
+    else zero(fa);
+    if (r + 8 < r1 && k < len) ld_weights(fb, base + static_cast<int64_t>(r + 8) * len + k);
+    else zero(fb);
+  }
+  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[8]) const {
+    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf;
+    const uint16_t* p = nullptr;
+    if (tok < a.tokens) {
+      if (unit < routed_units) {
+        const int s = unit / ue, k = (unit - s * ue) * 64 + t * 16, pair = tb.pair[s][tok];
+        if (pair >= 0 && k < a.inter) p = a.h + static_cast<int64_t>(2 * pair + part) * a.inter + k;
+      } else {
+        const int k = (unit - routed_units) * 64 + t * 16;
+        if (k < a.shared_inter) p = a.h_shared + static_cast<int64_t>(2 * tok + part) * a.shared_inter + k;
+      }
+    }
+    if (p != nullptr) ld_l2(x, p);
+    else zero(x);
+  }
+};
+
+// h = hi + lo in the layer's type.  An h beyond fp16's range stays infinite.
+template <typename T>
+MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
+  const uint16_t b = T::from_f32(h);
+  const float rest = h - T::to_f32(b);
+  *hi = b;
+  *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
+}
+
+// NT column tiles hold the tokens of the gate / up phase, ND those of the down phase (hi and lo).
+template <typename T, int NT, int ND>
+__global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
+  extern __shared__ float part[];
+  __shared__ Tables tb;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- routing, in every block ----
+  uint32_t* keys = reinterpret_cast<uint32_t*>(part);  // [16][E] words, then used[E] bytes: before the partials are
+  uint8_t* used = reinterpret_cast<uint8_t*>(keys + kMoeTokens * a.experts);
+  for (int i = tid; i < a.experts; i += kSThreads) used[i] = 0;
+  for (int i = tid; i < kMoePairs * kMoeTokens; i += kSThreads) {
+    (&tb.pair[0][0])[i] = -1;
+    (&tb.weight[0][0])[i] = 0.0f;
+  }
+  __syncthreads();
+  if (warp < a.tokens) {
+    int id = -1;
+    float wt = 0.0f;
+    if (a.ids_in == nullptr) {
+      route_warp<T>(a.logits + warp * a.experts, a, keys + warp * a.experts, id, wt);
+    } else if (lane < a.top_k) {
+      const int64_t given = a.ids_in[warp * a.top_k + lane];
+      wt = T::to_f32(a.w_in[warp * a.top_k + lane]);
+      id = given >= 0 && given < a.experts ? static_cast<int>(given) : -1;
+      if (given >= a.experts && blockIdx.x == 0) atomicOr(&g_dense_status, kStatusBadExpertId);
+    }
+    if (lane < a.top_k) {
+      if (blockIdx.x == 0 && a.ids_in == nullptr) {
+        if (a.ids_out) a.ids_out[warp * a.top_k + lane] = id;
+        if (a.w_out) a.w_out[warp * a.top_k + lane] = T::from_f32(wt);
+      }
+      if (id >= 0 && a.mask != nullptr && a.mask[id] == 0) id = -1;
+      if (id >= 0) used[id] = 1;
+      tb.id[warp][lane] = id;
+      tb.w[warp][lane] = wt;
+    }
+  }
+  __syncthreads();
+  int16_t* slot = reinterpret_cast<int16_t*>(keys);  // [E] place of an expert in the active list
+  if (warp == 0) {
+    int n = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const bool on = e0 + lane < a.experts && used[e0 + lane] != 0;
+      const uint32_t b = __ballot_sync(kFullMask, on);
+      if (on) {
+        const int s = n + __popc(b & ((1u << lane) - 1u));
+        tb.active[s] = e0 + lane;
+        slot[e0 + lane] = static_cast<int16_t>(s);
+      }
+      n += __popc(b);
+    }
+    if (lane == 0) tb.n_active = n;
+    __syncwarp();
+    if (lane < a.tokens)
+      for (int j = 0; j < a.top_k; ++j) {  // an expert given twice for a token counts with both weights
+        const int id = tb.id[lane][j];
+        if (id < 0) continue;
+        const int s = slot[id];
+        if (tb.pair[s][lane] < 0) tb.pair[s][lane] = static_cast<int16_t>(lane * a.top_k + j);
+        tb.weight[s][lane] += tb.w[lane][j];
+      }
+  }
+  __syncthreads();
+
+  // ---- h = w silu(gate) up ----
+  const int64_t rows = static_cast<int64_t>(tb.n_active) * a.inter + a.shared_inter;
+  const int lo = static_cast<int>(rows * blockIdx.x / gridDim.x), hi = static_cast<int>(rows * (blockIdx.x + 1) / gridDim.x);
+  {
+    const GateUpSrc<T, NT> src(a, tb, lo, hi);
+    const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0, units = (a.hidden + 63) / 64;
+    Streamer<T, NT, 16, 4, 8> s;
+    s.prologue(src, tiles, units);
+    s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
+      const int v0 = (lo / 8 + tile) * 8, v = v0 + row;
+      if (v < lo || v >= hi) return;
+      if (v0 < src.routed) {
+        const int e = v0 / a.inter, pair = tb.pair[e][col];
+        if (pair < 0) return;
+        const float h = tb.weight[e][col] * (silu_f32(sum(row, col)) * sum(row + 8, col));
+        uint16_t* p = a.h + static_cast<int64_t>(2 * pair) * a.inter + (v - e * a.inter);
+        store_split<T>(p, p + a.inter, h);
+      } else {
+        const float h = __ldcg(a.shared_open + col) * (silu_f32(sum(row, col)) * sum(row + 8, col));
+        uint16_t* p = a.h_shared + static_cast<int64_t>(2 * col) * a.shared_inter + (v - src.routed);
+        store_split<T>(p, p + a.shared_inter, h);
+      }
+    }, part);
+  }
+
+  // ---- out = r + sum over experts of D h ----
+  const int r0 = static_cast<int>(static_cast<int64_t>(a.hidden) * blockIdx.x / gridDim.x);
+  const int r1 = static_cast<int>(static_cast<int64_t>(a.hidden) * (blockIdx.x + 1) / gridDim.x);
+  const DownSrc<T, ND> src(a, tb, r0, r1);
+  const int tiles = (r1 - r0 + 15) / 16, units = src.units();
+  Streamer<T, ND, 16, 4, 16> s;
+  s.prologue(src, units > 0 ? tiles : 0, units > 0 ? units : 1);  // weights only: they do not wait for h
+  if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
+    if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
+    return;
+  }
+  auto store = [&](int n, int col, float v) {
+    if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
+    a.out[col * a.ldo + n] = T::from_f32(v);
+  };
+  if (units == 0) {  // every expert masked and no shared expert
+    for (int i = tid; i < (r1 - r0) * a.tokens; i += kSThreads) store(r0 + i % (r1 - r0), i / (r1 - r0), 0.0f);
+    return;
+  }
+  s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
+    const int n = r0 + 16 * tile + row;
+    if (n < r1) store(n, col, sum(row, col) + sum(row, col + 4 * ND));
+  }, part);
+}
+
+size_t moe_part_bytes(int experts) {
+  const size_t route = sizeof(uint32_t) * kMoeTokens * experts + experts;
+  const size_t stream = part_bytes<1>();  // the same for 1, 2 and 4 column tiles
+  static_assert(part_bytes<1>() == part_bytes<2>() && part_bytes<1>() == part_bytes<4>(), "one size for every plan");
+  return route > stream ? route : stream;
+}
+
+template <typename T, int NT, int ND>
+static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
+  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND>);
+  const size_t smem = moe_part_bytes(a.experts);
+  if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(sms);
+  cfg.blockDim = dim3(kSThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, NT, ND>, a);
+}
+
+template <typename T>
+static cudaError_t moe_both(const MoeArgs& a, int sms, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.router_w ? a.experts + (a.shared_gate_vec ? 1 : 0) : 1);
+  cfg.blockDim = dim3(kRouterThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, dense_router_kernel<T>, a);
+  if (e != cudaSuccess) return e;
+  if (a.tokens <= 4) return moe_main<T, 1, 1>(a, sms, st);
+  if (a.tokens <= 8) return moe_main<T, 1, 2>(a, sms, st);
+  return moe_main<T, 2, 4>(a, sms, st);
+}
+
+cudaError_t launch_dense_moe(const MoeArgs& a, int dtype, int sms, cudaStream_t st) {
+  return dtype == MOE_DTYPE_FP16 ? moe_both<Fp16>(a, sms, st) : moe_both<Bf16>(a, sms, st);
+}
+
+cudaError_t read_dense_status(int* status, cudaStream_t st) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_dense_status);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e;
+}
+
+}  // namespace dense
+}  // namespace moe

@@ -40,10 +40,11 @@ def _stream_on(device_index: int, stream) -> int:
 def _empty_on(shape, dtype, device, stream) -> torch.Tensor:
     """A new tensor that belongs to the stream the kernels run on: allocated for another
     stream, its memory could be handed out again while they still write it."""
-    if stream is None:
+    if stream is None or _stream_on(device.index, stream) == torch._C._cuda_getCurrentRawStream(device.index):
         return torch.empty(shape, dtype=dtype, device=device)
-    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=device)
-    with torch.cuda.stream(s):
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 

@@ -1,0 +1,162 @@
+"""``DenseMoeLayer``: a whole mixture-of-experts layer on unquantised weights, for a few tokens.
+
+The reference's MoE block with GPU-resident experts (nano_ktrans/models/mixtral.py:212-218,
+layers/hybrid_moe.py:3321-3329, :3442-3533): router projection, routing, gated experts, weighted
+sum, shared expert and the decoder layer's residual, in two kernel launches and without a host
+read.  ``MoeLayer`` is its counterpart on quantised weights.
+
+The layer borrows its weight tensors and keeps no other state: every call takes its workspace from
+the caching allocator of the stream it runs on, so calls on several streams are independent.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .dense import _DTYPES, _empty_on, _err_buffer, _stream_on
+
+MAX_TOKENS = _lib.DENSE_MAX_TOKENS
+
+
+class DenseMoeLayer:
+    """``gate`` / ``up`` [E, I, H], ``down`` [E, H, I] (bf16 or fp16, contiguous, on one CUDA device; H and I
+    multiples of 16); ``shared``: ``{"gate", "up": [S, H], "down": [H, S], "gate_vec": [H]}`` or None."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *, top_k: int,
+                 router_use_softmax: bool = True, normalize_topk_prob: bool = True, shared: Optional[dict] = None):
+        if gate.dim() != 3 or up.shape != gate.shape or down.shape != (gate.shape[0], gate.shape[2], gate.shape[1]):
+            raise ValueError(f"gate and up must be [E, I, H] and down [E, H, I], got {tuple(gate.shape)}, "
+                             f"{tuple(up.shape)}, {tuple(down.shape)}")
+        if gate.dtype not in _DTYPES or not gate.is_cuda:
+            raise ValueError(f"expert weights must be bf16 or fp16 CUDA tensors, got {gate.dtype} on {gate.device}")
+        self.num_experts, self.inter_size, self.hidden_size = gate.shape
+        self.dtype, self.device, self._dev = gate.dtype, gate.device, gate.get_device()
+        self.top_k = int(top_k)
+        self.router_use_softmax, self.normalize_topk_prob = bool(router_use_softmax), bool(normalize_topk_prob)
+        self.gate, self.up, self.down = gate, up, down
+        self.shared = dict(shared) if shared is not None else None
+        self.shared_inter = 0
+        h = self.hidden_size
+        named = [("gate", gate), ("up", up), ("down", down)]
+        if shared is not None:
+            s = self.shared_inter = int(shared["gate"].shape[0])
+            for name, shape in (("gate", (s, h)), ("up", (s, h)), ("down", (h, s)), ("gate_vec", (h,))):
+                if tuple(shared[name].shape) != shape or s < 1:
+                    raise ValueError(f"shared {name} must be {shape}, got {tuple(shared[name].shape)}")
+                named.append((f"shared {name}", shared[name]))
+        for name, w in named:
+            if w.dtype is not gate.dtype or w.device != gate.device or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {gate.dtype} tensor on {gate.device}")
+        ptr = (lambda n: self.shared[n].data_ptr()) if self.shared is not None else (lambda n: None)
+        self._desc = _lib.MoeDenseDesc(gate.data_ptr(), up.data_ptr(), down.data_ptr(), ptr("gate"), ptr("up"),
+                                       ptr("down"), ptr("gate_vec"), self.num_experts, self.top_k, h,
+                                       self.inter_size, self.shared_inter, int(self.router_use_softmax),
+                                       int(self.normalize_topk_prob), _DTYPES[gate.dtype])
+        self._space = []  # workspace bytes by token count
+        err = _err_buffer()
+        for t in range(MAX_TOKENS + 1):
+            self._desc.num_tokens = t
+            n = ctypes.c_int64(0)
+            rc = _lib.lib().moe_dense_workspace(ctypes.byref(self._desc), ctypes.byref(n), err, 512)
+            if rc != _lib.MOE_OK:
+                raise _lib.MoeError(rc, err.value.decode(errors="replace"))
+            self._space.append(n.value)
+        self._layer_bytes = bytes(self._desc)
+
+    # ------------------------------------------------------------------
+    def _rows(self, t: torch.Tensor, name: str, rows: Optional[int], cols: int) -> int:
+        """Row stride of a [rows, cols] tensor of the layer's type, after its checks."""
+        if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+            raise ValueError(f"{name} must be [{'T' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
+        if t.dtype is not self.dtype or t.get_device() != self._dev:
+            raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
+        ld, inner = t.stride()
+        if inner != 1:
+            raise ValueError(f"{name} must have unit stride along its rows")
+        return ld if t.shape[0] > 1 else cols
+
+    def _exact(self, t: torch.Tensor, name: str, shape: tuple, dtype) -> int:
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != self._dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {self.device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def _run(self, x, residual, out, offload_mask, add_shared, stream, *, router=None, logits=None, ids=None,
+             weights=None, out_ids=None, out_weights=None) -> torch.Tensor:
+        ldx = self._rows(x, "x", None, self.hidden_size)
+        t = x.shape[0]
+        d = _lib.MoeDenseDesc.from_buffer_copy(self._layer_bytes)
+        d.x_dev, d.ldx, d.num_tokens, d.add_shared = x.data_ptr(), ldx, t, add_shared
+        if router is not None:
+            d.router_w_dev = self._exact(router, "router_weight", (self.num_experts, self.hidden_size), self.dtype)
+        if logits is not None:
+            d.logits_dev = self._exact(logits, "router logits", (t, self.num_experts), self.dtype)
+        routing = (t, self.top_k)
+        if ids is not None:
+            d.ids_dev = self._exact(ids, "topk_ids", routing, torch.int64)
+            d.weights_dev = self._exact(weights, "topk_weights", routing, self.dtype)
+        if out_ids is not None:
+            d.ids_out_dev = self._exact(out_ids, "out_ids", routing, torch.int64)
+        if out_weights is not None:
+            d.weights_out_dev = self._exact(out_weights, "out_weights", routing, self.dtype)
+        if offload_mask is not None:
+            if offload_mask.dtype not in (torch.bool, torch.uint8):
+                raise ValueError(f"offload_mask must be bool or uint8, got {offload_mask.dtype}")
+            d.offload_mask_dev = self._exact(offload_mask, "offload_mask", (self.num_experts,), offload_mask.dtype)
+        if residual is not None:
+            d.ldr = self._rows(residual, "residual", t, self.hidden_size)
+            d.residual_dev = residual.data_ptr()
+        if out is None:
+            out = _empty_on((t, self.hidden_size), self.dtype, self.device, stream)
+        d.ldo = self._rows(out, "out", t, self.hidden_size)
+        d.out_dev = out.data_ptr()
+        if t == 0:
+            return out
+        ws = None
+        if t <= MAX_TOKENS:
+            n = d.workspace_bytes = self._space[t]
+            ws = _empty_on(n, torch.uint8, self.device, stream)
+            d.workspace_dev = ws.data_ptr()
+        err = _err_buffer()
+        if self._dev == torch.cuda.current_device():
+            rc = _lib.lib().moe_dense_forward(ctypes.byref(d), _stream_on(self._dev, stream), err, 512)
+        else:
+            with torch.cuda.device(self._dev):
+                rc = _lib.lib().moe_dense_forward(ctypes.byref(d), _stream_on(self._dev, stream), err, 512)
+        if rc != _lib.MOE_OK:
+            raise _lib.MoeError(rc, err.value.decode(errors="replace"))
+        return out
+
+    def forward_x(self, x: torch.Tensor, router_weight: torch.Tensor, *, residual=None, out=None, out_ids=None,
+                  out_weights=None, out_logits=None, offload_mask=None, add_shared: bool = True,
+                  stream=None) -> torch.Tensor:
+        """The layer from hidden states ``x`` [T, H], T <= 16: routes from ``x @ router_weight.T`` (rounded to the
+        layer's type; ``out_logits`` receives it), returns ``residual +`` the layer's output, rounded once.  ``out``
+        may be ``x`` or ``residual`` itself."""
+        return self._run(x, residual, out, offload_mask, add_shared, stream, router=router_weight, logits=out_logits,
+                         out_ids=out_ids, out_weights=out_weights)
+
+    def forward(self, x: torch.Tensor, router_logits: torch.Tensor, *, residual=None, out=None, out_ids=None,
+                out_weights=None, offload_mask=None, add_shared: bool = True, stream=None) -> torch.Tensor:
+        """The layer from given router logits [T, E]."""
+        return self._run(x, residual, out, offload_mask, add_shared, stream, logits=router_logits, out_ids=out_ids,
+                         out_weights=out_weights)
+
+    def experts_forward(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor, *, residual=None,
+                        out=None, offload_mask=None, add_shared: bool = False, stream=None) -> torch.Tensor:
+        """The experts on a given routing: ids [T, top_k] int64, negative ones mean no expert."""
+        return self._run(x, residual, out, offload_mask, add_shared, stream, ids=topk_ids, weights=topk_weights)
+
+    __call__ = forward
+
+    def read_status(self, stream=None) -> int:
+        """Status bits (as ``MoeLayer.read_status``) of the device's dense calls since the last read; synchronises."""
+        st, err = ctypes.c_int32(0), _err_buffer()
+        with torch.cuda.device(self._dev):
+            rc = _lib.lib().moe_dense_read_status(ctypes.byref(st), _stream_on(self._dev, stream), err, 512)
+        if rc != _lib.MOE_OK:
+            raise _lib.MoeError(rc, err.value.decode(errors="replace"))
+        return int(st.value)

@@ -70,3 +70,71 @@ def test_dense_mlp_checks_its_shapes():
         DenseMLP(g, g, g)
     mlp = DenseMLP(g, g, g.t())
     assert (mlp.hidden_size, mlp.intermediate_size) == (4, 8)
+
+
+def moe_desc(**kw):
+    from nano_ktrans_b200 import _lib
+
+    # addresses that no call here reaches: every one of these descriptions is refused
+    d = dict(gate_dev=0x100000, up_dev=0x200000, down_dev=0x300000, num_experts=8, top_k=2, hidden_size=64, inter_size=32,
+             shared_inter=0, router_use_softmax=1, normalize_topk_prob=1, dtype=0, x_dev=0x400000, router_w_dev=0x500000,
+             out_dev=0x600000, workspace_dev=0x700000, ldx=64, ldr=64, ldo=64, workspace_bytes=1 << 20, num_tokens=4,
+             add_shared=1)
+    d.update(kw)
+    return _lib.MoeDenseDesc(**d)
+
+
+SHARED = dict(shared_inter=16, shared_gate_dev=0x800000, shared_up_dev=0x810000, shared_down_dev=0x820000,
+              shared_gate_vec_dev=0x830000)
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(dtype=3), "dtype"), (dict(num_experts=0), "num_experts"), (dict(num_experts=1025), "num_experts"),
+    (dict(top_k=0), "top_k"), (dict(top_k=9), "top_k"), (dict(num_experts=32, top_k=17), "top_k"),
+    (dict(hidden_size=40), "hidden_size"), (dict(hidden_size=0), "hidden_size"), (dict(inter_size=8), "inter_size"),
+    (dict(shared_inter=8), "shared_inter"), (dict(num_tokens=-1), "token"), (dict(gate_dev=None), "null"),
+    (dict(x_dev=None), "null"), (dict(workspace_dev=None), "null"), (dict(SHARED, shared_up_dev=None), "shared"),
+    (dict(router_w_dev=None), "no routing"), (dict(ids_dev=0x900000), "given routing"),
+    (dict(ids_dev=0x900000, weights_dev=0x910000), "given routing"),
+    (dict(router_w_dev=None, ids_dev=0x900000, weights_dev=0x910000, ids_out_dev=0x920000), "not written"),
+    (dict(x_dev=0x400010), "32-byte"), (dict(down_dev=0x300008), "32-byte"), (dict(ldx=72), "32-byte"),
+    (dict(SHARED, shared_gate_vec_dev=0x830002), "32-byte"), (dict(out_dev=0x600001), "2-byte"),
+    (dict(ids_out_dev=0x900004), "8-byte"), (dict(ldx=48), "apart"), (dict(ldo=63), "apart"),
+    (dict(residual_dev=0x900000, ldr=32), "apart"), (dict(workspace_dev=0x700010), "workspace"),
+    (dict(workspace_bytes=100), "workspace"), (dict(out_dev=0x400080), "overlaps"), (dict(out_dev=0x100100), "overlaps"),
+    (dict(workspace_dev=0x400000), "overlaps"), (dict(out_dev=0x400000, ldo=80), "overlaps"),
+    (dict(weights_out_dev=0x600000), "two outputs"), (dict(logits_dev=0x600010), "two outputs"),
+    (dict(SHARED, out_dev=0x820000), "overlaps"),
+])
+def test_dense_moe_refuses(lib, kw, needle):
+    from nano_ktrans_b200 import _lib
+
+    err = ctypes.create_string_buffer(256)
+    d = moe_desc(**kw)
+    assert lib.moe_dense_forward(ctypes.byref(d), None, err, len(err)) == _lib.MOE_EINVAL
+    assert needle in err.value.decode(), err.value
+
+
+def test_dense_moe_token_limits_and_workspace(lib):
+    from nano_ktrans_b200 import _lib
+
+    err = ctypes.create_string_buffer(256)
+    n = ctypes.c_int64(-1)
+    assert lib.moe_dense_forward(ctypes.byref(moe_desc(num_tokens=0, x_dev=None)), None, err, len(err)) == _lib.MOE_OK
+    assert lib.moe_dense_forward(ctypes.byref(moe_desc(num_tokens=17)), None, err, len(err)) == _lib.MOE_ERANGE
+    assert lib.moe_dense_workspace(ctypes.byref(moe_desc(num_tokens=17)), ctypes.byref(n), err, len(err)) == _lib.MOE_ERANGE
+    assert lib.moe_dense_workspace(ctypes.byref(moe_desc(**SHARED)), ctypes.byref(n), err, len(err)) == _lib.MOE_OK
+    # barrier, shared gates, logits, both parts of h for every pair and for the shared expert
+    assert n.value >= 8 + 4 * 4 + 2 * 4 * 8 + 4 * 4 * 2 * 32 + 4 * 4 * 16 and n.value % 256 == 0
+    assert lib.moe_dense_workspace(None, ctypes.byref(n), err, len(err)) == _lib.MOE_EINVAL
+    assert lib.moe_dense_read_status(None, None, err, len(err)) == _lib.MOE_EINVAL
+
+
+def test_dense_moe_layer_refuses_host_weights():
+    from nano_ktrans_b200 import DenseMoeLayer
+
+    g, d = torch.zeros(4, 16, 32, dtype=torch.bfloat16), torch.zeros(4, 32, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        DenseMoeLayer(g, g, d, top_k=2)
+    with pytest.raises(ValueError, match="gate and up"):
+        DenseMoeLayer(g, d, d, top_k=2)
