@@ -33,6 +33,10 @@ int wide_elements(const LinearArgs& a);
 constexpr int kStreamTokens = 32;
 cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaStream_t st);
 
+// More tokens than that, wide_elements(a) != 0: tcgen05 kernels.
+cudaError_t launch_gemm(const LinearArgs& a, int dtype, int dev, int sms, cudaStream_t st);
+cudaError_t read_gemm_status(int* status, cudaStream_t st);
+
 // A whole expert layer for up to kMoeTokens tokens.
 constexpr int kMoeTokens = 16;
 constexpr int kMoeTopK = 16;

@@ -33,18 +33,23 @@ Span span(const void* p, int64_t rows, int64_t cols, int64_t ld) {
 }
 bool meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
 
-int sm_count() {
+int sm_count(int* device = nullptr) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (device != nullptr) *device = dev;
   return cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? sms : 0;
 }
 
+// A few tokens are bound by the weights' bytes (streaming kernel); more go to
+// the tensor-core GEMMs.  Rows that no 16-byte load can take, to the generic
+// kernel.
 cudaError_t launch_linear(const LinearArgs& a, int dtype, cudaStream_t st) {
-  const int sms = sm_count();
+  int dev = 0;
+  const int sms = sm_count(&dev);
   if (sms < 1) return cudaErrorInvalidDevice;
   if (moe::dense::wide_elements(a) == 0) return moe::dense::launch_generic(a, dtype, st);
   if (a.m <= moe::dense::kStreamTokens) return moe::dense::launch_stream_linear(a, dtype, sms, st);
-  return moe::dense::launch_generic(a, dtype, st);
+  return moe::dense::launch_gemm(a, dtype, dev, sms, st);
 }
 
 }  // namespace
@@ -261,9 +266,11 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
 int moe_dense_read_status(int32_t* status, void* stream, char* err, size_t err_len) {
   if (status == nullptr) return refuse(err, err_len, MOE_EINVAL, "moe_dense_read_status: null argument");
   int v = 0;
-  const cudaError_t e = moe::dense::read_dense_status(&v, static_cast<cudaStream_t>(stream));
+  int g = 0;
+  cudaError_t e = moe::dense::read_dense_status(&v, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = moe::dense::read_gemm_status(&g, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "moe_dense_read_status: %s", cudaGetErrorString(e));
-  *status = v;
+  *status = v | g;
   return MOE_OK;
 }
 

@@ -18,6 +18,7 @@ namespace dense {
 // 16-bit element types.  Tensors are addressed as raw 16-bit patterns; the
 // tag selects the conversion and the mma operand type.
 struct Bf16 {
+  static constexpr bool kBf16 = true;
   static MOE_DEV float to_f32(uint16_t b) { return bf16_to_f32(b); }
   static MOE_DEV uint16_t from_f32(float f) { return f32_to_bf16(f); }
   static MOE_DEV float2 unpack(uint32_t v) {
@@ -35,6 +36,7 @@ struct Bf16 {
 };
 
 struct Fp16 {
+  static constexpr bool kBf16 = false;
   static MOE_DEV float to_f32(uint16_t b) { return __half2float(__ushort_as_half(b)); }
   static MOE_DEV uint16_t from_f32(float f) { return __half_as_ushort(__float2half_rn(f)); }
   static MOE_DEV float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }

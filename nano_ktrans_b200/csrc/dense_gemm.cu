@@ -1,0 +1,729 @@
+// dense_gemm.cu — dense projections on the tcgen05 tensor cores, for more
+// tokens than the weight-streaming kernel takes: out = act(x W^T + b) + r and
+// act(x Wg^T) * (x Wu^T), accumulated in tensor memory in fp32, the epilogue
+// in the same kernel.  A = token rows (the MMA's M), B = weight rows (its N),
+// both K-major, TMA-loaded in 64-element K steps with the 128-byte swizzle;
+// rows and K beyond the tensors arrive as zeros.
+//
+// pair_gemm_kernel: many tokens.  A pair of SMs (cta_group::2) works on 256
+//   tokens x 256 weight rows: each SM stages half of both operands, so a byte
+//   brought into shared memory is used for 256 rows of the other operand.
+//   Gated: the first SM's half of B is 128 gate rows, the second's the same 128
+//   up rows, so gate and up of a feature are 128 accumulator columns apart.
+//   Persistent; two accumulators of 256 columns (all of tensor memory), so the
+//   epilogue of one tile runs under the next tile's MMAs.
+// split_gemm_kernel: a few hundred tokens, or too few tiles for every SM.  One
+//   SM per tile of up to 256 tokens x a slice of the features whose width is
+//   chosen so that the slices cover the SMs evenly, optionally with K split
+//   over a cluster of 2, 4 or 8 SMs that add their partial sums through
+//   distributed shared memory in rank order (no workspace, no atomics).
+//
+// Waits are bounded: one that runs out records kStatusTimeout and the kernel
+// unwinds, waiting (bounded) for what it has in flight.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "dense_common.cuh"
+#include "kernels.h"
+
+namespace moe {
+namespace dense {
+
+__device__ int g_gemm_status;  // kStatus* bits of this device's GEMM launches since the last read
+
+namespace {
+
+constexpr uint32_t kSpin = 1u << 22;
+constexpr int kBK = 64;                 // K elements per stage: one 128-byte swizzled row
+constexpr size_t kSmemLimit = 232448;
+
+MOE_DEV uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+MOE_DEV void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+MOE_DEV void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Arrive on a barrier of any block of the cluster.
+MOE_DEV void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+MOE_DEV bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kSpin; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+MOE_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address, in the cluster's shared window, of block `rank`'s copy of `addr`.
+MOE_DEV uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+MOE_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+MOE_DEV float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// 2-D tiled load into this block's shared memory (no multicast).  With PAIR the
+// barrier may be the pair's other block's.
+template <bool PAIR>
+MOE_DEV void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+        "[%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// K-major tile, 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart.
+MOE_DEV uint64_t tile_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+// Instruction descriptor: D fp32, A and B of the element type, K-major, M x n.
+template <typename T>
+MOE_DEV uint32_t instr_desc(int m, int n) {
+  constexpr uint32_t type = T::kBf16 ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <int GROUP>
+MOE_DEV void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (GROUP == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// One arrival on `bar` (of both blocks of a pair) once the MMAs issued so far are done.
+MOE_DEV void commit_one(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+MOE_DEV void commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+MOE_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+MOE_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 16 consecutive fp32 columns of this warp's 32 lanes; the values are there after tmem_wait.
+MOE_DEV void tmem_ld16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int N>
+MOE_DEV void activate_all(int act, float (&v)[N]) {
+  switch (act) {
+    case MOE_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate<MOE_ACT_SILU>(v[i]);
+      break;
+    case MOE_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate<MOE_ACT_GELU>(v[i]);
+      break;
+    case MOE_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate<MOE_ACT_GELU_TANH>(v[i]);
+      break;
+    case MOE_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate<MOE_ACT_RELU>(v[i]);
+      break;
+    default:
+      break;
+  }
+}
+
+MOE_DEV void give_up(volatile int* flag) {
+  if (!*flag) {
+    *flag = 1;
+    atomicOr(&g_gemm_status, kStatusTimeout);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// pair_gemm_kernel
+// ---------------------------------------------------------------------------
+constexpr int kPStages = 6, kPTile = 128 * 128, kPStage = 2 * kPTile;  // A and B half of one SM: 16 KB each
+constexpr int kPBarOff = kPStages * kPStage;
+constexpr size_t kPSmem = kPBarOff + 8 * (2 * kPStages + 4) + 16 + 1024;
+constexpr int kPThreads = 256;
+static_assert(kPSmem <= kSmemLimit, "shared-memory plan");
+
+// 16 output columns of one row from n on: wide stores where the row allows.
+template <typename T>
+MOE_DEV void store16(const LinearArgs& a, int64_t m, int n, float (&v)[16], bool wide) {
+  uint16_t* o = a.out + m * a.ldo + n;
+  const uint16_t* r = a.res ? a.res + m * a.ldr + n : nullptr;
+  if (wide && n + 16 <= a.n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (r) {
+        const uint4 q = *reinterpret_cast<const uint4*>(r + 8 * h);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = T::unpack(w[i]);
+          v[8 * h + 2 * i] += f.x;
+          v[8 * h + 2 * i + 1] += f.y;
+        }
+      }
+      uint32_t p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = T::pack(v[8 * h + 2 * i], v[8 * h + 2 * i + 1]);
+      *reinterpret_cast<uint4*>(o + 8 * h) = make_uint4(p[0], p[1], p[2], p[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (n + i < a.n) o[i] = T::from_f32(r ? v[i] + T::to_f32(r[i]) : v[i]);
+  }
+}
+
+template <typename T, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
+    pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ LinearArgs a, int wide) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int abort_s;
+  volatile int* aborted = &abort_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPBarOff);
+  uint64_t* full = bars;                      // [stages] of the first block: both blocks' tiles landed
+  uint64_t* empty = bars + kPStages;          // [stages] of each block: the MMAs that read the stage are done
+  uint64_t* acc_full = empty + kPStages;      // [2] of each block
+  uint64_t* acc_empty = acc_full + 2;         // [2] of the first block: both blocks' epilogue warps have read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+  if (tid == 0) {
+    for (int s = 0; s < kPStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&acc_full[s]), 1);
+      mbar_init(smem_u32(&acc_empty[s]), 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *aborted = 0;
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised, both have their tensor memory
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  constexpr int kTN = GATED ? 128 : 256;  // features per tile
+  const int mt = (a.m + 255) / 256, nt = (a.n + kTN - 1) / kTN, nk = (a.k + kBK - 1) / kBK;
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  // Tiles in groups of up to 16 row tiles, rows fastest: the pairs at work share
+  // few weight tiles and a block of tokens that stays in L2.
+  const int total = mt * nt;
+  auto place = [&](int i, int& m, int& n) {
+    const int per = 16 * nt, gidx = i / per, in = i - gidx * per, rows = min(16, mt - 16 * gidx);
+    n = in / rows;
+    m = 16 * gidx + in - n * rows;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int i = pair; i < total && ok; i += pairs) {
+        int m, n;
+        place(i, m, n);
+        const int xr = m * 256 + 128 * static_cast<int>(rank);
+        const int wr = GATED ? n * 128 : n * 256 + 128 * static_cast<int>(rank);
+        const CUtensorMap* tw = GATED && rank == 1 ? &tm_u : &tm_w;
+        for (int kc = 0; kc < nk; ++kc, ++it) {
+          const int s = it % kPStages;
+          if (*aborted || (it >= kPStages && !mbar_wait(smem_u32(&empty[s]), ((it / kPStages) - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * kPStage);
+          const uint32_t bar = map_rank(smem_u32(&full[s]), 0), dst = smem_u32(smem + s * kPStage);
+          tma_load<true>(dst, &tm_x, kc * kBK, xr, bar);
+          tma_load<true>(dst + kPTile, tw, kc * kBK, wr, bar);
+        }
+      }
+      if (!ok) give_up(aborted);
+      // nothing of this block's stages is in flight or being read when it exits
+      for (int j = max(0, it - kPStages); j < it; ++j) mbar_wait(smem_u32(&empty[j % kPStages]), (j / kPStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = instr_desc<T>(256, 256);
+      int it = 0, ti = 0;
+      bool ok = true;
+      for (int i = pair; i < total && ok; i += pairs, ++ti) {
+        const int acc = ti & 1;
+        if (ti >= 2 && !mbar_wait(smem_u32(&acc_empty[acc]), ((ti >> 1) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        for (int kc = 0; kc < nk; ++kc, ++it) {
+          const int s = it % kPStages;
+          if (*aborted || !mbar_wait(smem_u32(&full[s]), (it / kPStages) & 1)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t base = smem_u32(smem + s * kPStage);
+          const uint64_t da = tile_desc(base), db = tile_desc(base + kPTile);
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            umma<2>(tmem + acc * 256, da + 2 * kk, db + 2 * kk, idesc, kc > 0 || kk > 0);
+          commit_pair(smem_u32(&empty[s]));
+        }
+        commit_pair(smem_u32(&acc_full[acc]));
+      }
+      if (!ok) give_up(aborted);
+    }
+  } else if (warp >= 4) {
+    const int q = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    int ti = 0;
+    for (int i = pair; i < total; i += pairs, ++ti) {
+      int mi, ni;
+      place(i, mi, ni);
+      const int acc = ti & 1;
+      const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (ti >> 1) & 1);
+      if (!__all_sync(kFullMask, ok)) {
+        give_up(aborted);
+        break;
+      }
+      fence_after();
+      const int64_t m = static_cast<int64_t>(mi) * 256 + 128 * rank + q * 32 + lane;
+      const uint32_t base = tmem + acc * 256 + lanes;
+#pragma unroll 1
+      for (int c = 0; c < kTN; c += 16) {
+        const int n = ni * kTN + c;
+        if (n >= a.n) break;  // warp-uniform
+        float v[16];
+        tmem_ld16(base + c, v);
+        if constexpr (GATED) {
+          float u[16];
+          tmem_ld16(base + 128 + c, u);
+          activate_all(a.act, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] *= u[j];
+        } else {
+          if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (n + j < a.n) v[j] += T::to_f32(__ldg(a.bias + n + j));
+          }
+          activate_all(a.act, v);
+        }
+        if (m < a.m) store16<T>(a, m, n, v, wide != 0);
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&acc_empty[acc]), 0));
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// ---------------------------------------------------------------------------
+// split_gemm_kernel
+// ---------------------------------------------------------------------------
+struct SplitPlan {
+  int rows;     // token rows per tile: 128 or 256
+  int splits;   // blocks of a cluster that share a tile, each with a part of K
+  int slices;   // feature slices
+  int width;    // features of the widest slice, padded (gated: multiple of 8, else of 16)
+  int box_x;    // token rows loaded per stage
+  int stages;
+  int smem;
+};
+constexpr int kQThreads = 320;  // producer, MMA, 8 epilogue warps
+constexpr int kQTail = 1024 + 16384;  // alignment, and what an MMA reads past a tile of fewer than 128 rows
+
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(kQThreads, 1)
+    split_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ LinearArgs a,
+                      const __grid_constant__ SplitPlan p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[16], empty[16], acc_full;
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_s;
+  volatile int* aborted = &abort_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int slice = blockIdx.x / p.splits;
+  const int n0 = static_cast<int>(static_cast<int64_t>(a.n) * slice / p.slices);
+  const int n1 = static_cast<int>(static_cast<int64_t>(a.n) * (slice + 1) / p.slices);
+  const int m0 = blockIdx.y * p.rows, valid = min(p.rows, a.m - m0);
+  const int nk = (a.k + kBK - 1) / kBK;
+  const int k_lo = nk * rank / p.splits, k_hi = nk * (rank + 1) / p.splits, steps = k_hi - k_lo;
+  const int cols = GATED ? 2 * p.width : p.width;  // the MMA's N
+  const int row_tiles = (valid + 127) / 128;
+  const int x_bytes = p.box_x * 128, stage_bytes = x_bytes + cols * 128;
+  const uint32_t need = static_cast<uint32_t>((p.rows / 128) * cols);
+  const uint32_t tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(&acc_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *aborted = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                 "r"(tmem_cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_s;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < steps; ++it) {
+        const int s = it % p.stages;
+        if (*aborted || (it >= p.stages && !mbar_wait(smem_u32(&empty[s]), ((it / p.stages) - 1) & 1))) {
+          give_up(aborted);
+          break;
+        }
+        const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + s * stage_bytes);
+        const int k = (k_lo + it) * kBK;
+        mbar_expect_tx(bar, stage_bytes);
+        tma_load<false>(dst, &tm_x, k, m0, bar);
+        tma_load<false>(dst + x_bytes, &tm_w, k, n0, bar);
+        if constexpr (GATED) tma_load<false>(dst + x_bytes + p.width * 128, &tm_u, k, n0, bar);
+      }
+      if (*aborted)  // no copy may still be landing when the block exits
+        for (int j = max(0, it - p.stages); j < it; ++j) mbar_wait(smem_u32(&full[j % p.stages]), (j / p.stages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc<T>(128, cols);
+      for (int it = 0; it < steps; ++it) {
+        const int s = it % p.stages;
+        if (*aborted || !mbar_wait(smem_u32(&full[s]), (it / p.stages) & 1)) {
+          give_up(aborted);
+          break;
+        }
+        fence_after();
+        const uint32_t base = smem_u32(smem + s * stage_bytes);
+        const uint64_t db = tile_desc(base + x_bytes);
+        for (int r = 0; r < row_tiles; ++r) {
+          // a tile of fewer than 128 rows: the MMA reads on into other bytes of the
+          // stages; those accumulator lanes are never read
+          const uint64_t da = tile_desc(base + r * 16384);
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            umma<1>(tmem + r * cols, da + 2 * kk, db + 2 * kk, idesc, it > 0 || kk > 0);
+        }
+        commit_one(smem_u32(&empty[s]));
+      }
+      commit_one(smem_u32(&acc_full));
+      if (!mbar_wait(smem_u32(&acc_full), 0)) give_up(aborted);  // every MMA is done before tensor memory is freed
+    }
+  }
+  __syncwarp();
+  if (warp >= 2 && !__all_sync(kFullMask, mbar_wait(smem_u32(&acc_full), 0))) give_up(aborted);
+  __syncthreads();
+  const bool good = !*aborted;
+  // ---- partial sums into shared memory, [row][cols + 1] ----
+  float* part = reinterpret_cast<float*>(smem);
+  const int ldp = cols + 1;
+  if (good && warp >= 2) {
+    fence_after();
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    for (int r = 0; r < row_tiles; ++r) {
+      const int row = r * 128 + q * 32 + lane;
+      if (r * 128 + q * 32 >= valid) continue;  // warp-uniform
+      for (int c = half * 16; c < cols; c += 32) {
+        float v[16];
+        if (steps > 0) {
+          tmem_ld16(tmem + r * cols + c + (static_cast<uint32_t>(q * 32) << 16), v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+        }
+        if (row < valid) {
+          float* o = part + row * ldp + c;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = v[j];
+        }
+      }
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
+  }
+  if (p.splits > 1) cluster_sync();
+  // ---- this block's share of the rows: partials added in rank order ----
+  if (good) {
+    const int r_lo = valid * rank / p.splits, r_hi = valid * (rank + 1) / p.splits, w = n1 - n0;
+    uint32_t peer[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) peer[s] = s < p.splits && p.splits > 1 ? map_rank(smem_u32(part), s) : smem_u32(part);
+    for (int r = r_lo + warp; r < r_hi; r += kQThreads / 32) {
+      const int64_t m = m0 + r;
+      for (int c = lane; c < w; c += 32) {
+        const int n = n0 + c;
+        const uint32_t off = 4u * static_cast<uint32_t>(r * ldp + c);
+        float v = 0.0f, u = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < p.splits) {
+            v += ld_cluster(peer[s] + off);
+            if constexpr (GATED) u += ld_cluster(peer[s] + off + 4u * static_cast<uint32_t>(p.width));
+          }
+        if constexpr (GATED) {
+          v = activate_rt(a.act, v) * u;
+        } else {
+          if (a.bias) v += T::to_f32(a.bias[n]);
+          v = activate_rt(a.act, v);
+          if (a.res) v += T::to_f32(a.res[m * a.ldr + n]);
+        }
+        a.out[m * a.ldo + n] = T::from_f32(v);
+      }
+    }
+  }
+  if (p.splits > 1) cluster_sync();  // peers are done with this block's partials
+}
+
+// ---------------------------------------------------------------------------
+// Plans
+// ---------------------------------------------------------------------------
+
+// Blocks of the split kernel that run at once, by cluster size (asked of the
+// driver once per device: how many clusters fit depends on the SMs per GPC).
+int resident_blocks(int dev, int splits, int sms) {
+  static std::mutex mu;
+  static int known[64][9];
+  if (splits == 1 || dev < 0 || dev >= 64) return sms;
+  std::lock_guard<std::mutex> lock(mu);
+  int& v = known[dev][splits];
+  if (v == 0) {
+    if (!ensure_dynamic_smem(reinterpret_cast<const void*>(split_gemm_kernel<Bf16, false>), kSmemLimit - 2048, kQThreads)) {
+      v = -1;
+      return 0;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3(kQThreads);
+    cfg.dynamicSmemBytes = kSmemLimit - 2048;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, split_gemm_kernel<Bf16, false>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      v = -1;
+    } else {
+      v = n * splits < sms ? n * splits : sms;
+    }
+  }
+  return v < 0 ? 0 : v;
+}
+
+// Estimated clocks of a plan; the best of the candidates is taken.  Per K step
+// a block brings box_x + cols rows of 128 bytes into shared memory (about 40
+// bytes a clock and SM) and its MMAs take 2 clocks a column and row tile; a
+// launch, tensor-memory and epilogue overhead is added once per wave.
+SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
+  const bool gated = a.w_up != nullptr;
+  const int nk = (a.k + kBK - 1) / kBK, pad = gated ? 8 : 16, mul = gated ? 2 : 1;
+  SplitPlan best{};
+  clocks = 1e30;
+  for (int rows = 128; rows <= 256; rows += 128) {
+    if (rows == 256 && a.m <= 128) break;
+    const int mg = (a.m + rows - 1) / rows;
+    if (mg > 65535) continue;
+    const int box = a.m >= rows ? rows : (a.m + 7) / 8 * 8;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      if (splits > nk) break;
+      const int cap = resident_blocks(dev, splits, sms);
+      for (int waves = 1; waves <= 4; ++waves) {
+        int slices = cap * waves / (splits * mg);
+        if (slices < 1) continue;
+        const int most = (a.n + pad - 1) / pad;  // no narrower than the padding
+        if (slices > most) slices = most;
+        const int width = ((a.n + slices - 1) / slices + pad - 1) / pad * pad;
+        const int cols = width * mul;
+        if (cols > 256 || rows / 128 * cols > 512) continue;
+        const int stage = (box + cols) * 128;
+        int stages = static_cast<int>((kSmemLimit - 2048 - kQTail) / stage);
+        if (stages > 16) stages = 16;
+        if (stages < 2) continue;
+        const int64_t part = 4LL * (a.m < rows ? a.m : rows) * (cols + 1);
+        int64_t smem = static_cast<int64_t>(stages) * stage;
+        if (part > smem) smem = part;
+        smem += kQTail;
+        if (smem > static_cast<int64_t>(kSmemLimit) - 2048) continue;
+        const int steps = (nk + splits - 1) / splits, real_waves = (slices * mg * splits + cap - 1) / cap;
+        const double load = (box + cols) * 128 / 40.0, mma = 2.0 * cols * (box > 128 ? 2 : 1);
+        const double join = part / splits / 16.0 + (splits > 1 ? 1500.0 : 0.0);
+        const double t = real_waves * (steps * (load > mma ? load : mma) + join + 3000.0);
+        if (t < clocks) {
+          clocks = t;
+          best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem)};
+        }
+      }
+    }
+  }
+  return best;
+}
+
+// A tensor map wants a stride of whole 16 bytes even where there is one row.
+uint64_t row_stride(int64_t ld, int rows, int k) { return static_cast<uint64_t>(rows > 1 ? ld : k); }
+
+template <typename T, bool GATED>
+cudaError_t launch_split(const LinearArgs& a, const SplitPlan& p, cudaStream_t st) {
+  alignas(64) CUtensorMap tx, tw, tu;
+  if (!make_tmap_rows(&tx, a.x, T::kBf16, a.k, a.m, a.ldx, p.box_x) ||
+      !make_tmap_rows(&tw, a.w, T::kBf16, a.k, a.n, row_stride(a.ldw, a.n, a.k), p.width) ||
+      !make_tmap_rows(&tu, GATED ? a.w_up : a.w, T::kBf16, a.k, a.n,
+                      row_stride(GATED ? a.ldwu : a.ldw, a.n, a.k), p.width))
+    return cudaErrorInvalidValue;
+  const void* kern = reinterpret_cast<const void*>(split_gemm_kernel<T, GATED>);
+  if (!ensure_dynamic_smem(kern, p.smem, kQThreads)) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.slices * p.splits, (a.m + p.rows - 1) / p.rows);
+  cfg.blockDim = dim3(kQThreads);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, split_gemm_kernel<T, GATED>, tx, tw, tu, a, p);
+}
+
+template <typename T, bool GATED>
+cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t st) {
+  alignas(64) CUtensorMap tx, tw, tu;
+  if (!make_tmap_rows(&tx, a.x, T::kBf16, a.k, a.m, a.ldx, 128) ||
+      !make_tmap_rows(&tw, a.w, T::kBf16, a.k, a.n, row_stride(a.ldw, a.n, a.k), 128) ||
+      !make_tmap_rows(&tu, GATED ? a.w_up : a.w, T::kBf16, a.k, a.n,
+                      row_stride(GATED ? a.ldwu : a.ldw, a.n, a.k), 128))
+    return cudaErrorInvalidValue;
+  const void* kern = reinterpret_cast<const void*>(pair_gemm_kernel<T, GATED>);
+  if (!ensure_dynamic_smem(kern, kPSmem, kPThreads)) return cudaErrorInvalidConfiguration;
+  const auto aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+  const int wide = aligned(a.out, a.ldo) && (a.res == nullptr || aligned(a.res, a.ldr));
+  const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < sms / 2 ? tiles : sms / 2));
+  cfg.blockDim = dim3(kPThreads);
+  cfg.dynamicSmemBytes = kPSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, pair_gemm_kernel<T, GATED>, tx, tw, tu, a, wide);
+}
+
+template <typename T, bool GATED>
+cudaError_t gemm(const LinearArgs& a, int dev, int sms, cudaStream_t st) {
+  double split_clocks = 0;
+  const SplitPlan p = plan_split(a, dev, sms, split_clocks);
+  const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+  const int pairs = sms / 2, nk = (a.k + kBK - 1) / kBK;
+  const double pair_clocks = static_cast<double>((tiles + pairs - 1) / pairs) * nk * 600.0 + 8000.0;
+  if (split_clocks < pair_clocks) return launch_split<T, GATED>(a, p, st);
+  return launch_pair<T, GATED>(a, sms, st);
+}
+
+}  // namespace
+
+cudaError_t launch_gemm(const LinearArgs& a, int dtype, int dev, int sms, cudaStream_t st) {
+  if (dtype == MOE_DTYPE_FP16) return a.w_up ? gemm<Fp16, true>(a, dev, sms, st) : gemm<Fp16, false>(a, dev, sms, st);
+  return a.w_up ? gemm<Bf16, true>(a, dev, sms, st) : gemm<Bf16, false>(a, dev, sms, st);
+}
+
+cudaError_t read_gemm_status(int* status, cudaStream_t st) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_gemm_status);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e;
+}
+
+}  // namespace dense
+}  // namespace moe

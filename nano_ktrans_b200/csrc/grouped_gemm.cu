@@ -637,6 +637,20 @@ bool make_tmap_2d(void* out_map, const void* base, bool fp16, uint64_t inner, ui
   return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_rows(void* out_map, const void* base, bool bf16, uint64_t inner, uint64_t rows, uint64_t ld,
+                    uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {inner, rows};
+  cuuint64_t strides[1] = {ld * 2};
+  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(reinterpret_cast<CUtensorMap*>(out_map),
+            bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool gemm_shape_ok(int bits, const QuantProj& p) {
   if (bits != 4 && bits != 8) return false;
   if (p.n % gg::BM || p.k % gg::BK) return false;

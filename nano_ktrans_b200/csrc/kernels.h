@@ -138,6 +138,10 @@ void launch_dequant_rows(int bits, const QuantProj& p, int expert, int row0, int
 // entry point is unavailable or the encode fails.
 bool make_tmap_2d(void* out_map, const void* base, bool fp16, uint64_t inner, uint64_t rows, uint32_t box_inner,
                   uint32_t box_rows, bool swizzle128);
+// 2-D tensor map over `rows` rows of `inner` 16-bit elements, `ld` elements
+// apart (16-byte aligned), box {64, box_rows}, 128-byte swizzle.
+bool make_tmap_rows(void* out_map, const void* base, bool bf16, uint64_t inner, uint64_t rows, uint64_t ld,
+                    uint32_t box_rows);
 // Shape rules of the GEMM path for one projection (N % 128, K % 64, W4 group
 // % 64, W8 per-channel).
 bool gemm_shape_ok(int bits, const QuantProj& p);
