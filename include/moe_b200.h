@@ -446,7 +446,7 @@ int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_
  * two forms.
  * 0 <= num_tokens <= MOE_DENSE_MAX_TOKENS (above: MOE_ERANGE), num_experts in
  * [1, 1024], top_k in [1, min(16, num_experts)], hidden and inter multiples of
- * 16, x rows and all weights on 32-byte boundaries.  out may be x or residual
+ * 16, x rows and all weights on 16-byte boundaries.  out may be x or residual
  * itself, and overlaps nothing else.
  * workspace_dev: moe_dense_workspace bytes, 256-byte aligned, for this call
  * alone until its kernels have run (calls in flight at once, and graphs

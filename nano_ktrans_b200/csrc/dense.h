@@ -26,14 +26,14 @@ struct LinearArgs {
 // Every shape, stride and alignment.
 cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st);
 
-// Elements of the widest load that every row of x and of the weights allows:
-// 16 (32 bytes), 8 (16 bytes), or 0 (none).
-int wide_elements(const LinearArgs& a);
-// Up to kStreamTokens tokens, wide_elements(a) != 0.
+// Whether every row of x and of the weights lies on a 16-byte boundary and
+// holds whole 16-byte pieces: what all kernels but the generic one need.
+bool wide_rows(const LinearArgs& a);
+// Up to kStreamTokens tokens, wide rows.
 constexpr int kStreamTokens = 32;
 cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaStream_t st);
 
-// More tokens than that, wide_elements(a) != 0: tcgen05 kernels.
+// More tokens than that, wide rows: tcgen05 kernels.
 cudaError_t launch_gemm(const LinearArgs& a, int dtype, int dev, int sms, cudaStream_t st);
 cudaError_t read_gemm_status(int* status, cudaStream_t st);
 

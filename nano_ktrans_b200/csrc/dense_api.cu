@@ -47,7 +47,7 @@ cudaError_t launch_linear(const LinearArgs& a, int dtype, cudaStream_t st) {
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms < 1) return cudaErrorInvalidDevice;
-  if (moe::dense::wide_elements(a) == 0) return moe::dense::launch_generic(a, dtype, st);
+  if (!moe::dense::wide_rows(a)) return moe::dense::launch_generic(a, dtype, st);
   if (a.m <= moe::dense::kStreamTokens) return moe::dense::launch_stream_linear(a, dtype, sms, st);
   return moe::dense::launch_gemm(a, dtype, dev, sms, st);
 }
@@ -178,9 +178,9 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
                         shared ? d->shared_gate_dev : nullptr, shared ? d->shared_up_dev : nullptr,
                         shared ? d->shared_down_dev : nullptr, shared ? d->shared_gate_vec_dev : nullptr};
   for (const void* p : wide)
-    if (reinterpret_cast<uintptr_t>(p) % 32)
-      return refuse(err, err_len, MOE_EINVAL, "%s: x and the weights must start on 32-byte boundaries", me);
-  if (t > 1 && d->ldx % 16) return refuse(err, err_len, MOE_EINVAL, "%s: the rows of x must lie on 32-byte boundaries", me);
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      return refuse(err, err_len, MOE_EINVAL, "%s: x and the weights must start on 16-byte boundaries", me);
+  if (t > 1 && d->ldx % 8) return refuse(err, err_len, MOE_EINVAL, "%s: the rows of x must lie on 16-byte boundaries", me);
   const void* even[] = {d->logits_dev, d->weights_dev, d->residual_dev, d->out_dev, d->weights_out_dev};
   for (const void* p : even)
     if (reinterpret_cast<uintptr_t>(p) % 2) return refuse(err, err_len, MOE_EINVAL, "%s: pointers must be 2-byte aligned", me);

@@ -98,56 +98,54 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 // gated tile is 8 gate rows (mma rows 0-7) and the same 8 up rows (mma rows
 // 8-15), so gate and up of a feature meet in one thread.
 // ---------------------------------------------------------------------------
-template <typename T, bool GATED, int NT, int VEC>
+template <bool GATED, int NT>
 struct LinearSrc {
   const LinearArgs& a;
-  int r0, r1, g, t;
+  int r0, r1, g, t8;
   const uint16_t* xrow[NT];
   MOE_DEV LinearSrc(const LinearArgs& args, int lo, int hi) : a(args), r0(lo), r1(hi) {
     const int lane = threadIdx.x & 31;
     g = lane >> 2;
-    t = lane & 3;
+    t8 = 8 * (lane & 3);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.m ? a.x + (8 * j + g) * a.ldx : nullptr;
+    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.m ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
-  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[VEC / 2], uint32_t (&fb)[VEC / 2]) const {
-    const int k = unit * 4 * VEC + t * VEC;
+  MOE_DEV const uint16_t* any() const { return a.w; }
+  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
+    const int k = unit * 64;
+    len = a.k - k;
     if constexpr (GATED) {
       const int r = r0 + 8 * tile + g;
-      if (r < r1 && k < a.k) {
-        ld_weights(fa, a.w + r * a.ldw + k);
-        ld_weights(fb, a.w_up + r * a.ldwu + k);
-      } else {
-        zero(fa);
-        zero(fb);
-      }
+      pa = r < r1 ? a.w + r * a.ldw + k : nullptr;
+      pb = r < r1 ? a.w_up + r * a.ldwu + k : nullptr;
     } else {
       const int r = r0 + 16 * tile + g;
-      if (r < r1 && k < a.k) ld_weights(fa, a.w + r * a.ldw + k);
-      else zero(fa);
-      if (r + 8 < r1 && k < a.k) ld_weights(fb, a.w + (r + 8) * a.ldw + k);
-      else zero(fb);
+      pa = r < r1 ? a.w + r * a.ldw + k : nullptr;
+      pb = r + 8 < r1 ? a.w + (r + 8) * a.ldw + k : nullptr;
     }
   }
-  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[VEC / 2]) const {
-    const int k = unit * 4 * VEC + t * VEC;
-    if (xrow[j] != nullptr && k < a.k) ld_tokens(x, xrow[j] + k);
-    else zero(x);
+  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
+    const int k = unit * 64;
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    x0 = xrow[j] != nullptr && k + t8 < a.k ? ld_tokens(xrow[j] + k) : z;
+    x1 = xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
   }
 };
 
-template <typename T, bool GATED, int NT, int VEC>
+constexpr int kLinearDepth = 4;
+
+template <typename T, bool GATED, int NT>
 __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __grid_constant__ LinearArgs a) {
-  extern __shared__ float part[];
+  extern __shared__ __align__(16) unsigned char smem[];
   // A launch that may start early reads nothing before its predecessor is done
   // (weights too: they may be that kernel's output), and lets none start early.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int r0 = static_cast<int>(static_cast<int64_t>(a.n) * blockIdx.x / gridDim.x);
   const int r1 = static_cast<int>(static_cast<int64_t>(a.n) * (blockIdx.x + 1) / gridDim.x);
-  constexpr int kRows = GATED ? 8 : 16, kD = VEC == 16 ? 4 : 6;
-  const int tiles = (r1 - r0 + kRows - 1) / kRows, units = (a.k + 4 * VEC - 1) / (4 * VEC);
-  const LinearSrc<T, GATED, NT, VEC> src(a, r0, r1);
-  Streamer<T, NT, VEC, kD, kRows> s;
+  constexpr int kRows = GATED ? 8 : 16;
+  const int tiles = (r1 - r0 + kRows - 1) / kRows, units = (a.k + 63) / 64;
+  const LinearSrc<GATED, NT> src(a, r0, r1);
+  Streamer<T, NT, kLinearDepth, kRows> s(smem);
   s.prologue(src, tiles, units);
   s.run(src, tiles, units, a.m, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + kRows * tile + row;
@@ -161,51 +159,45 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
       if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
     }
     a.out[col * a.ldo + n] = T::from_f32(v);
-  }, part);
+  });
 }
 
-template <typename T, bool GATED, int NT, int VEC>
+template <typename T, bool GATED, int NT>
 static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) {
-  const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT, VEC>);
-  if (!ensure_dynamic_smem(kern, part_bytes<NT>(), kSThreads)) return cudaErrorInvalidConfiguration;
+  const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT>);
+  constexpr size_t smem = stream_bytes<NT, kLinearDepth>();
+  if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.n < sms ? a.n : sms);
   cfg.blockDim = dim3(kSThreads);
-  cfg.dynamicSmemBytes = part_bytes<NT>();
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, stream_linear_kernel<T, GATED, NT, VEC>, a);
-}
-
-template <typename T, bool GATED, int NT>
-static cudaError_t stream_vec(const LinearArgs& a, int vec, int sms, cudaStream_t st) {
-  return vec == 16 ? stream_launch<T, GATED, NT, 16>(a, sms, st) : stream_launch<T, GATED, NT, 8>(a, sms, st);
+  return cudaLaunchKernelEx(&cfg, stream_linear_kernel<T, GATED, NT>, a);
 }
 
 template <typename T, bool GATED>
-static cudaError_t stream_cols(const LinearArgs& a, int vec, int sms, cudaStream_t st) {
-  return a.m <= 8 ? stream_vec<T, GATED, 1>(a, vec, sms, st)
-         : a.m <= 16 ? stream_vec<T, GATED, 2>(a, vec, sms, st)
-                     : stream_vec<T, GATED, 4>(a, vec, sms, st);
+static cudaError_t stream_cols(const LinearArgs& a, int sms, cudaStream_t st) {
+  return a.m <= 8 ? stream_launch<T, GATED, 1>(a, sms, st)
+         : a.m <= 16 ? stream_launch<T, GATED, 2>(a, sms, st)
+                     : stream_launch<T, GATED, 4>(a, sms, st);
 }
 
-int wide_elements(const LinearArgs& a) {
+bool wide_rows(const LinearArgs& a) {
   const uintptr_t p = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) |
                       reinterpret_cast<uintptr_t>(a.w_up);
   // a single row has no stride to respect
   const int64_t l = (a.m > 1 ? a.ldx : 0) | (a.n > 1 ? a.ldw : 0) | (a.n > 1 && a.w_up ? a.ldwu : 0) | a.k;
-  return p % 32 == 0 && l % 16 == 0 ? 16 : p % 16 == 0 && l % 8 == 0 ? 8 : 0;
+  return p % 16 == 0 && l % 8 == 0;
 }
 
 cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaStream_t st) {
-  const int vec = wide_elements(a);
-  if (dtype == MOE_DTYPE_FP16)
-    return a.w_up ? stream_cols<Fp16, true>(a, vec, sms, st) : stream_cols<Fp16, false>(a, vec, sms, st);
-  return a.w_up ? stream_cols<Bf16, true>(a, vec, sms, st) : stream_cols<Bf16, false>(a, vec, sms, st);
+  if (dtype == MOE_DTYPE_FP16) return a.w_up ? stream_cols<Fp16, true>(a, sms, st) : stream_cols<Fp16, false>(a, sms, st);
+  return a.w_up ? stream_cols<Bf16, true>(a, sms, st) : stream_cols<Bf16, false>(a, sms, st);
 }
 
 }  // namespace dense

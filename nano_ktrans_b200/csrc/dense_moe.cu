@@ -35,7 +35,7 @@ namespace dense {
 
 __device__ int g_dense_status;  // kStatus* bits of this device's dense calls since the last read
 
-constexpr int kRouterThreads = 128;
+constexpr int kRouterThreads = 256;
 
 // Block e < num_experts: logits[t][e]; block num_experts: the shared gate.
 template <typename T>
@@ -51,21 +51,26 @@ __global__ void __launch_bounds__(kRouterThreads) dense_router_kernel(const __gr
   float acc[kMoeTokens];
 #pragma unroll
   for (int t = 0; t < kMoeTokens; ++t) acc[t] = 0.0f;
-  for (int k = tid * 16; k < a.hidden; k += kRouterThreads * 16) {
-    uint32_t wv[8];
-    ld_weights(wv, w + k);
+  for (int k = tid * 8; k < a.hidden; k += kRouterThreads * 8) {
+    const uint4 wq = *reinterpret_cast<const uint4*>(w + k);
+    const uint32_t wv[4] = {wq.x, wq.y, wq.z, wq.w};
 #pragma unroll
-    for (int t = 0; t < kMoeTokens; ++t)
-      if (t < a.tokens) {
-        uint32_t xv[8];
-        ld_tokens(xv, a.x + t * a.ldx + k);
+    for (int t0 = 0; t0 < kMoeTokens; t0 += 4) {
+      if (t0 >= a.tokens) break;
+      uint4 xq[4];  // four tokens' loads under way at once
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 p = T::unpack(wv[i]), q = T::unpack(xv[i]);
-          acc[t] = fmaf(p.x, q.x, acc[t]);
-          acc[t] = fmaf(p.y, q.y, acc[t]);
+      for (int i = 0; i < 4; ++i) xq[i] = *reinterpret_cast<const uint4*>(a.x + min(t0 + i, a.tokens - 1) * a.ldx + k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t xv[4] = {xq[i].x, xq[i].y, xq[i].z, xq[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = T::unpack(wv[j]), q = T::unpack(xv[j]);
+          acc[t0 + i] = fmaf(p.x, q.x, acc[t0 + i]);
+          acc[t0 + i] = fmaf(p.y, q.y, acc[t0 + i]);
         }
       }
+    }
   }
 #pragma unroll
   for (int t = 0; t < kMoeTokens; ++t)
@@ -76,7 +81,9 @@ __global__ void __launch_bounds__(kRouterThreads) dense_router_kernel(const __gr
     }
   __syncthreads();
   if (tid < a.tokens) {
-    const float v = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRouterThreads / 32; ++i) v += part[i][tid];
     if (e < a.experts) a.logits[tid * a.experts + e] = T::from_f32(v);
     else a.shared_open[tid] = sigmoid_f32(v);
   }
@@ -162,94 +169,99 @@ struct Tables {
 // list of rows; `lo` to `hi` are this block's.  Tile i is the list's group of
 // 8 rows number lo / 8 + i (a group never spans two experts: their sizes are
 // multiples of 16), rows outside the block's range masked.
-template <typename T, int NT>
+template <int NT>
 struct GateUpSrc {
   const MoeArgs& a;
   const Tables& tb;
-  int lo, hi, routed, g, t;
+  int lo, hi, routed, g, t8;
   const uint16_t* xrow[NT];
   MOE_DEV GateUpSrc(const MoeArgs& args, const Tables& tables, int lo_, int hi_)
       : a(args), tb(tables), lo(lo_), hi(hi_), routed(tables.n_active * args.inter) {
     const int lane = threadIdx.x & 31;
     g = lane >> 2;
-    t = lane & 3;
+    t8 = 8 * (lane & 3);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx : nullptr;
+    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
-  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[8], uint32_t (&fb)[8]) const {
-    const int k = unit * 64 + t * 16, v0 = (lo / 8 + tile) * 8, v = v0 + g;
-    if (v < lo || v >= hi || k >= a.hidden) {
-      zero(fa);
-      zero(fb);
-      return;
-    }
+  MOE_DEV const uint16_t* any() const { return a.gate; }
+  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
+    const int k = unit * 64, v0 = (lo / 8 + tile) * 8, v = v0 + g;
+    len = a.hidden - k;
+    pa = pb = nullptr;
+    if (v < lo || v >= hi) return;
     if (v0 < routed) {
       const int s = v0 / a.inter;
-      const int64_t row = static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter);
-      ld_weights(fa, a.gate + row * a.hidden + k);
-      ld_weights(fb, a.up + row * a.hidden + k);
+      const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden + k;
+      pa = a.gate + at;
+      pb = a.up + at;
     } else {
-      const int64_t row = v - routed;
-      ld_weights(fa, a.shared_gate + row * a.hidden + k);
-      ld_weights(fb, a.shared_up + row * a.hidden + k);
+      const int64_t at = static_cast<int64_t>(v - routed) * a.hidden + k;
+      pa = a.shared_gate + at;
+      pb = a.shared_up + at;
     }
   }
-  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[8]) const {
-    const int k = unit * 64 + t * 16;
-    if (xrow[j] != nullptr && k < a.hidden) ld_tokens(x, xrow[j] + k);
-    else zero(x);
+  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
+    const int k = unit * 64;
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    x0 = xrow[j] != nullptr && k + t8 < a.hidden ? ld_tokens(xrow[j] + k) : z;
+    x1 = xrow[j] != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow[j] + k + 32) : z;
   }
 };
 
 // Output rows [r0, r1); K runs over the routed experts' h, then the shared
 // expert's.  Columns: hi of token c for c < half, then lo of token c - half.
-template <typename T, int NT>
+template <int NT>
 struct DownSrc {
   static constexpr int kHalf = 4 * NT;
   const MoeArgs& a;
   const Tables& tb;
-  int r0, r1, ue, routed_units, g, t;
+  int r0, r1, ue, routed_units, g, t8;
   MOE_DEV DownSrc(const MoeArgs& args, const Tables& tables, int lo, int hi) : a(args), tb(tables), r0(lo), r1(hi) {
     const int lane = threadIdx.x & 31;
     g = lane >> 2;
-    t = lane & 3;
+    t8 = 8 * (lane & 3);
     ue = (a.inter + 63) / 64;
     routed_units = tables.n_active * ue;
   }
   MOE_DEV int units() const { return routed_units + (a.shared_inter + 63) / 64; }
-  MOE_DEV void load(int tile, int unit, uint32_t (&fa)[8], uint32_t (&fb)[8]) const {
+  MOE_DEV const uint16_t* any() const { return a.down; }
+  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
     const int r = r0 + 16 * tile + g;
     const uint16_t* base;
-    int k, len;
+    int k, ld;
     if (unit < routed_units) {
       const int s = unit / ue;
-      k = (unit - s * ue) * 64 + t * 16;
-      len = a.inter;
+      k = (unit - s * ue) * 64;
+      ld = a.inter;
       base = a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter;
     } else {
-      k = (unit - routed_units) * 64 + t * 16;
-      len = a.shared_inter;
+      k = (unit - routed_units) * 64;
+      ld = a.shared_inter;
       base = a.shared_down;
     }
-    if (r < r1 && k < len) ld_weights(fa, base + static_cast<int64_t>(r) * len + k);
-    else zero(fa);
-    if (r + 8 < r1 && k < len) ld_weights(fb, base + static_cast<int64_t>(r + 8) * len + k);
-    else zero(fb);
+    len = ld - k;
+    pa = r < r1 ? base + static_cast<int64_t>(r) * ld + k : nullptr;
+    pb = r + 8 < r1 ? base + static_cast<int64_t>(r + 8) * ld + k : nullptr;
   }
-  MOE_DEV void tokens(int unit, int j, uint32_t (&x)[8]) const {
+  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
     const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf;
     const uint16_t* p = nullptr;
+    int k = 0, len = 0;
     if (tok < a.tokens) {
       if (unit < routed_units) {
-        const int s = unit / ue, k = (unit - s * ue) * 64 + t * 16, pair = tb.pair[s][tok];
-        if (pair >= 0 && k < a.inter) p = a.h + static_cast<int64_t>(2 * pair + part) * a.inter + k;
+        const int s = unit / ue, pair = tb.pair[s][tok];
+        k = (unit - s * ue) * 64 + t8;
+        len = pair >= 0 ? a.inter : 0;
+        p = a.h + static_cast<int64_t>(2 * pair + part) * a.inter + k;
       } else {
-        const int k = (unit - routed_units) * 64 + t * 16;
-        if (k < a.shared_inter) p = a.h_shared + static_cast<int64_t>(2 * tok + part) * a.shared_inter + k;
+        k = (unit - routed_units) * 64 + t8;
+        len = a.shared_inter;
+        p = a.h_shared + static_cast<int64_t>(2 * tok + part) * a.shared_inter + k;
       }
     }
-    if (p != nullptr) ld_l2(x, p);
-    else zero(x);
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    x0 = k < len ? ld_l2(p) : z;
+    x1 = k + 32 < len ? ld_l2(p + 32) : z;
   }
 };
 
@@ -262,16 +274,23 @@ MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
 }
 
+// Steps in flight: four column tiles of partials leave room for three.
+template <int ND>
+constexpr int moe_depth() {
+  return ND == 4 ? 3 : 4;
+}
+
 // NT column tiles hold the tokens of the gate / up phase, ND those of the down phase (hi and lo).
 template <typename T, int NT, int ND>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
-  extern __shared__ float part[];
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Tables tb;
+  constexpr int kD = moe_depth<ND>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- routing, in every block ----
-  uint32_t* keys = reinterpret_cast<uint32_t*>(part);  // [16][E] words, then used[E] bytes: before the partials are
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);  // [16][E] words, then used[E] bytes: before the ring is in use
   uint8_t* used = reinterpret_cast<uint8_t*>(keys + kMoeTokens * a.experts);
   for (int i = tid; i < a.experts; i += kSThreads) used[i] = 0;
   for (int i = tid; i < kMoePairs * kMoeTokens; i += kSThreads) {
@@ -332,9 +351,9 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   const int64_t rows = static_cast<int64_t>(tb.n_active) * a.inter + a.shared_inter;
   const int lo = static_cast<int>(rows * blockIdx.x / gridDim.x), hi = static_cast<int>(rows * (blockIdx.x + 1) / gridDim.x);
   {
-    const GateUpSrc<T, NT> src(a, tb, lo, hi);
+    const GateUpSrc<NT> src(a, tb, lo, hi);
     const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0, units = (a.hidden + 63) / 64;
-    Streamer<T, NT, 16, 4, 8> s;
+    Streamer<T, NT, kD, 8> s(smem);
     s.prologue(src, tiles, units);
     s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
       const int v0 = (lo / 8 + tile) * 8, v = v0 + row;
@@ -350,15 +369,15 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
         uint16_t* p = a.h_shared + static_cast<int64_t>(2 * col) * a.shared_inter + (v - src.routed);
         store_split<T>(p, p + a.shared_inter, h);
       }
-    }, part);
+    });
   }
 
   // ---- out = r + sum over experts of D h ----
   const int r0 = static_cast<int>(static_cast<int64_t>(a.hidden) * blockIdx.x / gridDim.x);
   const int r1 = static_cast<int>(static_cast<int64_t>(a.hidden) * (blockIdx.x + 1) / gridDim.x);
-  const DownSrc<T, ND> src(a, tb, r0, r1);
+  const DownSrc<ND> src(a, tb, r0, r1);
   const int tiles = (r1 - r0 + 15) / 16, units = src.units();
-  Streamer<T, ND, 16, 4, 16> s;
+  Streamer<T, ND, kD, 16> s(smem);
   s.prologue(src, units > 0 ? tiles : 0, units > 0 ? units : 1);  // weights only: they do not wait for h
   if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
     if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
@@ -375,20 +394,15 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + 16 * tile + row;
     if (n < r1) store(n, col, sum(row, col) + sum(row, col + 4 * ND));
-  }, part);
-}
-
-size_t moe_part_bytes(int experts) {
-  const size_t route = sizeof(uint32_t) * kMoeTokens * experts + experts;
-  const size_t stream = part_bytes<1>();  // the same for 1, 2 and 4 column tiles
-  static_assert(part_bytes<1>() == part_bytes<2>() && part_bytes<1>() == part_bytes<4>(), "one size for every plan");
-  return route > stream ? route : stream;
+  });
 }
 
 template <typename T, int NT, int ND>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND>);
-  const size_t smem = moe_part_bytes(a.experts);
+  constexpr size_t smem = stream_bytes<ND, moe_depth<ND>()>();
+  static_assert(smem >= stream_bytes<NT, moe_depth<ND>()>() &&
+                smem >= (sizeof(uint32_t) * kMoeTokens + 1) * kMoeExperts, "shared-memory plan");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);

@@ -97,8 +97,8 @@ SHARED = dict(shared_inter=16, shared_gate_dev=0x800000, shared_up_dev=0x810000,
     (dict(router_w_dev=None), "no routing"), (dict(ids_dev=0x900000), "given routing"),
     (dict(ids_dev=0x900000, weights_dev=0x910000), "given routing"),
     (dict(router_w_dev=None, ids_dev=0x900000, weights_dev=0x910000, ids_out_dev=0x920000), "not written"),
-    (dict(x_dev=0x400010), "32-byte"), (dict(down_dev=0x300008), "32-byte"), (dict(ldx=72), "32-byte"),
-    (dict(SHARED, shared_gate_vec_dev=0x830002), "32-byte"), (dict(out_dev=0x600001), "2-byte"),
+    (dict(x_dev=0x400008), "16-byte"), (dict(down_dev=0x300008), "16-byte"), (dict(ldx=68), "16-byte"),
+    (dict(SHARED, shared_gate_vec_dev=0x830002), "16-byte"), (dict(out_dev=0x600001), "2-byte"),
     (dict(ids_out_dev=0x900004), "8-byte"), (dict(ldx=48), "apart"), (dict(ldo=63), "apart"),
     (dict(residual_dev=0x900000, ldr=32), "apart"), (dict(workspace_dev=0x700010), "workspace"),
     (dict(workspace_bytes=100), "workspace"), (dict(out_dev=0x400080), "overlaps"), (dict(out_dev=0x100100), "overlaps"),

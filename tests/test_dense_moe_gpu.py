@@ -141,11 +141,11 @@ def test_strided_rows_in_place_and_repeats(tokens, cuda_device):
     want = layer.forward_x(x, wr, residual=r)
     for _ in range(5):
         assert torch.equal(layer.forward_x(x, wr, residual=r), want)
-    wide = torch.full((tokens + 2, 256 + 48), float("nan"), dtype=BF16, device=cuda_device)
-    wide[1:-1, 16:272] = x
+    wide = torch.full((tokens + 2, 256 + 40), float("nan"), dtype=BF16, device=cuda_device)
+    wide[1:-1, 8:264] = x
     buf = torch.full((tokens + 2, 259), 7.0, dtype=BF16, device=cuda_device)
     out = buf[1:-1, 1:257]
-    layer.forward_x(wide[1:-1, 16:272], wr, residual=r, out=out)
+    layer.forward_x(wide[1:-1, 8:264], wr, residual=r, out=out)
     assert torch.equal(out, want)
     out.fill_(7.0)
     assert bool((buf == 7.0).all()), "wrote outside its rows"
@@ -219,10 +219,10 @@ def test_no_tokens_and_refusals(cuda_device):
         layer.experts_forward(x, torch.zeros(4, 2, dtype=torch.int64, device=cuda_device), torch.ones(4, 2, device=cuda_device))
     with pytest.raises(ValueError, match="offload_mask"):
         layer.forward_x(x, wr, offload_mask=torch.ones(7, dtype=torch.bool, device=cuda_device))
-    with pytest.raises(MoeError, match="32-byte"):
-        layer.forward_x(rnd(cuda_device, 1, 4, 72)[:, 8:], wr)
-    with pytest.raises(MoeError, match="32-byte"):
-        layer.forward_x(rnd(cuda_device, 1, 4, 72)[:, :64], wr)
+    with pytest.raises(MoeError, match="16-byte"):
+        layer.forward_x(rnd(cuda_device, 1, 4, 72)[:, 4:68], wr)
+    with pytest.raises(MoeError, match="16-byte"):
+        layer.forward_x(rnd(cuda_device, 1, 4, 68)[:, :64], wr)
     buf = rnd(cuda_device, 1, 5, 64)
     with pytest.raises(MoeError, match="overlaps"):
         layer.forward_x(buf[:4], wr, out=buf[1:])
