@@ -100,32 +100,32 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 template <bool GATED, int NT>
 struct LinearSrc {
+  static constexpr bool kWhole = false;
   const LinearArgs& a;
-  int r0, r1, g, t8;
+  int r0, r1, q, t8;
   const uint16_t* xrow[NT];
   MOE_DEV LinearSrc(const LinearArgs& args, int lo, int hi) : a(args), r0(lo), r1(hi) {
-    const int lane = threadIdx.x & 31;
-    g = lane >> 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    q = lane >> 3;
     t8 = 8 * (lane & 3);
 #pragma unroll
     for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.m ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
+  MOE_DEV int halves() const { return (a.k + 31) / 32; }
   MOE_DEV const uint16_t* any() const { return a.w; }
-  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
-    const int k = unit * 64;
-    len = a.k - k;
+  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
+    const int k = 32 * half;
+    n = a.k - k;
     if constexpr (GATED) {
-      const int r = r0 + 8 * tile + g;
-      pa = r < r1 ? a.w + r * a.ldw + k : nullptr;
-      pb = r < r1 ? a.w_up + r * a.ldwu + k : nullptr;
+      const int r = r0 + 8 * tile + q + 4 * (i & 1);
+      p = r < r1 ? (i < 2 ? a.w + r * a.ldw : a.w_up + r * a.ldwu) + k : nullptr;
     } else {
-      const int r = r0 + 16 * tile + g;
-      pa = r < r1 ? a.w + r * a.ldw + k : nullptr;
-      pb = r + 8 < r1 ? a.w + (r + 8) * a.ldw + k : nullptr;
+      const int r = r0 + 16 * tile + q + 4 * i;
+      p = r < r1 ? a.w + r * a.ldw + k : nullptr;
     }
   }
-  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
-    const int k = unit * 64;
+  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
+    const int k = 32 * half;
     const uint4 z = make_uint4(0, 0, 0, 0);
     x0 = xrow[j] != nullptr && k + t8 < a.k ? ld_tokens(xrow[j] + k) : z;
     x1 = xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
@@ -136,18 +136,18 @@ constexpr int kLinearDepth = 4;
 
 template <typename T, bool GATED, int NT>
 __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __grid_constant__ LinearArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   // A launch that may start early reads nothing before its predecessor is done
   // (weights too: they may be that kernel's output), and lets none start early.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int r0 = static_cast<int>(static_cast<int64_t>(a.n) * blockIdx.x / gridDim.x);
   const int r1 = static_cast<int>(static_cast<int64_t>(a.n) * (blockIdx.x + 1) / gridDim.x);
   constexpr int kRows = GATED ? 8 : 16;
-  const int tiles = (r1 - r0 + kRows - 1) / kRows, units = (a.k + 63) / 64;
+  const int tiles = (r1 - r0 + kRows - 1) / kRows;
   const LinearSrc<GATED, NT> src(a, r0, r1);
   Streamer<T, NT, kLinearDepth, kRows> s(smem);
-  s.prologue(src, tiles, units);
-  s.run(src, tiles, units, a.m, [&](int tile, int row, int col, auto sum) {
+  s.prologue(src, tiles);
+  s.run(src, a.m, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + kRows * tile + row;
     if (n >= r1) return;
     float v = sum(row, col);

@@ -171,37 +171,35 @@ struct Tables {
 // multiples of 16), rows outside the block's range masked.
 template <int NT>
 struct GateUpSrc {
+  static constexpr bool kWhole = false;
   const MoeArgs& a;
   const Tables& tb;
-  int lo, hi, routed, g, t8;
+  int lo, hi, routed, q, t8;
   const uint16_t* xrow[NT];
   MOE_DEV GateUpSrc(const MoeArgs& args, const Tables& tables, int lo_, int hi_)
       : a(args), tb(tables), lo(lo_), hi(hi_), routed(tables.n_active * args.inter) {
-    const int lane = threadIdx.x & 31;
-    g = lane >> 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    q = lane >> 3;
     t8 = 8 * (lane & 3);
 #pragma unroll
     for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
+  MOE_DEV int halves() const { return (a.hidden + 31) / 32; }
   MOE_DEV const uint16_t* any() const { return a.gate; }
-  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
-    const int k = unit * 64, v0 = (lo / 8 + tile) * 8, v = v0 + g;
-    len = a.hidden - k;
-    pa = pb = nullptr;
+  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
+    const int k = 32 * half, v0 = (lo / 8 + tile) * 8, v = v0 + q + 4 * (i & 1);
+    n = a.hidden - k;
+    p = nullptr;
     if (v < lo || v >= hi) return;
     if (v0 < routed) {
       const int s = v0 / a.inter;
-      const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden + k;
-      pa = a.gate + at;
-      pb = a.up + at;
+      p = (i < 2 ? a.gate : a.up) + (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden + k;
     } else {
-      const int64_t at = static_cast<int64_t>(v - routed) * a.hidden + k;
-      pa = a.shared_gate + at;
-      pb = a.shared_up + at;
+      p = (i < 2 ? a.shared_gate : a.shared_up) + static_cast<int64_t>(v - routed) * a.hidden + k;
     }
   }
-  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
-    const int k = unit * 64;
+  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
+    const int k = 32 * half;
     const uint4 z = make_uint4(0, 0, 0, 0);
     x0 = xrow[j] != nullptr && k + t8 < a.hidden ? ld_tokens(xrow[j] + k) : z;
     x1 = xrow[j] != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow[j] + k + 32) : z;
@@ -212,39 +210,35 @@ struct GateUpSrc {
 // expert's.  Columns: hi of token c for c < half, then lo of token c - half.
 template <int NT>
 struct DownSrc {
+  static constexpr bool kWhole = true;  // a step of 64 elements lies in one expert
   static constexpr int kHalf = 4 * NT;
   const MoeArgs& a;
   const Tables& tb;
-  int r0, r1, ue, routed_units, g, t8;
+  int r0, r1, ue, routed_units, q, g, t8;
   MOE_DEV DownSrc(const MoeArgs& args, const Tables& tables, int lo, int hi) : a(args), tb(tables), r0(lo), r1(hi) {
     const int lane = threadIdx.x & 31;
+    q = lane >> 3;
     g = lane >> 2;
     t8 = 8 * (lane & 3);
     ue = (a.inter + 63) / 64;
     routed_units = tables.n_active * ue;
   }
-  MOE_DEV int units() const { return routed_units + (a.shared_inter + 63) / 64; }
+  MOE_DEV int halves() const { return 2 * (routed_units + (a.shared_inter + 63) / 64); }
   MOE_DEV const uint16_t* any() const { return a.down; }
-  MOE_DEV void rows(int tile, int unit, const uint16_t*& pa, const uint16_t*& pb, int& len) const {
-    const int r = r0 + 16 * tile + g;
-    const uint16_t* base;
-    int k, ld;
+  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
+    const int r = r0 + 16 * tile + q + 4 * i, unit = half / 2;
     if (unit < routed_units) {
-      const int s = unit / ue;
-      k = (unit - s * ue) * 64;
-      ld = a.inter;
-      base = a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter;
+      const int s = unit / ue, k = (unit - s * ue) * 64;
+      n = a.inter - k;
+      p = r < r1 ? a.down + (static_cast<int64_t>(tb.active[s]) * a.hidden + r) * a.inter + k : nullptr;
     } else {
-      k = (unit - routed_units) * 64;
-      ld = a.shared_inter;
-      base = a.shared_down;
+      const int k = (unit - routed_units) * 64;
+      n = a.shared_inter - k;
+      p = r < r1 ? a.shared_down + static_cast<int64_t>(r) * a.shared_inter + k : nullptr;
     }
-    len = ld - k;
-    pa = r < r1 ? base + static_cast<int64_t>(r) * ld + k : nullptr;
-    pb = r + 8 < r1 ? base + static_cast<int64_t>(r + 8) * ld + k : nullptr;
   }
-  MOE_DEV void tokens(int unit, int j, uint4& x0, uint4& x1) const {
-    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf;
+  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
+    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf, unit = half / 2;
     const uint16_t* p = nullptr;
     int k = 0, len = 0;
     if (tok < a.tokens) {
@@ -283,7 +277,7 @@ constexpr int moe_depth() {
 // NT column tiles hold the tokens of the gate / up phase, ND those of the down phase (hi and lo).
 template <typename T, int NT, int ND>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Tables tb;
   constexpr int kD = moe_depth<ND>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -352,10 +346,10 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   const int lo = static_cast<int>(rows * blockIdx.x / gridDim.x), hi = static_cast<int>(rows * (blockIdx.x + 1) / gridDim.x);
   {
     const GateUpSrc<NT> src(a, tb, lo, hi);
-    const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0, units = (a.hidden + 63) / 64;
+    const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0;
     Streamer<T, NT, kD, 8> s(smem);
-    s.prologue(src, tiles, units);
-    s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
+    s.prologue(src, tiles);
+    s.run(src, a.tokens, [&](int tile, int row, int col, auto sum) {
       const int v0 = (lo / 8 + tile) * 8, v = v0 + row;
       if (v < lo || v >= hi) return;
       if (v0 < src.routed) {
@@ -376,9 +370,9 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   const int r0 = static_cast<int>(static_cast<int64_t>(a.hidden) * blockIdx.x / gridDim.x);
   const int r1 = static_cast<int>(static_cast<int64_t>(a.hidden) * (blockIdx.x + 1) / gridDim.x);
   const DownSrc<ND> src(a, tb, r0, r1);
-  const int tiles = (r1 - r0 + 15) / 16, units = src.units();
+  const bool none = src.halves() == 0;  // every expert masked and no shared expert
   Streamer<T, ND, kD, 16> s(smem);
-  s.prologue(src, units > 0 ? tiles : 0, units > 0 ? units : 1);  // weights only: they do not wait for h
+  s.prologue(src, none ? 0 : (r1 - r0 + 15) / 16);  // weights only: they do not wait for h
   if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
     if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
     return;
@@ -387,11 +381,11 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
     a.out[col * a.ldo + n] = T::from_f32(v);
   };
-  if (units == 0) {  // every expert masked and no shared expert
+  if (none) {
     for (int i = tid; i < (r1 - r0) * a.tokens; i += kSThreads) store(r0 + i % (r1 - r0), i / (r1 - r0), 0.0f);
     return;
   }
-  s.run(src, tiles, units, a.tokens, [&](int tile, int row, int col, auto sum) {
+  s.run(src, a.tokens, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + 16 * tile + row;
     if (n < r1) store(n, col, sum(row, col) + sum(row, col + 4 * ND));
   });
@@ -401,7 +395,7 @@ template <typename T, int NT, int ND>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND>);
   constexpr size_t smem = stream_bytes<ND, moe_depth<ND>()>();
-  static_assert(smem >= stream_bytes<NT, moe_depth<ND>()>() &&
+  static_assert(stream_bytes<NT, moe_depth<ND>()>() <= smem &&
                 smem >= (sizeof(uint32_t) * kMoeTokens + 1) * kMoeExperts, "shared-memory plan");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};

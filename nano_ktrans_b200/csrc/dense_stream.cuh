@@ -3,27 +3,26 @@
 //
 // With a handful of tokens a projection is bound by reading its weights once.
 // A block owns a range of weight rows, cut into tiles of 16 (the mma's M;
-// tokens are its N, 8 per column tile).  K is cut into units of 64 elements,
-// and step s = tile * units + unit goes to warp s % 16: every warp has the same
-// number of steps to within one, whatever the sizes.  In a step lane (g, t) of
-// a warp takes 8 consecutive elements at 8 t and at 32 + 8 t of rows g and g + 8
-// as the mma's A registers and the same K positions of token column g as B: an
-// mma is unchanged by a permutation of K that both operands share, so nothing
-// is shuffled.
+// tokens are its N, 8 per column tile).  The 16 warps split K evenly, in halves
+// of 32 elements, and each walks its part in steps of 64 elements; for a step
+// it takes up to RT tiles one after the other, so a token fragment is loaded
+// once for RT weight tiles (loading it for every tile cost 8 of 31 us at 118
+// MB of weights and 7 tokens: those loads queue behind the weights').  Lane
+// (g, t) feeds the mma with 8 consecutive elements at 8 t and at 32 + 8 t of
+// rows g and g + 8 (A) and of token column g (B): an mma is unchanged by a
+// permutation of K that both operands share, so nothing is shuffled.
 //
-// Weights in flight: every lane copies its own four 16-byte pieces of a step
-// into a ring of D steps in shared memory with cp.async and reads back what it
-// copied itself, so the ring needs no barrier between threads; 16 warps x D x
-// 2 KB = 128 KB per SM are under way (6.5 TB/s x 1 us / 148 SMs is 44 KB).
-// Loading straight into registers instead kept one step in flight, not D: the
-// hardware's scoreboards were shared between the loads (118 MB of weights, 7
-// tokens: 29.5 us; every step of a warp waited out a whole memory latency).
+// Weights in flight: a warp copies a step's 16 rows x 128 bytes into its own
+// ring of D steps in shared memory with cp.async, whole 128-byte lines at a
+// time, and waits for its own copies only; 16 warps x D x 2 KB = 128 KB per SM
+// are under way (6.5 TB/s x 1 us / 148 SMs is 44 KB).  Rows are stored with
+// the 64-byte halves of odd rows swapped, so that the fragment reads (two rows
+// a phase) meet no bank conflict.
 //
-// Partial sums: a warp adds up its steps of a tile in registers, puts the
-// 16 x 8 partial tiles into shared memory, and once per round of tiles the
-// block adds the 16 partials of each output in warp order (no atomics: the
-// same bits every run).  Partials are double buffered, and the next round's
-// copies are in flight meanwhile.
+// Partial sums: a warp keeps RT tiles in registers over its part of K, puts the
+// 16 x 8 partial tiles into shared memory, and the block adds the 16 partials
+// of each output in warp order (no atomics: the same bits every run) while the
+// next tiles' copies are in flight.
 #pragma once
 
 #include "dense_common.cuh"
@@ -66,148 +65,166 @@ MOE_DEV uint4 ld_l2(const uint16_t* p) {
 
 constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
-// Tiles whose partials one round holds.
+// Tiles a warp keeps in registers.
 template <int NT>
 constexpr int round_tiles() {
-  return NT == 1 ? 2 : 1;
-}
-template <int NT>
-constexpr int part_floats() {
-  return 2 * round_tiles<NT>() * kSW * NT * kPartTile;
+  return NT >= 4 ? 2 : 4 / NT;
 }
 // Dynamic shared memory of a Streamer: the ring, then the partials.
 template <int NT, int D>
 constexpr size_t stream_bytes() {
-  return static_cast<size_t>(kSW) * D * kStepBytes + sizeof(float) * part_floats<NT>();
+  return static_cast<size_t>(kSW) * D * kStepBytes + sizeof(float) * round_tiles<NT>() * kSW * NT * kPartTile;
 }
 
 // NT column tiles of 8 tokens, D steps in flight.
-//   src.rows(tile, unit, pa, pb, len)  rows g and g + 8 of the tile at the unit's first element (null: zeros), and the
-//                                      elements from there to the end of the row
-//   src.tokens(unit, j, x0, x1)        column 8 j + g at 8 t and 32 + 8 t of the unit (zeros outside)
-//   fin(tile, row, col, sum)           one output; sum(row, col) adds the partials
+//   src.halves()                  K in halves of 32 elements; Src::kWhole: a warp's part starts on an even half
+//   src.row(tile, half, i, p, n)  row (lane / 8) + 4 i of the tile at the half's first element (null: zeros), and the
+//                                 elements from there to the row's end
+//   src.tokens(half, j, x0, x1)   column 8 j + g at 8 t and 32 + 8 t from the half's first element (zeros outside)
+//   fin(tile, row, col, sum)      one output; sum(row, col) adds the partials
 // FROWS outputs per column and tile (16, or 8 where rows g and g + 8 belong to
 // one output), `cols` columns.
 template <typename T, int NT, int D, int FROWS>
 struct Streamer {
-  static constexpr int R = round_tiles<NT>();
-  uint32_t ring;  // this lane's 16 bytes of the warp's first piece
+  static constexpr int RT = round_tiles<NT>();
+  uint32_t ring;      // the warp's ring
   float* part;
-  int lt, lu;     // next step to load
+  int h0, h1, steps;  // the warp's halves and steps
+  int tiles;
+  int lb, ls, li;     // next to load: first tile of its round, step, tile within the round
 
   MOE_DEV explicit Streamer(unsigned char* smem) {
-    const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    ring = base + (threadIdx.x >> 5) * (D * kStepBytes) + (threadIdx.x & 31) * 16;
+    ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * (D * kStepBytes);
     part = reinterpret_cast<float*>(smem + kSW * D * kStepBytes);
-  }
-
-  static MOE_DEV void step(int& t, int& u, int units) {
-    u += kSW;
-    while (u >= units) {
-      u -= units;
-      ++t;
-    }
   }
 
   // One group, empty past the last step, so that the groups count the steps.
   template <class Src>
-  MOE_DEV void load(const Src& src, int slot, int tiles, int units) {
-    if (lt < tiles) {
-      const uint16_t *pa, *pb;
-      int len;
-      src.rows(lt, lu, pa, pb, len);
-      const int t8 = 8 * (threadIdx.x & 3);
-      const uint32_t dst = ring + slot * kStepBytes;
-      const uint16_t* safe = src.any();
-      const bool in0 = t8 < len, in1 = 32 + t8 < len;
-      copy16(dst, pa != nullptr && in0 ? pa + t8 : safe, pa != nullptr && in0);
-      copy16(dst + 512, pb != nullptr && in0 ? pb + t8 : safe, pb != nullptr && in0);
-      copy16(dst + 1024, pa != nullptr && in1 ? pa + 32 + t8 : safe, pa != nullptr && in1);
-      copy16(dst + 1536, pb != nullptr && in1 ? pb + 32 + t8 : safe, pb != nullptr && in1);
-      step(lt, lu, units);
+  MOE_DEV void load(const Src& src, int slot) {
+    if (lb < tiles && ls < steps) {
+      const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3, h = h0 + 2 * ls;
+      // the second half of a warp's last step may belong to the next warp
+      const bool mine = piece < 4 || h + 1 < h1;
+      const uint32_t dst = ring + slot * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t* p;
+        int n;
+        src.row(lb + li, h, i, p, n);
+        const bool take = p != nullptr && 8 * piece < n && mine;
+        copy16(dst + i * 512, take ? p + 8 * piece : src.any(), take);
+      }
+      if (++li == min(RT, tiles - lb)) {
+        li = 0;
+        if (++ls == steps) {
+          ls = 0;
+          lb += RT;
+        }
+      }
     }
     copy_commit();
   }
 
   template <class Src>
-  MOE_DEV void prologue(const Src& src, int tiles, int units) {
-    lt = 0;
-    lu = (threadIdx.x >> 5) - kSW;
-    step(lt, lu, units);
+  MOE_DEV void prologue(const Src& src, int n_tiles) {
+    const int warp = threadIdx.x >> 5, halves = src.halves();
+    h0 = static_cast<int>(static_cast<int64_t>(halves) * warp / kSW);
+    h1 = static_cast<int>(static_cast<int64_t>(halves) * (warp + 1) / kSW);
+    if constexpr (Src::kWhole) {
+      h0 = (h0 + 1) & ~1;
+      h1 = warp == kSW - 1 ? halves : (h1 + 1) & ~1;
+    }
+    steps = h1 > h0 ? (h1 - h0 + 1) / 2 : 0;
+    tiles = n_tiles;
+    lb = ls = li = 0;
 #pragma unroll
-    for (int i = 0; i < D; ++i) load(src, i, tiles, units);
+    for (int i = 0; i < D; ++i) load(src, i);
   }
 
   template <class Src, class Fin>
-  MOE_DEV void run(const Src& src, int tiles, int units, int cols, const Fin& fin) {
+  MOE_DEV void run(const Src& src, int cols, const Fin& fin) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    int ct = 0, cu = warp - kSW;
-    step(ct, cu, units);
-    float acc[NT][4];
-    int cur = -1, round = 0, slot = 0;
-    auto place = [&](int tile, int w) {
-      return part + static_cast<size_t>((((tile / R) & 1) * R + tile % R) * kSW + w) * (NT * kPartTile);
-    };
-    auto flush = [&]() {
-      if (cur < 0) return;
-      float* p = place(cur, warp);
+    const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
+    const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
+    int slot = 0;
+    for (int base = 0; base < tiles; base += RT) {
+      const int nt = min(RT, tiles - base);
+      float acc[RT][NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float* q = p + j * kPartTile + 2 * t4 * kPartCol + g;
-        q[0] = acc[j][0];
-        q[kPartCol] = acc[j][1];
-        q[8] = acc[j][2];
-        q[kPartCol + 8] = acc[j][3];
-      }
-    };
-    auto end_round = [&]() {
-      __syncthreads();
-      const int t0 = round * R, nt = min(R, tiles - t0), per = FROWS * cols;
-      for (int i = threadIdx.x; i < nt * per; i += kSThreads) {
-        const int tl = i / per, rc = i - tl * per, col = rc / FROWS, row = rc % FROWS, tile = t0 + tl;
-        // warps that have a step of this tile: all of them once a tile has 16 units
-        const int first = static_cast<int>((static_cast<int64_t>(tile) * units) % kSW);
-        fin(tile, row, col, [&](int r, int c) {
-          const float* p = place(tile, 0) + (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
-          float s = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kSW; ++w)
-            if (units >= kSW || ((w - first + kSW) & (kSW - 1)) < units) s += p[w * (NT * kPartTile)];
-          return s;
-        });
-      }
-      ++round;
-    };
-    while (ct < tiles) {
-      if (ct != cur) {
-        flush();
-        cur = ct;
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[j][c] = 0.0f;
-        while (ct >= (round + 1) * R) end_round();
-      }
-      uint4 x[NT][2];
+          for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
+      uint4 next[NT][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) src.tokens(cu, j, x[j][0], x[j][1]);
-      copy_wait<D - 1>();
-      const uint32_t from = ring + slot * kStepBytes;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 wa = ld_shared(from + 1024 * h), wb = ld_shared(from + 1024 * h + 512);
+      for (int j = 0; j < NT; ++j) next[j][0] = next[j][1] = make_uint4(0, 0, 0, 0);
+      auto fetch = [&](int s) {
+        const int h = h0 + 2 * s;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          T::mma(acc[j], wa.x, wb.x, wa.y, wb.y, x[j][h].x, x[j][h].y);
-          T::mma(acc[j], wa.z, wb.z, wa.w, wb.w, x[j][h].z, x[j][h].w);
+          src.tokens(h, j, next[j][0], next[j][1]);
+          if (h + 1 >= h1) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
+        }
+      };
+      if (steps > 0) fetch(0);
+      for (int s = 0; s < steps; ++s) {
+        uint4 x[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          x[j][0] = next[j][0];
+          x[j][1] = next[j][1];
+        }
+        if (s + 1 < steps) fetch(s + 1);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          if (i < nt) {
+            copy_wait<D - 1>();
+            __syncwarp();
+            const uint32_t from = ring + slot * kStepBytes;
+            const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
+            const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
+              T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
+              T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
+              T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
+            }
+            __syncwarp();  // every lane has read the slot
+            load(src, slot);
+            slot = slot + 1 == D ? 0 : slot + 1;
+          }
         }
       }
-      load(src, slot, tiles, units);
-      slot = slot + 1 == D ? 0 : slot + 1;
-      step(ct, cu, units);
+      if (base > 0) __syncthreads();  // the last round's partials have been added
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (i < nt) {
+          float* p = part + (i * kSW + warp) * (NT * kPartTile) + 2 * t4 * kPartCol + g;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            float* q = p + j * kPartTile;
+            q[0] = acc[i][j][0];
+            q[kPartCol] = acc[i][j][1];
+            q[8] = acc[i][j][2];
+            q[kPartCol + 8] = acc[i][j][3];
+          }
+        }
+      }
+      __syncthreads();
+      const int per = FROWS * cols;
+      for (int o = threadIdx.x; o < nt * per; o += kSThreads) {
+        const int tl = o / per, rc = o - tl * per, col = rc / FROWS, row = rc % FROWS;
+        fin(base + tl, row, col, [&](int r, int c) {
+          const float* p = part + tl * kSW * (NT * kPartTile) + (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kSW; ++w) v += p[w * (NT * kPartTile)];
+          return v;
+        });
+      }
     }
-    flush();
-    while (round * R < tiles) end_round();
   }
 };
 
