@@ -101,6 +101,13 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 template <bool GATED, int NT>
 struct LinearSrc {
   static constexpr bool kWhole = false;
+  struct Tile {
+    const uint16_t *p, *u;  // this lane's first row, of each weight when gated
+    int left;               // rows from there to the block's end
+  };
+  struct Step {
+    int k;
+  };
   const LinearArgs& a;
   int r0, r1, q, t8;
   const uint16_t* xrow[NT];
@@ -113,26 +120,24 @@ struct LinearSrc {
   }
   MOE_DEV int halves() const { return (a.k + 31) / 32; }
   MOE_DEV const uint16_t* any() const { return a.w; }
-  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
-    const int k = 32 * half;
-    n = a.k - k;
-    if constexpr (GATED) {
-      const int r = r0 + 8 * tile + q + 4 * (i & 1);
-      p = r < r1 ? (i < 2 ? a.w + r * a.ldw : a.w_up + r * a.ldwu) + k : nullptr;
-    } else {
-      const int r = r0 + 16 * tile + q + 4 * i;
-      p = r < r1 ? a.w + r * a.ldw + k : nullptr;
-    }
+  MOE_DEV Tile tile(int i) const {
+    const int r = r0 + (GATED ? 8 : 16) * i + q;
+    return {a.w + r * a.ldw, GATED ? a.w_up + r * a.ldwu : nullptr, r1 - r};
   }
-  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
-    const int k = 32 * half;
+  MOE_DEV Step step(int half) const { return {32 * half}; }
+  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
+    n = a.k - s.k;
+    if constexpr (GATED)
+      p = t.left > 4 * (i & 1) ? (i < 2 ? t.p + (i & 1) * 4 * a.ldw : t.u + (i & 1) * 4 * a.ldwu) + s.k : nullptr;
+    else
+      p = t.left > 4 * i ? t.p + 4 * i * a.ldw + s.k : nullptr;
+  }
+  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = xrow[j] != nullptr && k + t8 < a.k ? ld_tokens(xrow[j] + k) : z;
-    x1 = xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
+    x0 = xrow[j] != nullptr && s.k + t8 < a.k ? ld_tokens(xrow[j] + s.k) : z;
+    x1 = xrow[j] != nullptr && s.k + 32 + t8 < a.k ? ld_tokens(xrow[j] + s.k + 32) : z;
   }
 };
-
-constexpr int kLinearDepth = 4;
 
 template <typename T, bool GATED, int NT>
 __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __grid_constant__ LinearArgs a) {
@@ -145,9 +150,9 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
   constexpr int kRows = GATED ? 8 : 16;
   const int tiles = (r1 - r0 + kRows - 1) / kRows;
   const LinearSrc<GATED, NT> src(a, r0, r1);
-  Streamer<T, NT, kLinearDepth, kRows> s(smem);
-  s.prologue(src, tiles);
-  s.run(src, a.m, [&](int tile, int row, int col, auto sum) {
+  Streamer<T, NT, kRows, LinearSrc<GATED, NT>> s(src, smem);
+  s.prologue(tiles);
+  s.run(a.m, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + kRows * tile + row;
     if (n >= r1) return;
     float v = sum(row, col);
@@ -165,7 +170,7 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
 template <typename T, bool GATED, int NT>
 static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT>);
-  constexpr size_t smem = stream_bytes<NT, kLinearDepth>();
+  constexpr size_t smem = kStreamBytes;
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.n < sms ? a.n : sms);

@@ -172,6 +172,13 @@ struct Tables {
 template <int NT>
 struct GateUpSrc {
   static constexpr bool kWhole = false;
+  struct Tile {
+    const uint16_t *g, *u;  // this lane's first gate and up row
+    bool first, second;     // whether that row and the one 4 below are this block's
+  };
+  struct Step {
+    int k;
+  };
   const MoeArgs& a;
   const Tables& tb;
   int lo, hi, routed, q, t8;
@@ -186,23 +193,30 @@ struct GateUpSrc {
   }
   MOE_DEV int halves() const { return (a.hidden + 31) / 32; }
   MOE_DEV const uint16_t* any() const { return a.gate; }
-  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
-    const int k = 32 * half, v0 = (lo / 8 + tile) * 8, v = v0 + q + 4 * (i & 1);
-    n = a.hidden - k;
-    p = nullptr;
-    if (v < lo || v >= hi) return;
+  MOE_DEV Tile tile(int i) const {
+    const int v0 = (lo / 8 + i) * 8, v = v0 + q;
+    Tile t{a.gate, a.up, v >= lo && v < hi, v + 4 >= lo && v + 4 < hi};
     if (v0 < routed) {
       const int s = v0 / a.inter;
-      p = (i < 2 ? a.gate : a.up) + (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden + k;
+      const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden;
+      t.g = a.gate + at;
+      t.u = a.up + at;
     } else {
-      p = (i < 2 ? a.shared_gate : a.shared_up) + static_cast<int64_t>(v - routed) * a.hidden + k;
+      const int64_t at = static_cast<int64_t>(v - routed) * a.hidden;
+      t.g = a.shared_gate + at;
+      t.u = a.shared_up + at;
     }
+    return t;
   }
-  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
-    const int k = 32 * half;
+  MOE_DEV Step step(int half) const { return {32 * half}; }
+  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
+    n = a.hidden - s.k;
+    p = ((i & 1) ? t.second : t.first) ? (i < 2 ? t.g : t.u) + (i & 1) * 4 * a.hidden + s.k : nullptr;
+  }
+  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = xrow[j] != nullptr && k + t8 < a.hidden ? ld_tokens(xrow[j] + k) : z;
-    x1 = xrow[j] != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow[j] + k + 32) : z;
+    x0 = xrow[j] != nullptr && s.k + t8 < a.hidden ? ld_tokens(xrow[j] + s.k) : z;
+    x1 = xrow[j] != nullptr && s.k + 32 + t8 < a.hidden ? ld_tokens(xrow[j] + s.k + 32) : z;
   }
 };
 
@@ -212,6 +226,13 @@ template <int NT>
 struct DownSrc {
   static constexpr bool kWhole = true;  // a step of 64 elements lies in one expert
   static constexpr int kHalf = 4 * NT;
+  struct Tile {
+    int row, left;  // this lane's first row, rows from there to the block's end
+  };
+  struct Step {
+    const uint16_t* w;  // row 0 of the expert at the step's first element
+    int ld, k, slot;    // row length, place in the row, place in the active list (-1: shared)
+  };
   const MoeArgs& a;
   const Tables& tb;
   int r0, r1, ue, routed_units, q, g, t8;
@@ -225,37 +246,28 @@ struct DownSrc {
   }
   MOE_DEV int halves() const { return 2 * (routed_units + (a.shared_inter + 63) / 64); }
   MOE_DEV const uint16_t* any() const { return a.down; }
-  MOE_DEV void row(int tile, int half, int i, const uint16_t*& p, int& n) const {
-    const int r = r0 + 16 * tile + q + 4 * i, unit = half / 2;
+  MOE_DEV Tile tile(int i) const { return {r0 + 16 * i + q, r1 - (r0 + 16 * i + q)}; }
+  MOE_DEV Step step(int half) const {
+    const int unit = half / 2;
     if (unit < routed_units) {
       const int s = unit / ue, k = (unit - s * ue) * 64;
-      n = a.inter - k;
-      p = r < r1 ? a.down + (static_cast<int64_t>(tb.active[s]) * a.hidden + r) * a.inter + k : nullptr;
-    } else {
-      const int k = (unit - routed_units) * 64;
-      n = a.shared_inter - k;
-      p = r < r1 ? a.shared_down + static_cast<int64_t>(r) * a.shared_inter + k : nullptr;
+      return {a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter + k, a.inter, k, s};
     }
+    const int k = (unit - routed_units) * 64;
+    return {a.shared_down + k, a.shared_inter, k, -1};
   }
-  MOE_DEV void tokens(int half, int j, uint4& x0, uint4& x1) const {
-    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf, unit = half / 2;
-    const uint16_t* p = nullptr;
-    int k = 0, len = 0;
-    if (tok < a.tokens) {
-      if (unit < routed_units) {
-        const int s = unit / ue, pair = tb.pair[s][tok];
-        k = (unit - s * ue) * 64 + t8;
-        len = pair >= 0 ? a.inter : 0;
-        p = a.h + static_cast<int64_t>(2 * pair + part) * a.inter + k;
-      } else {
-        k = (unit - routed_units) * 64 + t8;
-        len = a.shared_inter;
-        p = a.h_shared + static_cast<int64_t>(2 * tok + part) * a.shared_inter + k;
-      }
-    }
+  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
+    n = s.ld - s.k;
+    p = t.left > 4 * i ? s.w + static_cast<int64_t>(t.row + 4 * i) * s.ld : nullptr;
+  }
+  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
+    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf, k = s.k + t8;
+    int pair = -1;
+    if (tok < a.tokens) pair = s.slot < 0 ? tok : tb.pair[s.slot][tok];
+    const uint16_t* p = (s.slot < 0 ? a.h_shared : a.h) + static_cast<int64_t>(2 * pair + part) * s.ld + k;
     const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = k < len ? ld_l2(p) : z;
-    x1 = k + 32 < len ? ld_l2(p + 32) : z;
+    x0 = pair >= 0 && k < s.ld ? ld_l2(p) : z;
+    x1 = pair >= 0 && k + 32 < s.ld ? ld_l2(p + 32) : z;
   }
 };
 
@@ -268,18 +280,11 @@ MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
 }
 
-// Steps in flight: four column tiles of partials leave room for three.
-template <int ND>
-constexpr int moe_depth() {
-  return ND == 4 ? 3 : 4;
-}
-
 // NT column tiles hold the tokens of the gate / up phase, ND those of the down phase (hi and lo).
 template <typename T, int NT, int ND>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Tables tb;
-  constexpr int kD = moe_depth<ND>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -347,9 +352,9 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   {
     const GateUpSrc<NT> src(a, tb, lo, hi);
     const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0;
-    Streamer<T, NT, kD, 8> s(smem);
-    s.prologue(src, tiles);
-    s.run(src, a.tokens, [&](int tile, int row, int col, auto sum) {
+    Streamer<T, NT, 8, GateUpSrc<NT>> s(src, smem);
+    s.prologue(tiles);
+    s.run(a.tokens, [&](int tile, int row, int col, auto sum) {
       const int v0 = (lo / 8 + tile) * 8, v = v0 + row;
       if (v < lo || v >= hi) return;
       if (v0 < src.routed) {
@@ -371,8 +376,8 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   const int r1 = static_cast<int>(static_cast<int64_t>(a.hidden) * (blockIdx.x + 1) / gridDim.x);
   const DownSrc<ND> src(a, tb, r0, r1);
   const bool none = src.halves() == 0;  // every expert masked and no shared expert
-  Streamer<T, ND, kD, 16> s(smem);
-  s.prologue(src, none ? 0 : (r1 - r0 + 15) / 16);  // weights only: they do not wait for h
+  Streamer<T, ND, 16, DownSrc<ND>> s(src, smem);
+  s.prologue(none ? 0 : (r1 - r0 + 15) / 16);  // weights only: they do not wait for h
   if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
     if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
     return;
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     for (int i = tid; i < (r1 - r0) * a.tokens; i += kSThreads) store(r0 + i % (r1 - r0), i / (r1 - r0), 0.0f);
     return;
   }
-  s.run(src, a.tokens, [&](int tile, int row, int col, auto sum) {
+  s.run(a.tokens, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + 16 * tile + row;
     if (n < r1) store(n, col, sum(row, col) + sum(row, col + 4 * ND));
   });
@@ -394,9 +399,8 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
 template <typename T, int NT, int ND>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND>);
-  constexpr size_t smem = stream_bytes<ND, moe_depth<ND>()>();
-  static_assert(stream_bytes<NT, moe_depth<ND>()>() <= smem &&
-                smem >= (sizeof(uint32_t) * kMoeTokens + 1) * kMoeExperts, "shared-memory plan");
+  constexpr size_t smem = kStreamBytes;
+  static_assert((sizeof(uint32_t) * kMoeTokens + 1) * kMoeExperts <= smem, "routing scratch");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);

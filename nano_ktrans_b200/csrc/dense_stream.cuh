@@ -12,12 +12,15 @@
 // rows g and g + 8 (A) and of token column g (B): an mma is unchanged by a
 // permutation of K that both operands share, so nothing is shuffled.
 //
-// Weights in flight: a warp copies a step's 16 rows x 128 bytes into its own
-// ring of D steps in shared memory with cp.async, whole 128-byte lines at a
-// time, and waits for its own copies only; 16 warps x D x 2 KB = 128 KB per SM
-// are under way (6.5 TB/s x 1 us / 148 SMs is 44 KB).  Rows are stored with
-// the 64-byte halves of odd rows swapped, so that the fragment reads (two rows
-// a phase) meet no bank conflict.
+// Weights in flight: a warp copies a step's 16 rows x 128 bytes of each tile
+// into its own ring of D = PD x RT slots in shared memory with cp.async, whole
+// 128-byte lines at a time, PD steps ahead, and waits for its own copies only;
+// 16 warps x D x 2 KB = 128 KB per SM are under way (6.5 TB/s x 1 us / 148 SMs
+// is 44 KB).  Rows are stored with the 64-byte halves of odd rows swapped, so
+// that the fragment reads (two rows a phase) meet no bank conflict.  Addresses
+// are split into a part per tile (kept in registers for a round of RT tiles)
+// and a part per step, so that a slot costs a few tens of instructions: with
+// both worked out per slot the issue slots, not the memory, were the limit.
 //
 // Partial sums: a warp keeps RT tiles in registers over its part of K, puts the
 // 16 x 8 partial tiles into shared memory, and the block adds the 16 partials
@@ -65,68 +68,78 @@ MOE_DEV uint4 ld_l2(const uint16_t* p) {
 
 constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
-// Tiles a warp keeps in registers.
+// Tiles a warp keeps in registers, and steps it copies ahead.
 template <int NT>
 constexpr int round_tiles() {
-  return NT >= 4 ? 2 : 4 / NT;
+  return 4 / NT;
 }
-// Dynamic shared memory of a Streamer: the ring, then the partials.
-template <int NT, int D>
-constexpr size_t stream_bytes() {
-  return static_cast<size_t>(kSW) * D * kStepBytes + sizeof(float) * round_tiles<NT>() * kSW * NT * kPartTile;
+template <int NT>
+constexpr int steps_ahead() {
+  return NT;
 }
+// Dynamic shared memory of a Streamer: the ring of four slots a warp, then the partials.
+constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * 4 * kStepBytes + sizeof(float) * 4 * kSW * kPartTile;
 
-// NT column tiles of 8 tokens, D steps in flight.
-//   src.halves()                  K in halves of 32 elements; Src::kWhole: a warp's part starts on an even half
-//   src.row(tile, half, i, p, n)  row (lane / 8) + 4 i of the tile at the half's first element (null: zeros), and the
-//                                 elements from there to the row's end
-//   src.tokens(half, j, x0, x1)   column 8 j + g at 8 t and 32 + 8 t from the half's first element (zeros outside)
-//   fin(tile, row, col, sum)      one output; sum(row, col) adds the partials
+// NT column tiles of 8 tokens (1, 2 or 4).  Src:
+//   halves()                  K in halves of 32 elements; kWhole: a warp's part starts on an even half
+//   Tile tile(int)            what copying a tile's rows needs, rows (lane / 8) + 4 i
+//   Step step(int half)       what a step needs: where it is in K
+//   row(Tile, Step, i, p, n)  row i's address at the step's first element (null: zeros), elements from there to its end
+//   tokens(Step, j, x0, x1)   column 8 j + g at 8 t and 32 + 8 t of the step (zeros outside)
+//   fin(tile, row, col, sum)  one output; sum(row, col) adds the partials
 // FROWS outputs per column and tile (16, or 8 where rows g and g + 8 belong to
 // one output), `cols` columns.
-template <typename T, int NT, int D, int FROWS>
+template <typename T, int NT, int FROWS, class Src>
 struct Streamer {
-  static constexpr int RT = round_tiles<NT>();
+  static constexpr int RT = round_tiles<NT>(), PD = steps_ahead<NT>(), D = RT * PD;
+  using Tile = typename Src::Tile;
+  using Step = typename Src::Step;
+  const Src& src;
   uint32_t ring;      // the warp's ring
   float* part;
   int h0, h1, steps;  // the warp's halves and steps
   int tiles;
-  int lb, ls, li;     // next to load: first tile of its round, step, tile within the round
+  int lb, ls;         // next to load: first tile of its round, step
+  Tile lt[RT];
 
-  MOE_DEV explicit Streamer(unsigned char* smem) {
+  MOE_DEV Streamer(const Src& source, unsigned char* smem) : src(source) {
     ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * (D * kStepBytes);
     part = reinterpret_cast<float*>(smem + kSW * D * kStepBytes);
   }
 
-  // One group, empty past the last step, so that the groups count the steps.
-  template <class Src>
-  MOE_DEV void load(const Src& src, int slot) {
-    if (lb < tiles && ls < steps) {
-      const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3, h = h0 + 2 * ls;
-      // the second half of a warp's last step may belong to the next warp
-      const bool mine = piece < 4 || h + 1 < h1;
-      const uint32_t dst = ring + slot * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
+  MOE_DEV void load_round() {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i, max(tiles - 1, 0)));
+  }
+
+  // Slot i of the ring's `turn`: one group, empty past the last tile, so that the groups count the slots.
+  MOE_DEV void load(const Step& at, bool both, int turn, int i) {
+    if (lb + i < tiles) {
+      const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3;
+      const uint32_t dst = ring + (turn * RT + i) * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
+      const bool mine = piece < 4 || both;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
         const uint16_t* p;
         int n;
-        src.row(lb + li, h, i, p, n);
+        src.row(lt[i], at, r, p, n);
         const bool take = p != nullptr && 8 * piece < n && mine;
-        copy16(dst + i * 512, take ? p + 8 * piece : src.any(), take);
-      }
-      if (++li == min(RT, tiles - lb)) {
-        li = 0;
-        if (++ls == steps) {
-          ls = 0;
-          lb += RT;
-        }
+        copy16(dst + r * 512, take ? p + 8 * piece : src.any(), take);
       }
     }
     copy_commit();
   }
+  // The second half of a warp's last step may belong to the next warp.
+  MOE_DEV bool both(int s) const { return h0 + 2 * s + 1 < h1; }
+  MOE_DEV void next_step() {
+    if (++ls == steps) {
+      ls = 0;
+      lb += RT;
+      if (lb < tiles) load_round();
+    }
+  }
 
-  template <class Src>
-  MOE_DEV void prologue(const Src& src, int n_tiles) {
+  MOE_DEV void prologue(int n_tiles) {
     const int warp = threadIdx.x >> 5, halves = src.halves();
     h0 = static_cast<int>(static_cast<int64_t>(halves) * warp / kSW);
     h1 = static_cast<int>(static_cast<int64_t>(halves) * (warp + 1) / kSW);
@@ -136,19 +149,25 @@ struct Streamer {
     }
     steps = h1 > h0 ? (h1 - h0 + 1) / 2 : 0;
     tiles = n_tiles;
-    lb = ls = li = 0;
+    lb = ls = 0;
+    if (steps == 0) return;
+    load_round();
 #pragma unroll
-    for (int i = 0; i < D; ++i) load(src, i);
+    for (int p = 0; p < PD; ++p) {
+      const Step at = src.step(h0 + 2 * ls);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) load(at, both(ls), p, i);
+      next_step();
+    }
   }
 
-  template <class Src, class Fin>
-  MOE_DEV void run(const Src& src, int cols, const Fin& fin) {
+  template <class Fin>
+  MOE_DEV void run(int cols, const Fin& fin) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
     const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
-    int slot = 0;
+    int turn = 0;
     for (int base = 0; base < tiles; base += RT) {
-      const int nt = min(RT, tiles - base);
       float acc[RT][NT][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -157,17 +176,16 @@ struct Streamer {
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
       uint4 next[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) next[j][0] = next[j][1] = make_uint4(0, 0, 0, 0);
       auto fetch = [&](int s) {
-        const int h = h0 + 2 * s;
+        const Step at = src.step(h0 + 2 * s);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          src.tokens(h, j, next[j][0], next[j][1]);
-          if (h + 1 >= h1) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
+          src.tokens(at, j, next[j][0], next[j][1]);
+          if (!both(s)) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
         }
       };
       if (steps > 0) fetch(0);
+#pragma unroll 1
       for (int s = 0; s < steps; ++s) {
         uint4 x[NT][2];
 #pragma unroll
@@ -176,27 +194,30 @@ struct Streamer {
           x[j][1] = next[j][1];
         }
         if (s + 1 < steps) fetch(s + 1);
+        const Step at = src.step(h0 + 2 * ls);
+        const bool whole = both(ls);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-          if (i < nt) {
-            copy_wait<D - 1>();
-            __syncwarp();
-            const uint32_t from = ring + slot * kStepBytes;
-            const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
-            const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+          copy_wait<D - 1>();
+          __syncwarp();
+          const uint32_t from = ring + (turn * RT + i) * kStepBytes;
+          const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
+          const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+          // a slot past the last tile holds an earlier tile's bytes: its sums are never read
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
-              T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
-              T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
-              T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
-            }
-            __syncwarp();  // every lane has read the slot
-            load(src, slot);
-            slot = slot + 1 == D ? 0 : slot + 1;
+          for (int j = 0; j < NT; ++j) {
+            T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
+            T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
+            T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
+            T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
           }
+          __syncwarp();  // every lane has read the slot
+          load(at, whole, turn, i);
         }
+        next_step();
+        turn = turn + 1 == PD ? 0 : turn + 1;
       }
+      const int nt = min(RT, tiles - base);
       if (base > 0) __syncthreads();  // the last round's partials have been added
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
