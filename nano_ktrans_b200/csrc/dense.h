@@ -58,12 +58,14 @@ struct MoeArgs {
   // workspace of the call
   unsigned long long* bar;
   float* shared_open;        // [tokens]
-  uint16_t* h;               // [tokens * top_k][hi, lo][inter]
-  uint16_t* h_shared;        // [tokens][hi, lo][shared_inter]
+  float* partial;            // [moe_pieces][tokens][hidden]
+  int h_cap;                 // set by the launcher
   int64_t ldx, ldr, ldo;
   int tokens, experts, top_k, hidden, inter, shared_inter, use_softmax, renorm;
 };
-cudaError_t launch_dense_moe(const MoeArgs& a, int dtype, int sms, cudaStream_t st);
+constexpr int kHBytes = 26624;  // of a block's h in shared memory
+int64_t moe_pieces(const MoeArgs& a, int sms);
+cudaError_t launch_dense_moe(MoeArgs a, int dtype, int sms, cudaStream_t st);
 cudaError_t read_dense_status(int* status, cudaStream_t st);
 
 }  // namespace dense

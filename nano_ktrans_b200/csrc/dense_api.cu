@@ -111,19 +111,26 @@ int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len
 
 namespace {
 
+constexpr int kB200Sms = 148;  // for the checks of a call on a host without a device
+
 struct MoeSpace {
-  size_t bar, open, logits, h, h_shared, bytes;
+  size_t bar, open, logits, partial, bytes;
 };
-MoeSpace moe_space(const moe_dense_desc& d) {
+MoeSpace moe_space(const moe_dense_desc& d, int sms) {
   const auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   const size_t t = d.num_tokens;
+  moe::dense::MoeArgs a{};
+  a.tokens = d.num_tokens;
+  a.experts = d.num_experts;
+  a.top_k = d.top_k;
+  a.inter = d.inter_size;
+  a.shared_inter = d.shared_inter;
   MoeSpace s{};
   s.bar = 0;
   s.open = 256;
   s.logits = s.open + up(4 * t);
-  s.h = s.logits + up(2 * t * d.num_experts);
-  s.h_shared = s.h + up(4 * t * d.top_k * d.inter_size);
-  s.bytes = s.h_shared + up(4 * t * d.shared_inter);
+  s.partial = s.logits + up(2 * t * d.num_experts);
+  s.bytes = s.partial + (t ? 4 * t * d.hidden_size * static_cast<size_t>(moe::dense::moe_pieces(a, sms)) : 0);
   return s;
 }
 
@@ -133,7 +140,7 @@ const char* check_layer(const moe_dense_desc& d) {
   if (d.num_experts < 1 || d.num_experts > moe::dense::kMoeExperts) return "num_experts must be in [1, 1024]";
   if (d.top_k < 1 || d.top_k > moe::dense::kMoeTopK || d.top_k > d.num_experts)
     return "top_k must be in [1, min(16, num_experts)]";
-  const int32_t big = 1 << 20;
+  const int32_t big = 1 << 16;
   if (d.hidden_size < 16 || d.hidden_size % 16 || d.hidden_size > big) return "hidden_size must be a positive multiple of 16";
   if (d.inter_size < 16 || d.inter_size % 16 || d.inter_size > big) return "inter_size must be a positive multiple of 16";
   if (d.shared_inter < 0 || d.shared_inter % 16 || d.shared_inter > big) return "shared_inter must be a multiple of 16";
@@ -148,7 +155,8 @@ int moe_dense_workspace(const moe_dense_desc* d, int64_t* bytes, char* err, size
   if (const char* why = check_layer(*d)) return refuse(err, err_len, MOE_EINVAL, "moe_dense_workspace: %s", why);
   if (d->num_tokens > MOE_DENSE_MAX_TOKENS)
     return refuse(err, err_len, MOE_ERANGE, "moe_dense_workspace: %d tokens, at most %d", d->num_tokens, MOE_DENSE_MAX_TOKENS);
-  *bytes = static_cast<int64_t>(moe_space(*d).bytes);
+  const int sms = sm_count();
+  *bytes = static_cast<int64_t>(moe_space(*d, sms > 0 ? sms : kB200Sms).bytes);
   return MOE_OK;
 }
 
@@ -188,7 +196,8 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
     return refuse(err, err_len, MOE_EINVAL, "%s: ids must be 8-byte aligned", me);
   if (d->ldx < H || d->ldo < H || (d->residual_dev && d->ldr < H))
     return refuse(err, err_len, MOE_EINVAL, "%s: the rows of x, residual and out must be at least hidden_size apart", me);
-  const MoeSpace ws = moe_space(*d);
+  const int sms = sm_count();
+  const MoeSpace ws = moe_space(*d, sms > 0 ? sms : kB200Sms);
   if (reinterpret_cast<uintptr_t>(d->workspace_dev) % 256 || d->workspace_bytes < static_cast<int64_t>(ws.bytes))
     return refuse(err, err_len, MOE_EINVAL, "%s: the workspace must be 256-byte aligned and hold %lld bytes", me,
                   static_cast<long long>(ws.bytes));
@@ -220,6 +229,7 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
     for (int j = 0; j < i; ++j)
       if (meet(written[i], written[j])) return refuse(err, err_len, MOE_EINVAL, "%s: two outputs overlap", me);
   }
+  if (sms < 1) return refuse(err, err_len, MOE_ECUDA, "%s: no device", me);
   char* w = static_cast<char*>(d->workspace_dev);
   moe::dense::MoeArgs a{};
   a.x = static_cast<const uint16_t*>(d->x_dev);
@@ -243,8 +253,7 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
   a.w_out = static_cast<uint16_t*>(d->weights_out_dev);
   a.bar = reinterpret_cast<unsigned long long*>(w + ws.bar);
   a.shared_open = reinterpret_cast<float*>(w + ws.open);
-  a.h = reinterpret_cast<uint16_t*>(w + ws.h);
-  a.h_shared = reinterpret_cast<uint16_t*>(w + ws.h_shared);
+  a.partial = reinterpret_cast<float*>(w + ws.partial);
   a.ldx = d->ldx;
   a.ldr = d->ldr;
   a.ldo = d->ldo;
@@ -256,8 +265,6 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
   a.shared_inter = static_cast<int>(S);
   a.use_softmax = d->router_use_softmax != 0;
   a.renorm = d->normalize_topk_prob != 0;
-  const int sms = sm_count();
-  if (sms < 1) return refuse(err, err_len, MOE_ECUDA, "%s: no device", me);
   const cudaError_t e = moe::dense::launch_dense_moe(a, d->dtype, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "%s: %s", me, cudaGetErrorString(e));
   return MOE_OK;

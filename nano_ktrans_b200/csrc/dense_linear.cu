@@ -139,7 +139,7 @@ struct LinearSrc {
   }
 };
 
-template <typename T, bool GATED, int NT>
+template <typename T, bool GATED, int NT, int RT>
 __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __grid_constant__ LinearArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   // A launch that may start early reads nothing before its predecessor is done
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
   constexpr int kRows = GATED ? 8 : 16;
   const int tiles = (r1 - r0 + kRows - 1) / kRows;
   const LinearSrc<GATED, NT> src(a, r0, r1);
-  Streamer<T, NT, kRows, LinearSrc<GATED, NT>> s(src, smem);
+  Streamer<T, NT, RT, kRows, LinearSrc<GATED, NT>> s(src, smem);
   s.prologue(tiles);
   s.run(a.m, [&](int tile, int row, int col, auto sum) {
     const int n = r0 + kRows * tile + row;
@@ -164,12 +164,12 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
       if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
     }
     a.out[col * a.ldo + n] = T::from_f32(v);
-  });
+  }, [] {});
 }
 
-template <typename T, bool GATED, int NT>
+template <typename T, bool GATED, int NT, int RT>
 static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) {
-  const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT>);
+  const void* kern = reinterpret_cast<const void*>(stream_linear_kernel<T, GATED, NT, RT>);
   constexpr size_t smem = kStreamBytes;
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
@@ -182,14 +182,25 @@ static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, stream_linear_kernel<T, GATED, NT>, a);
+  return cudaLaunchKernelEx(&cfg, stream_linear_kernel<T, GATED, NT, RT>, a);
+}
+
+template <typename T, bool GATED, int NT>
+static cudaError_t stream_tiles(const LinearArgs& a, int sms, cudaStream_t st) {
+  const int rows = (a.n + sms - 1) / sms, tile = GATED ? 8 : 16;  // a block's rows
+  const int rt = tiles_at_once<NT>((rows + tile - 1) / tile);
+  if constexpr (NT == 1)
+    if (rt == 4) return stream_launch<T, GATED, NT, 4>(a, sms, st);
+  if constexpr (NT <= 2)
+    if (rt == 2) return stream_launch<T, GATED, NT, 2>(a, sms, st);
+  return stream_launch<T, GATED, NT, 1>(a, sms, st);
 }
 
 template <typename T, bool GATED>
 static cudaError_t stream_cols(const LinearArgs& a, int sms, cudaStream_t st) {
-  return a.m <= 8 ? stream_launch<T, GATED, 1>(a, sms, st)
-         : a.m <= 16 ? stream_launch<T, GATED, 2>(a, sms, st)
-                     : stream_launch<T, GATED, 4>(a, sms, st);
+  return a.m <= 8 ? stream_tiles<T, GATED, 1>(a, sms, st)
+         : a.m <= 16 ? stream_tiles<T, GATED, 2>(a, sms, st)
+                     : stream_tiles<T, GATED, 4>(a, sms, st);
 }
 
 bool wide_rows(const LinearArgs& a) {

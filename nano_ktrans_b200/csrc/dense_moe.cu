@@ -11,21 +11,26 @@
 //   h_te  = w_te * silu(x_t G_e^T) * (x_t U_e^T)            (fp32)
 //   out_t = round(r_t + sum_e D_e h_te + D_s h_ts),  h_ts weighted by sigmoid(x_t . g_s)
 //
-// With the weight inside h the weighted sum over experts is part of the down
-// projection's K loop: out = [D_e1 | D_e2 | ...] [h_e1; h_e2; ...], one
-// accumulator per output.  h is kept as hi + lo, two values of the layer's
-// type (hi = round(h), lo = round(h - hi): relative error 2^-16 for bf16,
-// 2^-22 for fp16), each a token column of its own: the tensor cores have room,
-// since the kernel is bound by reading each routed expert's weights once.
-//
 // dense_router_kernel: one block per expert, logits of all tokens; one more
 // block for the shared expert's gate; zeroes the grid barrier of the call.
 // dense_moe_kernel: one block per SM, cooperative.  Every block routes all
 // tokens by itself (one warp a token) and lists the routed experts in
-// ascending order; then the gate / up rows of all of them, and after one grid
-// barrier the output rows, are split evenly over the blocks by rows and
-// streamed (dense_stream.cuh).  The first down-projection steps are loaded
-// before the barrier, so its latency passes with 128 KB per SM in flight.
+// ascending order.  Their intermediate rows (and the shared expert's), one
+// after the other, are split evenly over the blocks, and a block does both
+// halves of its rows' work: it streams their gate and up rows
+// (dense_stream.cuh), keeps h in shared memory, and streams the down
+// projection's columns of just these rows past it.  So h never leaves the SM
+// and no block waits for another between the projections; a block's partial
+// outputs (fp32, per expert piece and token) go to the workspace, and after one
+// grid barrier every block adds up its share of the outputs over the pieces,
+// in order (no atomics).  Splitting the down projection by output rows instead
+// needs the barrier between the projections and all of h in every block, read
+// from L2 step by step: 16 tokens, 128 x 768 experts, 190 us.
+//
+// h is kept as hi + lo, two values of the layer's type (hi = round(h), lo =
+// round(h - hi): relative error 2^-16 for bf16, 2^-22 for fp16), each a column
+// of its own: the tensor cores have room, since the kernel is bound by reading
+// each routed expert's weights once.
 #include "async_copy.cuh"
 #include "dense_stream.cuh"
 #include "kernels.h"
@@ -102,50 +107,63 @@ MOE_DEV float key16_value(uint32_t k) {
   return T::to_f32(static_cast<uint16_t>((k & 0x8000u) ? (k & 0x7fffu) : (~k & 0xffffu)));
 }
 
-// One warp routes one token: lane j < top_k returns the j-th pick.  keys: this
-// warp's scratch of `E` words.  Values are rounded to the layer's type before
-// they are ranked, equal ones go to the lowest expert.
-template <typename T>
-MOE_DEV void route_warp(const uint16_t* row, const MoeArgs& a, uint32_t* keys, int& id, float& wt) {
+// One warp routes one token: lane j < top_k returns the j-th pick.  Values are
+// rounded to the layer's type before they are ranked, equal ones go to the
+// lowest expert.  EPL: experts per lane, in registers.
+template <typename T, int EPL>
+MOE_DEV void route_warp(const uint16_t* row, const MoeArgs& a, int& id, float& wt) {
   const int lane = threadIdx.x & 31, E = a.experts;
-  float m = -INFINITY, s = 0.0f;
+  float v[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) v[i] = i * 32 + lane < E ? T::to_f32(__ldcg(row + i * 32 + lane)) : -INFINITY;
   if (a.use_softmax) {
-    for (int e = lane; e < E; e += 32) {
-      const float v = T::to_f32(__ldcg(row + e));
-      keys[e] = __float_as_uint(v);
-      m = fmaxf(m, v);
-    }
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) m = fmaxf(m, v[i]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
-    for (int e = lane; e < E; e += 32) {
-      const float p = expf(__uint_as_float(keys[e]) - m);
-      keys[e] = __float_as_uint(p);
-      s += p;
-    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (i * 32 + lane < E) {
+        v[i] = expf(v[i] - m);
+        s += v[i];
+      }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
-    for (int e = lane; e < E; e += 32)
-      keys[e] = (key16<T>(__uint_as_float(keys[e]) / s) << 16) | static_cast<uint32_t>(0xffff - e);
-  } else {
-    for (int e = lane; e < E; e += 32)
-      keys[e] = (key16<T>(T::to_f32(__ldcg(row + e))) << 16) | static_cast<uint32_t>(0xffff - e);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = v[i] / s;
   }
+  // unique 32-bit keys, each lane's in descending order (valid keys are never 0)
+  uint32_t key[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    key[i] = i * 32 + lane < E ? (key16<T>(v[i]) << 16) | static_cast<uint32_t>(0xffff - (i * 32 + lane)) : 0u;
+#pragma unroll
+  for (int p = 0; p < EPL - 1; ++p)
+#pragma unroll
+    for (int i = 0; i < EPL - 1 - p; ++i) {
+      const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+      key[i] = hi;
+      key[i + 1] = lo;
+    }
   float val = 0.0f, sum = 0.0f, v0 = 0.0f, exsum = 0.0f;
   id = -1;
+#pragma unroll 1
   for (int j = 0; j < a.top_k; ++j) {
-    uint32_t best = 0;
-    for (int e = lane; e < E; e += 32) best = max(best, keys[e]);
-    best = __reduce_max_sync(kFullMask, best);
-    const int e = 0xffff - static_cast<int>(best & 0xffffu);
-    if ((e & 31) == lane) keys[e] = 0;  // valid keys are never 0; each lane reads back only its own words
-    const float v = key16_value<T>(best >> 16);
-    if (lane == j) {
-      val = v;
-      id = e;
+    const uint32_t best = __reduce_max_sync(kFullMask, key[0]);
+    if (key[0] == best) {
+#pragma unroll
+      for (int i = 0; i < EPL - 1; ++i) key[i] = key[i + 1];
+      key[EPL - 1] = 0;
     }
-    sum += v;
-    if (j == 0) v0 = v;
-    if (!a.use_softmax) exsum += expf(v - v0);
+    const float x = key16_value<T>(best >> 16);
+    if (lane == j) {
+      val = x;
+      id = 0xffff - static_cast<int>(best & 0xffffu);
+    }
+    sum += x;
+    if (j == 0) v0 = x;
+    if (!a.use_softmax) exsum += expf(x - v0);
   }
   if (a.use_softmax)
     wt = a.renorm ? val / T::to_f32(T::from_f32(sum)) : val;
@@ -154,27 +172,46 @@ MOE_DEV void route_warp(const uint16_t* row, const MoeArgs& a, uint32_t* keys, i
   wt = T::to_f32(T::from_f32(wt));
 }
 
-// Routing tables of a call, in shared memory.
+// Routing of a call, in shared memory.
 struct Tables {
-  int16_t pair[kMoePairs][kMoeTokens];  // [active expert][token]: t * top_k + slot, -1 when not routed there
-  float weight[kMoePairs][kMoeTokens];
-  int active[kMoePairs];                // routed experts, ascending
-  int id[kMoeTokens][kMoeTopK];
-  float w[kMoeTokens][kMoeTopK];
+  float weight[kMoePairs + 1][kMoeTokens];  // [place in the active list][token]; entries of routed pairs only
+  uint32_t tokens[kMoePairs + 1];           // tokens of an active expert, one bit each; the shared expert's come last
+  int active[kMoePairs];                    // routed experts, ascending
+  uint32_t used[kMoeExperts / 32];          // routed experts, one bit each
+  int2 ranges[kMoePairs + 1];               // first and last range of an active expert's rows
   int n_active;
   int ok;
 };
 
-// Gate and up rows of the routed experts, then of the shared expert, as one
-// list of rows; `lo` to `hi` are this block's.  Tile i is the list's group of
-// 8 rows number lo / 8 + i (a group never spans two experts: their sizes are
-// multiples of 16), rows outside the block's range masked.
+// How the intermediate rows are split: `groups` groups of 8 rows over `ranges`
+// ranges, block b working on ranges [b * per_block, (b + 1) * per_block).
+struct Split {
+  uint32_t groups;
+  int ranges, per_block;
+  MOE_DEV Split(int64_t rows, int cap) : groups(static_cast<uint32_t>(rows / 8)) {
+    const uint32_t blocks = gridDim.x, most = blocks * (cap / 8);
+    per_block = groups > most ? static_cast<int>((groups + most - 1) / most) : 1;
+    ranges = groups < blocks ? static_cast<int>(groups) : static_cast<int>(blocks) * per_block;  // none is empty
+  }
+  // a / b; the 64-bit division only where it takes one
+  static MOE_DEV uint32_t quotient(uint64_t a, uint32_t b) {
+    return (a >> 32) == 0 ? static_cast<uint32_t>(a) / b : static_cast<uint32_t>(a / b);
+  }
+  MOE_DEV int begin(int r) const { return static_cast<int>(8 * quotient(static_cast<uint64_t>(groups) * r, ranges)); }
+  // range of the row (a multiple of 8)
+  MOE_DEV int of_row(int row) const {
+    return static_cast<int>(quotient(static_cast<uint64_t>(row / 8 + 1) * ranges + groups - 1, groups)) - 1;
+  }
+};
+
+// Gate and up rows [lo, hi) of the list of intermediate rows (multiples of 8).
+// Tile i is its i-th group of 8 (a group never spans two experts: their sizes
+// are multiples of 16).
 template <int NT>
 struct GateUpSrc {
   static constexpr bool kWhole = false;
   struct Tile {
     const uint16_t *g, *u;  // this lane's first gate and up row
-    bool first, second;     // whether that row and the one 4 below are this block's
   };
   struct Step {
     int k;
@@ -192,26 +229,22 @@ struct GateUpSrc {
     for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
   MOE_DEV int halves() const { return (a.hidden + 31) / 32; }
+  MOE_DEV int tiles() const { return (hi - lo) / 8; }
   MOE_DEV const uint16_t* any() const { return a.gate; }
   MOE_DEV Tile tile(int i) const {
-    const int v0 = (lo / 8 + i) * 8, v = v0 + q;
-    Tile t{a.gate, a.up, v >= lo && v < hi, v + 4 >= lo && v + 4 < hi};
-    if (v0 < routed) {
-      const int s = v0 / a.inter;
-      const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter)) * a.hidden;
-      t.g = a.gate + at;
-      t.u = a.up + at;
-    } else {
-      const int64_t at = static_cast<int64_t>(v - routed) * a.hidden;
-      t.g = a.shared_gate + at;
-      t.u = a.shared_up + at;
+    const int v = lo + 8 * i;
+    if (v < routed) {
+      const int s = v / a.inter;
+      const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter) + q) * a.hidden;
+      return {a.gate + at, a.up + at};
     }
-    return t;
+    const int64_t at = static_cast<int64_t>(v - routed + q) * a.hidden;
+    return {a.shared_gate + at, a.shared_up + at};
   }
   MOE_DEV Step step(int half) const { return {32 * half}; }
   MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
     n = a.hidden - s.k;
-    p = ((i & 1) ? t.second : t.first) ? (i < 2 ? t.g : t.u) + (i & 1) * 4 * a.hidden + s.k : nullptr;
+    p = (i < 2 ? t.g : t.u) + (i & 1) * 4 * a.hidden + s.k;
   }
   MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
@@ -220,54 +253,148 @@ struct GateUpSrc {
   }
 };
 
-// Output rows [r0, r1); K runs over the routed experts' h, then the shared
-// expert's.  Columns: hi of token c for c < half, then lo of token c - half.
-template <int NT>
-struct DownSrc {
-  static constexpr bool kWhole = true;  // a step of 64 elements lies in one expert
-  static constexpr int kHalf = 4 * NT;
-  struct Tile {
-    int row, left;  // this lane's first row, rows from there to the block's end
-  };
-  struct Step {
-    const uint16_t* w;  // row 0 of the expert at the step's first element
-    int ld, k, slot;    // row length, place in the row, place in the active list (-1: shared)
+// The down projection's columns of rows [lo, hi), all output rows: every warp
+// takes whole tiles of 16 output rows (tile w, w + 16, ...), RT at a time, over
+// the K of one expert's piece after the other.  Column 2 i of the mma is hi and
+// column 2 i + 1 lo of the expert's i-th token, so that one thread holds both
+// sums of an output; of ND column tiles (4 tokens each) only those that the
+// expert has tokens for are worked on.  The ring is the Streamer's.
+template <typename T, int ND, int RT>
+struct DownStreamer {
+  static constexpr int D = kSlots, PD = D / RT;
+  struct Piece {
+    const uint16_t* w;  // row 0 at the piece's first column
+    int ld, len, place, v;
   };
   const MoeArgs& a;
   const Tables& tb;
-  int r0, r1, ue, routed_units, q, g, t8;
-  MOE_DEV DownSrc(const MoeArgs& args, const Tables& tables, int lo, int hi) : a(args), tb(tables), r0(lo), r1(hi) {
-    const int lane = threadIdx.x & 31;
-    q = lane >> 3;
-    g = lane >> 2;
-    t8 = 8 * (lane & 3);
-    ue = (a.inter + 63) / 64;
-    routed_units = tables.n_active * ue;
+  const uint16_t* hs;  // [hi, lo][token of the expert][cap] from row lo on
+  int lo, hi, routed, cap, range;
+  uint32_t ring;
+  int count;        // this warp's tiles
+  Piece lp;         // next to load: piece, first tile of its group, step
+  int lg, ls;
+
+  MOE_DEV DownStreamer(const MoeArgs& args, const Tables& tables, unsigned char* smem, const uint16_t* h, int cap_, int range_,
+                       int lo_, int hi_)
+      : a(args), tb(tables), hs(h), lo(lo_), hi(hi_), routed(tables.n_active * args.inter), cap(cap_), range(range_) {
+    const int warp = threadIdx.x >> 5, tiles = a.hidden / 16;
+    ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (D * kStepBytes);
+    count = warp < tiles ? (tiles - warp + kSW - 1) / kSW : 0;
   }
-  MOE_DEV int halves() const { return 2 * (routed_units + (a.shared_inter + 63) / 64); }
-  MOE_DEV const uint16_t* any() const { return a.down; }
-  MOE_DEV Tile tile(int i) const { return {r0 + 16 * i + q, r1 - (r0 + 16 * i + q)}; }
-  MOE_DEV Step step(int half) const {
-    const int unit = half / 2;
-    if (unit < routed_units) {
-      const int s = unit / ue, k = (unit - s * ue) * 64;
-      return {a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter + k, a.inter, k, s};
+  MOE_DEV Piece piece(int v) const {
+    if (v < routed) {
+      const int s = v / a.inter, off = v - s * a.inter;
+      return {a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter + off, a.inter, min(hi, (s + 1) * a.inter) - v,
+              s, v};
     }
-    const int k = (unit - routed_units) * 64;
-    return {a.shared_down + k, a.shared_inter, k, -1};
+    return {a.shared_down + (v - routed), a.shared_inter, hi - v, tb.n_active, v};
   }
-  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
-    n = s.ld - s.k;
-    p = t.left > 4 * i ? s.w + static_cast<int64_t>(t.row + 4 * i) * s.ld : nullptr;
+  MOE_DEV void load(int turn, int i) {
+    if (lp.v < hi && lg + i < count) {
+      const int lane = threadIdx.x & 31, c = lane & 7, row = lane >> 3;
+      const uint32_t dst = ring + (turn * RT + i) * kStepBytes + row * 128 + ((c ^ ((row & 1) << 2)) << 4);
+      const int r = 16 * ((threadIdx.x >> 5) + kSW * (lg + i)) + row, k = 64 * ls + 8 * c;
+      const bool take = k < lp.len;
+      const uint16_t* p = take ? lp.w + static_cast<int64_t>(r) * lp.ld + k : a.down;
+      const int64_t four = take ? 4 * static_cast<int64_t>(lp.ld) : 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) copy16(dst + q * 512, p + q * four, take);
+    }
+    copy_commit();
   }
-  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
-    const int col = 8 * j + g, part = col >= kHalf ? 1 : 0, tok = col - part * kHalf, k = s.k + t8;
-    int pair = -1;
-    if (tok < a.tokens) pair = s.slot < 0 ? tok : tb.pair[s.slot][tok];
-    const uint16_t* p = (s.slot < 0 ? a.h_shared : a.h) + static_cast<int64_t>(2 * pair + part) * s.ld + k;
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = pair >= 0 && k < s.ld ? ld_l2(p) : z;
-    x1 = pair >= 0 && k + 32 < s.ld ? ld_l2(p + 32) : z;
+  MOE_DEV void next_step() {
+    if (64 * ++ls >= lp.len) {
+      ls = 0;
+      lg += RT;
+      if (lg >= count) {
+        lg = 0;
+        const int v = lp.v + lp.len;
+        if (v < hi) lp = piece(v);
+        else lp.v = v;
+      }
+    }
+  }
+  MOE_DEV void prologue() {
+    lg = ls = 0;
+    if (count == 0 || lo >= hi) return;
+    lp = piece(lo);
+#pragma unroll
+    for (int p = 0; p < PD; ++p) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) load(p, i);
+      next_step();
+    }
+  }
+  MOE_DEV void run() {
+    if (count == 0) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4), frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);
+    int turn = 0;
+    for (int v = lo; v < hi;) {
+      const Piece p = piece(v);
+      const int n = __popc(tb.tokens[p.place]);  // the expert's tokens
+      const uint16_t* hrow[ND];
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        const int i = 4 * j + (g >> 1);
+        hrow[j] = i < n ? hs + ((g & 1) * a.tokens + i) * cap + (v - lo) + 8 * t4 : nullptr;
+      }
+      float* out = a.partial + (static_cast<int64_t>(range + p.place) * a.tokens + t4) * a.hidden + g;
+      for (int grp = 0; grp < count; grp += RT) {
+        float acc[RT][ND][4];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
+#pragma unroll 1
+        for (int k = 0; k < p.len; k += 64) {
+          uint4 x[ND][2];
+          const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < ND; ++j)
+            if (4 * j < n) {
+              x[j][0] = hrow[j] != nullptr && k + 8 * t4 < p.len ? *reinterpret_cast<const uint4*>(hrow[j] + k) : z;
+              x[j][1] = hrow[j] != nullptr && k + 32 + 8 * t4 < p.len ? *reinterpret_cast<const uint4*>(hrow[j] + k + 32) : z;
+            }
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            copy_wait<D - 1>();
+            __syncwarp();
+            const uint32_t from = ring + (turn * RT + i) * kStepBytes;
+            const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
+            const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+            // a slot past the warp's last tile holds other bytes: its sums are not stored
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+              if (4 * j < n) {
+                T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
+                T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
+                T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
+                T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
+              }
+            __syncwarp();
+            load(turn, i);
+          }
+          next_step();
+          turn = turn + 1 == PD ? 0 : turn + 1;
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          if (grp + i < count) {
+            float* o = out + 16 * ((threadIdx.x >> 5) + kSW * (grp + i));
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+              if (4 * j + t4 < n) {
+                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden, acc[i][j][0] + acc[i][j][1]);
+                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden + 8, acc[i][j][2] + acc[i][j][3]);
+              }
+          }
+      }
+      v += p.len;
+    }
   }
 };
 
@@ -280,8 +407,9 @@ MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
 }
 
-// NT column tiles hold the tokens of the gate / up phase, ND those of the down phase (hi and lo).
-template <typename T, int NT, int ND>
+// NT column tiles hold the tokens of the gate / up phase; the down phase has up
+// to ND column tiles of 4 tokens and RD row tiles at once.
+template <typename T, int NT, int ND, int RD>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Tables tb;
@@ -289,118 +417,170 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- routing, in every block ----
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);  // [16][E] words, then used[E] bytes: before the ring is in use
-  uint8_t* used = reinterpret_cast<uint8_t*>(keys + kMoeTokens * a.experts);
-  for (int i = tid; i < a.experts; i += kSThreads) used[i] = 0;
-  for (int i = tid; i < kMoePairs * kMoeTokens; i += kSThreads) {
-    (&tb.pair[0][0])[i] = -1;
-    (&tb.weight[0][0])[i] = 0.0f;
-  }
+  if (tid < kMoeExperts / 32) tb.used[tid] = 0;
+  if (tid <= kMoePairs) tb.tokens[tid] = 0;
   __syncthreads();
+  int id = -1;
+  float wt = 0.0f;
   if (warp < a.tokens) {
-    int id = -1;
-    float wt = 0.0f;
     if (a.ids_in == nullptr) {
-      route_warp<T>(a.logits + warp * a.experts, a, keys + warp * a.experts, id, wt);
-    } else if (lane < a.top_k) {
-      const int64_t given = a.ids_in[warp * a.top_k + lane];
-      wt = T::to_f32(a.w_in[warp * a.top_k + lane]);
-      id = given >= 0 && given < a.experts ? static_cast<int>(given) : -1;
-      if (given >= a.experts && blockIdx.x == 0) atomicOr(&g_dense_status, kStatusBadExpertId);
-    }
-    if (lane < a.top_k) {
-      if (blockIdx.x == 0 && a.ids_in == nullptr) {
+      const uint16_t* row = a.logits + warp * a.experts;
+      if (a.experts <= 64) route_warp<T, 2>(row, a, id, wt);
+      else if (a.experts <= 128) route_warp<T, 4>(row, a, id, wt);
+      else if (a.experts <= 256) route_warp<T, 8>(row, a, id, wt);
+      else route_warp<T, 32>(row, a, id, wt);
+      if (blockIdx.x == 0 && lane < a.top_k) {
         if (a.ids_out) a.ids_out[warp * a.top_k + lane] = id;
         if (a.w_out) a.w_out[warp * a.top_k + lane] = T::from_f32(wt);
       }
-      if (id >= 0 && a.mask != nullptr && a.mask[id] == 0) id = -1;
-      if (id >= 0) used[id] = 1;
-      tb.id[warp][lane] = id;
-      tb.w[warp][lane] = wt;
+    } else {
+      int64_t given = -1;
+      if (lane < a.top_k) {
+        given = a.ids_in[warp * a.top_k + lane];
+        wt = T::to_f32(a.w_in[warp * a.top_k + lane]);
+      }
+      if (given >= a.experts && blockIdx.x == 0) atomicOr(&g_dense_status, kStatusBadExpertId);
+      id = given >= 0 && given < a.experts ? static_cast<int>(given) : -1;
+      // an expert given twice for a token counts once, with both weights
+      float total = 0.0f;
+      bool first = true;
+      for (int j = 0; j < a.top_k; ++j) {
+        const int other = __shfl_sync(kFullMask, id, j);
+        const float w = __shfl_sync(kFullMask, wt, j);
+        if (other == id) {
+          total += w;
+          first = first && j >= lane;
+        }
+      }
+      wt = total;
+      if (!first) id = -1;
     }
+    if (lane >= a.top_k || (id >= 0 && a.mask != nullptr && a.mask[id] == 0)) id = -1;
+    if (id >= 0) atomicOr(&tb.used[id >> 5], 1u << (id & 31));
   }
   __syncthreads();
-  int16_t* slot = reinterpret_cast<int16_t*>(keys);  // [E] place of an expert in the active list
-  if (warp == 0) {
-    int n = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const bool on = e0 + lane < a.experts && used[e0 + lane] != 0;
-      const uint32_t b = __ballot_sync(kFullMask, on);
-      if (on) {
-        const int s = n + __popc(b & ((1u << lane) - 1u));
-        tb.active[s] = e0 + lane;
-        slot[e0 + lane] = static_cast<int16_t>(s);
-      }
-      n += __popc(b);
-    }
+  if (id >= 0) {
+    int place = __popc(tb.used[id >> 5] & ((1u << (id & 31)) - 1u));
+    for (int i = 0; i < id >> 5; ++i) place += __popc(tb.used[i]);
+    tb.active[place] = id;
+    tb.weight[place][warp] = wt;
+    atomicOr(&tb.tokens[place], 1u << warp);
+  }
+  if (warp == kSW - 1) {  // 32 words of 32 experts
+    int n = __popc(tb.used[lane]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(kFullMask, n, off);
     if (lane == 0) tb.n_active = n;
-    __syncwarp();
-    if (lane < a.tokens)
-      for (int j = 0; j < a.top_k; ++j) {  // an expert given twice for a token counts with both weights
-        const int id = tb.id[lane][j];
-        if (id < 0) continue;
-        const int s = slot[id];
-        if (tb.pair[s][lane] < 0) tb.pair[s][lane] = static_cast<int16_t>(lane * a.top_k + j);
-        tb.weight[s][lane] += tb.w[lane][j];
-      }
+    if (a.shared_inter > 0) {  // every token's, in the place after the last routed expert
+      if (lane == 0) tb.tokens[n] = (1u << a.tokens) - 1u;
+      if (lane < a.tokens) tb.weight[n][lane] = __ldcg(a.shared_open + lane);
+    }
   }
   __syncthreads();
 
-  // ---- h = w silu(gate) up ----
-  const int64_t rows = static_cast<int64_t>(tb.n_active) * a.inter + a.shared_inter;
-  const int lo = static_cast<int>(rows * blockIdx.x / gridDim.x), hi = static_cast<int>(rows * (blockIdx.x + 1) / gridDim.x);
-  {
+  // ---- this block's rows: h, then their part of the outputs ----
+  const Split split(static_cast<int64_t>(tb.n_active) * a.inter + a.shared_inter, a.h_cap);
+  uint16_t* hs = reinterpret_cast<uint16_t*>(smem + kStreamBytes);
+  const int first = min(static_cast<int>(blockIdx.x) * split.per_block, split.ranges);
+  const int last = min(first + split.per_block, split.ranges);
+  for (int r = first; r < last; ++r) {
+    const int lo = split.begin(r), hi = split.begin(r + 1);
     const GateUpSrc<NT> src(a, tb, lo, hi);
-    const int tiles = hi > lo ? (hi + 7) / 8 - lo / 8 : 0;
-    Streamer<T, NT, 8, GateUpSrc<NT>> s(src, smem);
-    s.prologue(tiles);
-    s.run(a.tokens, [&](int tile, int row, int col, auto sum) {
-      const int v0 = (lo / 8 + tile) * 8, v = v0 + row;
-      if (v < lo || v >= hi) return;
-      if (v0 < src.routed) {
-        const int e = v0 / a.inter, pair = tb.pair[e][col];
-        if (pair < 0) return;
-        const float h = tb.weight[e][col] * (silu_f32(sum(row, col)) * sum(row + 8, col));
-        uint16_t* p = a.h + static_cast<int64_t>(2 * pair) * a.inter + (v - e * a.inter);
-        store_split<T>(p, p + a.inter, h);
-      } else {
-        const float h = __ldcg(a.shared_open + col) * (silu_f32(sum(row, col)) * sum(row + 8, col));
-        uint16_t* p = a.h_shared + static_cast<int64_t>(2 * col) * a.shared_inter + (v - src.routed);
-        store_split<T>(p, p + a.shared_inter, h);
-      }
-    });
+    Streamer<T, NT, kSlots / NT, 8, GateUpSrc<NT>> up(src, smem);
+    DownStreamer<T, ND, RD> down(a, tb, smem, hs, a.h_cap, r, lo, hi);
+    up.prologue(src.tiles());
+    up.run(a.tokens, [&](int tile, int row, int col, auto sum) {
+      const int v = lo + 8 * tile, place = v < src.routed ? v / a.inter : tb.n_active;
+      const uint32_t toks = tb.tokens[place], bit = 1u << col;
+      if ((toks & bit) == 0) return;
+      const float h = tb.weight[place][col] * (silu_f32(sum(row, col)) * sum(row + 8, col));
+      uint16_t* p = hs + __popc(toks & (bit - 1u)) * a.h_cap + 8 * tile + row;
+      store_split<T>(p, p + a.tokens * a.h_cap, h);
+    }, [&] { down.prologue(); });
+    __syncthreads();  // h is complete
+    down.run();
+    __syncthreads();  // h may be written again
   }
-
-  // ---- out = r + sum over experts of D h ----
-  const int r0 = static_cast<int>(static_cast<int64_t>(a.hidden) * blockIdx.x / gridDim.x);
-  const int r1 = static_cast<int>(static_cast<int64_t>(a.hidden) * (blockIdx.x + 1) / gridDim.x);
-  const DownSrc<ND> src(a, tb, r0, r1);
-  const bool none = src.halves() == 0;  // every expert masked and no shared expert
-  Streamer<T, ND, 16, DownSrc<ND>> s(src, smem);
-  s.prologue(none ? 0 : (r1 - r0 + 15) / 16);  // weights only: they do not wait for h
+  const int places = tb.n_active + (a.shared_inter > 0 ? 1 : 0);
+  if (tid < places) {
+    const int begin = tid * a.inter, len = tid < tb.n_active ? a.inter : a.shared_inter;
+    tb.ranges[tid] = make_int2(split.of_row(begin), split.of_row(begin + len - 8));
+  }
   if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
     if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
     return;
   }
-  auto store = [&](int n, int col, float v) {
-    if (a.res) v += T::to_f32(a.res[col * a.ldr + n]);
-    a.out[col * a.ldo + n] = T::from_f32(v);
-  };
-  if (none) {
-    for (int i = tid; i < (r1 - r0) * a.tokens; i += kSThreads) store(r0 + i % (r1 - r0), i / (r1 - r0), 0.0f);
-    return;
+
+  // ---- out = r + the pieces' sums, experts ascending ----
+  // Four outputs of a token by `slices` threads, each adding every slices-th
+  // piece, then one thread the slices' sums.
+  const int quads = a.hidden / 4;
+  const int64_t all = static_cast<int64_t>(quads) * a.tokens;
+  const int q0 = static_cast<int>(all * blockIdx.x / gridDim.x), q1 = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x);
+  int slices = 1;
+  while (slices < 64 && 2 * slices * (q1 - q0) <= kSThreads) slices *= 2;
+  float4* sums = reinterpret_cast<float4*>(smem);
+  for (int base = q0; base < q1; base += kSThreads / slices) {
+    const int q = base + tid / slices, slice = tid % slices;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int tok = q < q1 ? q / quads : 0, col = q - tok * quads;
+    if (q < q1) {
+      int before = 0;  // pieces of earlier experts
+      for (int place = 0; place < places; ++place) {
+        const uint32_t toks = tb.tokens[place];
+        if ((toks & (1u << tok)) == 0) continue;
+        const int r0 = tb.ranges[place].x, r1 = tb.ranges[place].y;
+        const float* p = a.partial + static_cast<int64_t>(__popc(toks & ((1u << tok) - 1u))) * a.hidden + 4 * col;
+        for (int r = r0 + ((slice - before) & (slices - 1)); r <= r1; r += slices) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(p + static_cast<int64_t>(r + place) * a.tokens * a.hidden));
+          s.x += f.x;
+          s.y += f.y;
+          s.z += f.z;
+          s.w += f.w;
+        }
+        before += r1 - r0 + 1;
+      }
+    }
+    __syncthreads();
+    sums[tid] = s;
+    __syncthreads();
+    if (slice == 0 && q < q1) {
+      for (int i = 1; i < slices; ++i) {
+        const float4 f = sums[tid + i];
+        s.x += f.x;
+        s.y += f.y;
+        s.z += f.z;
+        s.w += f.w;
+      }
+      const float v[4] = {s.x, s.y, s.z, s.w};
+      uint16_t* o = a.out + tok * a.ldo + 4 * col;
+      const uint16_t* res = a.res ? a.res + tok * a.ldr + 4 * col : nullptr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = T::from_f32(res ? v[i] + T::to_f32(res[i]) : v[i]);
+    }
   }
-  s.run(a.tokens, [&](int tile, int row, int col, auto sum) {
-    const int n = r0 + 16 * tile + row;
-    if (n < r1) store(n, col, sum(row, col) + sum(row, col + 4 * ND));
-  });
 }
 
-template <typename T, int NT, int ND>
+// Rows of h that a block holds at a time: 32 more than a multiple of 64, so
+// that the fragment reads of two token rows fall into different banks.
+int moe_h_cap(int tokens) {
+  const int rows = kHBytes / (4 * tokens);
+  return (rows - 32) / 64 * 64 + 32;
+}
+// Partial rows [tokens][hidden] of the largest split: a piece per range and
+// expert boundary.
+int64_t moe_pieces(const MoeArgs& a, int sms) {
+  const int most = a.tokens * a.top_k < a.experts ? a.tokens * a.top_k : a.experts;
+  const int64_t groups = (static_cast<int64_t>(most) * a.inter + a.shared_inter) / 8, cap = moe_h_cap(a.tokens) / 8;
+  const int64_t per_block = (groups + sms * cap - 1) / (sms * cap);
+  return sms * (per_block > 0 ? per_block : 1) + most + 1;
+}
+
+template <typename T, int NT, int ND, int RD>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
-  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND>);
-  constexpr size_t smem = kStreamBytes;
-  static_assert((sizeof(uint32_t) * kMoeTokens + 1) * kMoeExperts <= smem, "routing scratch");
+  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND, RD>);
+  constexpr size_t smem = kStreamBytes + kHBytes;
+  static_assert(smem + sizeof(Tables) + 1024 <= 232448, "shared-memory plan");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms);
@@ -414,7 +594,17 @@ static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, NT, ND>, a);
+  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, NT, ND, RD>, a);
+}
+
+template <typename T, int NT, int ND>
+static cudaError_t moe_tiles(const MoeArgs& a, int sms, cudaStream_t st) {
+  const int rd = tiles_at_once<ND>((a.hidden / 16 + kSW - 1) / kSW);  // a warp's tiles
+  if constexpr (ND == 1)
+    if (rd == 4) return moe_main<T, NT, ND, 4>(a, sms, st);
+  if constexpr (ND <= 2)
+    if (rd == 2) return moe_main<T, NT, ND, 2>(a, sms, st);
+  return moe_main<T, NT, ND, 1>(a, sms, st);
 }
 
 template <typename T>
@@ -430,12 +620,13 @@ static cudaError_t moe_both(const MoeArgs& a, int sms, cudaStream_t st) {
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, dense_router_kernel<T>, a);
   if (e != cudaSuccess) return e;
-  if (a.tokens <= 4) return moe_main<T, 1, 1>(a, sms, st);
-  if (a.tokens <= 8) return moe_main<T, 1, 2>(a, sms, st);
-  return moe_main<T, 2, 4>(a, sms, st);
+  if (a.tokens <= 4) return moe_tiles<T, 1, 1>(a, sms, st);
+  if (a.tokens <= 8) return moe_tiles<T, 1, 2>(a, sms, st);
+  return moe_tiles<T, 2, 4>(a, sms, st);
 }
 
-cudaError_t launch_dense_moe(const MoeArgs& a, int dtype, int sms, cudaStream_t st) {
+cudaError_t launch_dense_moe(MoeArgs a, int dtype, int sms, cudaStream_t st) {
+  a.h_cap = moe_h_cap(a.tokens);
   return dtype == MOE_DTYPE_FP16 ? moe_both<Fp16>(a, sms, st) : moe_both<Bf16>(a, sms, st);
 }
 

@@ -68,19 +68,21 @@ MOE_DEV uint4 ld_l2(const uint16_t* p) {
 
 constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
-// Tiles a warp keeps in registers, and steps it copies ahead.
+constexpr int kSlots = 4;  // of a warp's ring
+
+// Tiles a warp keeps in registers when its block has `tiles`: as many as share
+// a token fragment, but no more than there are, since a ring slot of a tile
+// that does not exist is a copy less in flight (2048 x 2048, one token: 4.0 us,
+// with slots for four tiles where there is one 5.0).
 template <int NT>
-constexpr int round_tiles() {
-  return 4 / NT;
-}
-template <int NT>
-constexpr int steps_ahead() {
-  return NT;
+inline int tiles_at_once(int tiles) {
+  const int most = kSlots / NT;
+  return tiles >= 3 && most >= 4 ? 4 : tiles >= 2 && most >= 2 ? 2 : 1;
 }
 // Dynamic shared memory of a Streamer: the ring of four slots a warp, then the partials.
-constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * 4 * kStepBytes + sizeof(float) * 4 * kSW * kPartTile;
+constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * kSlots * kStepBytes + sizeof(float) * 4 * kSW * kPartTile;
 
-// NT column tiles of 8 tokens (1, 2 or 4).  Src:
+// NT column tiles of 8 tokens (1, 2 or 4), RT row tiles (RT * NT <= 4).  Src:
 //   halves()                  K in halves of 32 elements; kWhole: a warp's part starts on an even half
 //   Tile tile(int)            what copying a tile's rows needs, rows (lane / 8) + 4 i
 //   Step step(int half)       what a step needs: where it is in K
@@ -89,9 +91,10 @@ constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * 4 * kStepBytes + size
 //   fin(tile, row, col, sum)  one output; sum(row, col) adds the partials
 // FROWS outputs per column and tile (16, or 8 where rows g and g + 8 belong to
 // one output), `cols` columns.
-template <typename T, int NT, int FROWS, class Src>
+template <typename T, int NT, int RT, int FROWS, class Src>
 struct Streamer {
-  static constexpr int RT = round_tiles<NT>(), PD = steps_ahead<NT>(), D = RT * PD;
+  static constexpr int D = kSlots, PD = D / RT;  // steps ahead
+  static_assert(RT * NT <= 4, "partials");
   using Tile = typename Src::Tile;
   using Step = typename Src::Step;
   const Src& src;
@@ -161,8 +164,9 @@ struct Streamer {
     }
   }
 
-  template <class Fin>
-  MOE_DEV void run(int cols, const Fin& fin) {
+  // `ahead` runs once the last step is consumed, before the partials are added: the next stage's first copies.
+  template <class Fin, class Ahead>
+  MOE_DEV void run(int cols, const Fin& fin, const Ahead& ahead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
     const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
@@ -218,6 +222,7 @@ struct Streamer {
         turn = turn + 1 == PD ? 0 : turn + 1;
       }
       const int nt = min(RT, tiles - base);
+      if (base + RT >= tiles) ahead();
       if (base > 0) __syncthreads();  // the last round's partials have been added
 #pragma unroll
       for (int i = 0; i < RT; ++i) {

@@ -78,7 +78,7 @@ def moe_desc(**kw):
     # addresses that no call here reaches: every one of these descriptions is refused
     d = dict(gate_dev=0x100000, up_dev=0x200000, down_dev=0x300000, num_experts=8, top_k=2, hidden_size=64, inter_size=32,
              shared_inter=0, router_use_softmax=1, normalize_topk_prob=1, dtype=0, x_dev=0x400000, router_w_dev=0x500000,
-             out_dev=0x600000, workspace_dev=0x700000, ldx=64, ldr=64, ldo=64, workspace_bytes=1 << 20, num_tokens=4,
+             out_dev=0x600000, workspace_dev=0x1700000, ldx=64, ldr=64, ldo=64, workspace_bytes=1 << 24, num_tokens=4,
              add_shared=1)
     d.update(kw)
     return _lib.MoeDenseDesc(**d)
@@ -100,7 +100,7 @@ SHARED = dict(shared_inter=16, shared_gate_dev=0x800000, shared_up_dev=0x810000,
     (dict(x_dev=0x400008), "16-byte"), (dict(down_dev=0x300008), "16-byte"), (dict(ldx=68), "16-byte"),
     (dict(SHARED, shared_gate_vec_dev=0x830002), "16-byte"), (dict(out_dev=0x600001), "2-byte"),
     (dict(ids_out_dev=0x900004), "8-byte"), (dict(ldx=48), "apart"), (dict(ldo=63), "apart"),
-    (dict(residual_dev=0x900000, ldr=32), "apart"), (dict(workspace_dev=0x700010), "workspace"),
+    (dict(residual_dev=0x900000, ldr=32), "apart"), (dict(workspace_dev=0x1700010), "workspace"),
     (dict(workspace_bytes=100), "workspace"), (dict(out_dev=0x400080), "overlaps"), (dict(out_dev=0x100100), "overlaps"),
     (dict(workspace_dev=0x400000), "overlaps"), (dict(out_dev=0x400000, ldo=80), "overlaps"),
     (dict(weights_out_dev=0x600000), "two outputs"), (dict(logits_dev=0x600010), "two outputs"),
@@ -124,8 +124,8 @@ def test_dense_moe_token_limits_and_workspace(lib):
     assert lib.moe_dense_forward(ctypes.byref(moe_desc(num_tokens=17)), None, err, len(err)) == _lib.MOE_ERANGE
     assert lib.moe_dense_workspace(ctypes.byref(moe_desc(num_tokens=17)), ctypes.byref(n), err, len(err)) == _lib.MOE_ERANGE
     assert lib.moe_dense_workspace(ctypes.byref(moe_desc(**SHARED)), ctypes.byref(n), err, len(err)) == _lib.MOE_OK
-    # barrier, shared gates, logits, both parts of h for every pair and for the shared expert
-    assert n.value >= 8 + 4 * 4 + 2 * 4 * 8 + 4 * 4 * 2 * 32 + 4 * 4 * 16 and n.value % 256 == 0
+    # barrier, shared gates, logits, a row of partial sums for every token and piece of the split
+    assert n.value >= 8 + 4 * 4 + 2 * 4 * 8 + 148 * 4 * 64 * 4 and n.value % 256 == 0
     assert lib.moe_dense_workspace(None, ctypes.byref(n), err, len(err)) == _lib.MOE_EINVAL
     assert lib.moe_dense_read_status(None, None, err, len(err)) == _lib.MOE_EINVAL
 
