@@ -76,10 +76,8 @@ MOE_DEV uint32_t map_rank(uint32_t addr, uint32_t rank) {
 MOE_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-MOE_DEV float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+MOE_DEV void st_cluster(uint32_t addr, float x, float y, float z, float w) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
 
 // 2-D tiled load into this block's shared memory (no multicast).  With PAIR the
@@ -151,6 +149,17 @@ MOE_DEV void tmem_ld16(uint32_t taddr, float* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 8 columns.
+MOE_DEV void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 template <int N>
@@ -389,14 +398,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
 struct SplitPlan {
   int rows;     // token rows per tile: 128 or 256
   int splits;   // blocks of a cluster that share a tile, each with a part of K
-  int slices;   // feature slices
+  int slices;   // feature slices, in groups of 8 features
   int width;    // features of the widest slice, padded (gated: multiple of 8, else of 16)
   int box_x;    // token rows loaded per stage
   int stages;
   int smem;
+  int wide;     // out and residual rows allow 16-byte accesses
 };
 constexpr int kQThreads = 320;  // producer, MMA, 8 epilogue warps
 constexpr int kQTail = 1024 + 16384;  // alignment, and what an MMA reads past a tile of fewer than 128 rows
+
+// Bias and residual of 8 columns of a row, read ahead of the sums they join.
+template <typename T>
+struct Extra8 {
+  uint32_t b[4], r[4];
+  MOE_DEV void load(const LinearArgs& a, int64_t m, int n, bool row, bool wide) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = r[i] = 0;
+    const auto pick = [&](const uint16_t* p, uint32_t (&o)[4], bool vec) {
+      if (vec) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        o[0] = q.x;
+        o[1] = q.y;
+        o[2] = q.z;
+        o[3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < a.n) o[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
+      }
+    };
+    if (a.bias) pick(a.bias + n, b, false);
+    if (a.res && row) pick(a.res + m * a.ldr + n, r, wide && n + 8 <= a.n);
+  }
+};
+
+// Epilogue of 8 columns of a row.
+template <typename T, bool GATED>
+MOE_DEV void finish8(const LinearArgs& a, int64_t m, int n, float (&v)[8], const float (&u)[8], const Extra8<T>& e, bool wide) {
+  if constexpr (GATED) {
+    activate_all(a.act, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= u[i];
+  } else {
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = T::unpack(e.b[i]);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+      }
+    }
+    activate_all(a.act, v);
+    if (a.res) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = T::unpack(e.r[i]);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+      }
+    }
+  }
+  uint16_t* o = a.out + m * a.ldo + n;
+  if (wide && n + 8 <= a.n) {
+    *reinterpret_cast<uint4*>(o) =
+        make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < a.n) o[i] = T::from_f32(v[i]);
+  }
+}
 
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(kQThreads, 1)
@@ -413,8 +485,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int slice = blockIdx.x / p.splits;
-  const int n0 = static_cast<int>(static_cast<int64_t>(a.n) * slice / p.slices);
-  const int n1 = static_cast<int>(static_cast<int64_t>(a.n) * (slice + 1) / p.slices);
+  const int64_t eights = (a.n + 7) / 8;
+  const int n0 = static_cast<int>(8 * (eights * slice / p.slices));
+  const int n1 = min(a.n, static_cast<int>(8 * (eights * (slice + 1) / p.slices)));
   const int m0 = blockIdx.y * p.rows, valid = min(p.rows, a.m - m0);
   const int nk = (a.k + kBK - 1) / kBK;
   const int k_lo = nk * rank / p.splits, k_hi = nk * (rank + 1) / p.splits, steps = k_hi - k_lo;
@@ -490,71 +563,115 @@ __global__ void __launch_bounds__(kQThreads, 1)
     }
   }
   __syncwarp();
-  if (warp >= 2 && !__all_sync(kFullMask, mbar_wait(smem_u32(&acc_full), 0))) give_up(aborted);
-  __syncthreads();
-  const bool good = !*aborted;
-  // ---- partial sums into shared memory, [row][cols + 1] ----
-  float* part = reinterpret_cast<float*>(smem);
-  const int ldp = cols + 1;
-  if (good && warp >= 2) {
+
+  // ---- epilogue: a lane is a token row, columns in chunks of 8 ----
+  // Items (chunk, 32 rows): warp e takes item e, e + 8, ... of a lane quarter it may read.
+  const int chunks = (n1 - n0 + 7) / 8, q = warp & 3, half = (warp - 2) >> 2;
+  bool good = true;
+  if (warp >= 2) {
+    Extra8<T> next;
+    if (p.splits == 1) {
+      if (half < chunks) next.load(a, m0 + q * 32 + lane, n0 + 8 * half, q * 32 + lane < valid, p.wide);
+    }
+    good = __all_sync(kFullMask, mbar_wait(smem_u32(&acc_full), 0));
+    if (!good) give_up(aborted);
     fence_after();
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    for (int r = 0; r < row_tiles; ++r) {
-      const int row = r * 128 + q * 32 + lane;
-      if (r * 128 + q * 32 >= valid) continue;  // warp-uniform
-      for (int c = half * 16; c < cols; c += 32) {
-        float v[16];
-        if (steps > 0) {
-          tmem_ld16(tmem + r * cols + c + (static_cast<uint32_t>(q * 32) << 16), v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = 0.0f;
-        }
-        if (row < valid) {
-          float* o = part + row * ldp + c;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = v[j];
+    if (good && p.splits == 1 && !*aborted) {
+      for (int r = 0; r < row_tiles; ++r) {
+        const int row = r * 128 + q * 32 + lane;
+        for (int c = half; c < chunks; c += 2) {
+          const Extra8<T> e = next;
+          // the next item's bias and residual are under way while this one's sums are worked on
+          const int nc = c + 2 < chunks ? c + 2 : half, nrow = c + 2 < chunks ? row : row + 128;
+          next.load(a, m0 + nrow, n0 + 8 * nc, nrow < valid, p.wide);
+          const uint32_t at = tmem + r * cols + 8 * c + (static_cast<uint32_t>(q * 32) << 16);
+          float v[8], u[8];
+          tmem_ld8(at, v);
+          if constexpr (GATED) tmem_ld8(at + p.width, u);
+          if (row < valid) finish8<T, GATED>(a, m0 + row, n0 + 8 * c, v, u, e, p.wide);
         }
       }
     }
     fence_before();
+  }
+  if (p.splits > 1) {
+    // Chunk c belongs to block c % splits of the cluster.  Every block sends its
+    // partial sums of a chunk to the owner's shared memory, [sender][chunk]
+    // [4 columns][row], once all blocks are past their MMAs; the owner adds them
+    // in sender order.
+    constexpr int kSub = GATED ? 4 : 2;  // quads of columns of a chunk
+    const int own = (chunks + p.splits - 1) / p.splits, quad_bytes = valid * 16;
+    __syncthreads();
+    cluster_sync();
+    if (warp >= 2 && !*aborted) {
+      fence_after();
+      const uint32_t mine = smem_u32(smem) + static_cast<uint32_t>(rank * own * kSub * quad_bytes);
+      for (int r = 0; r < row_tiles; ++r) {
+        const int row = r * 128 + q * 32 + lane;
+        if (r * 128 + q * 32 >= valid) continue;  // warp-uniform
+        for (int c = half; c < chunks; c += 2) {
+          const uint32_t at = tmem + r * cols + 8 * c + (static_cast<uint32_t>(q * 32) << 16);
+          float v[8], u[8];
+          tmem_ld8(at, v);
+          if constexpr (GATED) tmem_ld8(at + p.width, u);
+          if (row < valid) {
+            const uint32_t to = map_rank(mine + (c / p.splits) * kSub * quad_bytes + row * 16, c % p.splits);
+            st_cluster(to, v[0], v[1], v[2], v[3]);
+            st_cluster(to + quad_bytes, v[4], v[5], v[6], v[7]);
+            if constexpr (GATED) {
+              st_cluster(to + 2 * quad_bytes, u[0], u[1], u[2], u[3]);
+              st_cluster(to + 3 * quad_bytes, u[4], u[5], u[6], u[7]);
+            }
+          }
+        }
+      }
+      fence_before();
+    }
+    // items of this block's chunks: 32 rows x a chunk per warp
+    const int groups = (valid + 31) / 32, mine_chunks = rank < chunks ? (chunks - rank + p.splits - 1) / p.splits : 0;
+    const int items = groups * mine_chunks;
+    Extra8<T> next;
+    const auto fetch = [&](int i) {
+      const int row = (i % groups) * 32 + lane, c = rank + (i / groups) * p.splits;
+      next.load(a, m0 + row, n0 + 8 * c, row < valid, p.wide);
+    };
+    if (warp < items) fetch(warp);
+    __syncwarp();
+    cluster_sync();
+    if (!*aborted) {
+      for (int i = warp; i < items; i += kQThreads / 32) {
+        const Extra8<T> e = next;
+        if (i + kQThreads / 32 < items) fetch(i + kQThreads / 32);
+        const int row = (i % groups) * 32 + lane, slot = i / groups;
+        if (row >= valid) continue;
+        float v[8] = {}, u[8] = {};
+        for (int s = 0; s < p.splits; ++s) {
+          const unsigned char* from = smem + static_cast<size_t>((s * own + slot) * kSub) * quad_bytes + row * 16;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 f = *reinterpret_cast<const float4*>(from + h * quad_bytes);
+            v[4 * h] += f.x;
+            v[4 * h + 1] += f.y;
+            v[4 * h + 2] += f.z;
+            v[4 * h + 3] += f.w;
+            if constexpr (GATED) {
+              const float4 g = *reinterpret_cast<const float4*>(from + (2 + h) * quad_bytes);
+              u[4 * h] += g.x;
+              u[4 * h + 1] += g.y;
+              u[4 * h + 2] += g.z;
+              u[4 * h + 3] += g.w;
+            }
+          }
+        }
+        finish8<T, GATED>(a, m0 + row, n0 + 8 * (rank + slot * p.splits), v, u, e, p.wide);
+      }
+    }
   }
   __syncthreads();
   if (warp == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
   }
-  if (p.splits > 1) cluster_sync();
-  // ---- this block's share of the rows: partials added in rank order ----
-  if (good) {
-    const int r_lo = valid * rank / p.splits, r_hi = valid * (rank + 1) / p.splits, w = n1 - n0;
-    uint32_t peer[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) peer[s] = s < p.splits && p.splits > 1 ? map_rank(smem_u32(part), s) : smem_u32(part);
-    for (int r = r_lo + warp; r < r_hi; r += kQThreads / 32) {
-      const int64_t m = m0 + r;
-      for (int c = lane; c < w; c += 32) {
-        const int n = n0 + c;
-        const uint32_t off = 4u * static_cast<uint32_t>(r * ldp + c);
-        float v = 0.0f, u = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (s < p.splits) {
-            v += ld_cluster(peer[s] + off);
-            if constexpr (GATED) u += ld_cluster(peer[s] + off + 4u * static_cast<uint32_t>(p.width));
-          }
-        if constexpr (GATED) {
-          v = activate_rt(a.act, v) * u;
-        } else {
-          if (a.bias) v += T::to_f32(a.bias[n]);
-          v = activate_rt(a.act, v);
-          if (a.res) v += T::to_f32(a.res[m * a.ldr + n]);
-        }
-        a.out[m * a.ldo + n] = T::from_f32(v);
-      }
-    }
-  }
-  if (p.splits > 1) cluster_sync();  // peers are done with this block's partials
 }
 
 // ---------------------------------------------------------------------------
@@ -596,9 +713,10 @@ int resident_blocks(int dev, int splits, int sms) {
 }
 
 // Estimated clocks of a plan; the best of the candidates is taken.  Per K step
-// a block brings box_x + cols rows of 128 bytes into shared memory (about 40
-// bytes a clock and SM) and its MMAs take 2 clocks a column and row tile; a
-// launch, tensor-memory and epilogue overhead is added once per wave.
+// a block brings box_x + cols rows of 128 bytes into shared memory (about 50
+// bytes a clock and SM) and its MMAs take 2 clocks a column and row tile; the
+// epilogue, and where K is split the exchange of the partial sums, come once
+// per wave.
 SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
   const bool gated = a.w_up != nullptr;
   const int nk = (a.k + kBK - 1) / kBK, pad = gated ? 8 : 16, mul = gated ? 2 : 1;
@@ -617,25 +735,28 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
         if (slices < 1) continue;
         const int most = (a.n + pad - 1) / pad;  // no narrower than the padding
         if (slices > most) slices = most;
-        const int width = ((a.n + slices - 1) / slices + pad - 1) / pad * pad;
+        const int eights = (a.n + 7) / 8, width = (8 * ((eights + slices - 1) / slices) + pad - 1) / pad * pad;
         const int cols = width * mul;
         if (cols > 256 || rows / 128 * cols > 512) continue;
         const int stage = (box + cols) * 128;
         int stages = static_cast<int>((kSmemLimit - 2048 - kQTail) / stage);
         if (stages > 16) stages = 16;
         if (stages < 2) continue;
-        const int64_t part = 4LL * (a.m < rows ? a.m : rows) * (cols + 1);
+        // partial sums that a block receives: its chunks of 8 columns from every block
+        const int valid = a.m < rows ? a.m : rows, own = ((width + 7) / 8 + splits - 1) / splits;
+        const int64_t part = splits > 1 ? 32LL * mul * valid * own * splits : 0;
         int64_t smem = static_cast<int64_t>(stages) * stage;
         if (part > smem) smem = part;
         smem += kQTail;
         if (smem > static_cast<int64_t>(kSmemLimit) - 2048) continue;
         const int steps = (nk + splits - 1) / splits, real_waves = (slices * mg * splits + cap - 1) / cap;
-        const double load = (box + cols) * 128 / 40.0, mma = 2.0 * cols * (box > 128 ? 2 : 1);
-        const double join = part / splits / 16.0 + (splits > 1 ? 1500.0 : 0.0);
+        const double load = stage / 50.0, mma = 2.0 * cols * (box > 128 ? 2 : 1);
+        const double items = (valid + 31) / 32 * ((width + 7) / 8) * mul / 8.0;  // 32 rows x 8 columns a warp
+        const double join = splits > 1 ? 2500.0 + 90.0 * items + 60.0 * items : 110.0 * items;
         const double t = real_waves * (steps * (load > mma ? load : mma) + join + 3000.0);
         if (t < clocks) {
           clocks = t;
-          best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem)};
+          best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem), 0};
         }
       }
     }
@@ -646,8 +767,17 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
 // A tensor map wants a stride of whole 16 bytes even where there is one row.
 uint64_t row_stride(int64_t ld, int rows, int k) { return static_cast<uint64_t>(rows > 1 ? ld : k); }
 
+// 16-byte accesses to the rows of out and residual.
+int wide_output(const LinearArgs& a) {
+  const auto aligned = [&](const void* p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.m == 1 || ld % 8 == 0);
+  };
+  return aligned(a.out, a.ldo) && (a.res == nullptr || aligned(a.res, a.ldr));
+}
+
 template <typename T, bool GATED>
-cudaError_t launch_split(const LinearArgs& a, const SplitPlan& p, cudaStream_t st) {
+cudaError_t launch_split(const LinearArgs& a, SplitPlan p, cudaStream_t st) {
+  p.wide = wide_output(a);
   alignas(64) CUtensorMap tx, tw, tu;
   if (!make_tmap_rows(&tx, a.x, T::kBf16, a.k, a.m, a.ldx, p.box_x) ||
       !make_tmap_rows(&tw, a.w, T::kBf16, a.k, a.n, row_stride(a.ldw, a.n, a.k), p.width) ||
@@ -682,8 +812,7 @@ cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t st) {
     return cudaErrorInvalidValue;
   const void* kern = reinterpret_cast<const void*>(pair_gemm_kernel<T, GATED>);
   if (!ensure_dynamic_smem(kern, kPSmem, kPThreads)) return cudaErrorInvalidConfiguration;
-  const auto aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
-  const int wide = aligned(a.out, a.ldo) && (a.res == nullptr || aligned(a.res, a.ldr));
+  const int wide = wide_output(a);
   const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < sms / 2 ? tiles : sms / 2));
