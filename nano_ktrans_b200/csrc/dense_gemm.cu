@@ -287,7 +287,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      int it = 0, s = 0;
+      uint32_t phase = 1;  // a stage's first use waits for nothing
+      const uint32_t full0 = map_rank(smem_u32(&full[0]), 0);
       bool ok = true;
       for (int i = pair; i < total && ok; i += pairs) {
         int m, n;
@@ -296,15 +298,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
         const int wr = GATED ? n * 128 : n * 256 + 128 * static_cast<int>(rank);
         const CUtensorMap* tw = GATED && rank == 1 ? &tm_u : &tm_w;
         for (int kc = 0; kc < nk; ++kc, ++it) {
-          const int s = it % kPStages;
-          if (*aborted || (it >= kPStages && !mbar_wait(smem_u32(&empty[s]), ((it / kPStages) - 1) & 1))) {
+          if (it >= kPStages && !mbar_wait(smem_u32(&empty[s]), phase)) {
             ok = false;
             break;
           }
           if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * kPStage);
-          const uint32_t bar = map_rank(smem_u32(&full[s]), 0), dst = smem_u32(smem + s * kPStage);
+          const uint32_t bar = full0 + 8 * s, dst = smem_u32(smem) + s * kPStage;
           tma_load<true>(dst, &tm_x, kc * kBK, xr, bar);
           tma_load<true>(dst + kPTile, tw, kc * kBK, wr, bar);
+          if (++s == kPStages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
       }
       if (!ok) give_up(aborted);
@@ -314,7 +319,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = instr_desc<T>(256, 256);
-      int it = 0, ti = 0;
+      const uint64_t da0 = tile_desc(smem_u32(smem)), db0 = tile_desc(smem_u32(smem) + kPTile);
+      int s = 0, ti = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int i = pair; i < total && ok; i += pairs, ++ti) {
         const int acc = ti & 1;
@@ -323,19 +330,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
           break;
         }
         fence_after();
-        for (int kc = 0; kc < nk; ++kc, ++it) {
-          const int s = it % kPStages;
-          if (*aborted || !mbar_wait(smem_u32(&full[s]), (it / kPStages) & 1)) {
+        for (int kc = 0; kc < nk; ++kc) {
+          if (!mbar_wait(smem_u32(&full[s]), phase)) {
             ok = false;
             break;
           }
           fence_after();
-          const uint32_t base = smem_u32(smem + s * kPStage);
-          const uint64_t da = tile_desc(base), db = tile_desc(base + kPTile);
+          const uint64_t da = da0 + static_cast<uint64_t>(s) * (kPStage >> 4);
+          const uint64_t db = db0 + static_cast<uint64_t>(s) * (kPStage >> 4);
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk)
             umma<2>(tmem + acc * 256, da + 2 * kk, db + 2 * kk, idesc, kc > 0 || kk > 0);
           commit_pair(smem_u32(&empty[s]));
+          if (++s == kPStages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
         commit_pair(smem_u32(&acc_full[acc]));
       }
@@ -517,21 +527,33 @@ __global__ void __launch_bounds__(kQThreads, 1)
   const uint32_t tmem = tmem_s;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
+  // One thread walks the stages in each role, so what it does per step is paid in
+  // full latency: positions and descriptors are carried along, not worked out
+  // (with divisions by the stage count a step took 500 ns whatever its size).
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
-      for (; it < steps; ++it) {
-        const int s = it % p.stages;
-        if (*aborted || (it >= p.stages && !mbar_wait(smem_u32(&empty[s]), ((it / p.stages) - 1) & 1))) {
+      uint32_t bar = smem_u32(&full[0]), gone = smem_u32(&empty[0]), dst = smem_u32(smem);
+      int s = 0, it = 0, k = k_lo * kBK;
+      uint32_t phase = 1;  // a stage's first use waits for nothing
+      for (; it < steps; ++it, k += kBK) {
+        if (it >= p.stages && !mbar_wait(gone, phase)) {
           give_up(aborted);
           break;
         }
-        const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + s * stage_bytes);
-        const int k = (k_lo + it) * kBK;
         mbar_expect_tx(bar, stage_bytes);
         tma_load<false>(dst, &tm_x, k, m0, bar);
         tma_load<false>(dst + x_bytes, &tm_w, k, n0, bar);
         if constexpr (GATED) tma_load<false>(dst + x_bytes + p.width * 128, &tm_u, k, n0, bar);
+        bar += 8;
+        gone += 8;
+        dst += stage_bytes;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
+          bar = smem_u32(&full[0]);
+          gone = smem_u32(&empty[0]);
+          dst = smem_u32(smem);
+        }
       }
       if (*aborted)  // no copy may still be landing when the block exits
         for (int j = max(0, it - p.stages); j < it; ++j) mbar_wait(smem_u32(&full[j % p.stages]), (j / p.stages) & 1);
@@ -539,24 +561,39 @@ __global__ void __launch_bounds__(kQThreads, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = instr_desc<T>(128, cols);
+      const uint64_t da0 = tile_desc(smem_u32(smem)), db0 = tile_desc(smem_u32(smem + x_bytes));
+      const uint64_t next = static_cast<uint64_t>(stage_bytes >> 4);
+      uint64_t da = da0, db = db0;
+      uint32_t bar = smem_u32(&full[0]), gone = smem_u32(&empty[0]), phase = 0;
+      int s = 0;
       for (int it = 0; it < steps; ++it) {
-        const int s = it % p.stages;
-        if (*aborted || !mbar_wait(smem_u32(&full[s]), (it / p.stages) & 1)) {
+        if (!mbar_wait(bar, phase)) {
           give_up(aborted);
           break;
         }
         fence_after();
-        const uint32_t base = smem_u32(smem + s * stage_bytes);
-        const uint64_t db = tile_desc(base + x_bytes);
-        for (int r = 0; r < row_tiles; ++r) {
-          // a tile of fewer than 128 rows: the MMA reads on into other bytes of the
-          // stages; those accumulator lanes are never read
-          const uint64_t da = tile_desc(base + r * 16384);
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk) umma<1>(tmem, da + 2 * kk, db + 2 * kk, idesc, it > 0 || kk > 0);
+        // A tile of fewer than 128 rows: the MMA reads on into other bytes of the
+        // stages; those accumulator lanes are never read.
+        if (row_tiles > 1) {
 #pragma unroll
           for (int kk = 0; kk < kBK / 16; ++kk)
-            umma<1>(tmem + r * cols, da + 2 * kk, db + 2 * kk, idesc, it > 0 || kk > 0);
+            umma<1>(tmem + cols, da + 1024 + 2 * kk, db + 2 * kk, idesc, it > 0 || kk > 0);
         }
-        commit_one(smem_u32(&empty[s]));
+        commit_one(gone);
+        bar += 8;
+        gone += 8;
+        da += next;
+        db += next;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
+          bar = smem_u32(&full[0]);
+          gone = smem_u32(&empty[0]);
+          da = da0;
+          db = db0;
+        }
       }
       commit_one(smem_u32(&acc_full));
       if (!mbar_wait(smem_u32(&acc_full), 0)) give_up(aborted);  // every MMA is done before tensor memory is freed
