@@ -91,11 +91,15 @@ MOE_DEV bool grid_sync_epoch(unsigned long long* bar, unsigned long long seen, i
 }
 
 // Grid-wide barrier on a counter that an earlier kernel of the stream zeroed
-// for this launch alone.
-MOE_DEV bool grid_sync_zeroed(unsigned long long* bar, int* ok_smem) {
+// for this launch alone, in two halves: the CTA arrives with what it has
+// written so far, and may do other work before it waits for the others.
+MOE_DEV void grid_arrive(unsigned long long* bar) {
   __syncthreads();  // the CTA's writes are ordered before thread 0's release (cumulativity)
+  if (threadIdx.x == 0) asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(bar) : "memory");
+}
+
+MOE_DEV bool grid_wait(unsigned long long* bar, int* ok_smem) {
   if (threadIdx.x == 0) {
-    asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(bar) : "memory");
     cuda::atomic_ref<unsigned long long, cuda::thread_scope_device> count(*bar);
     int ok = 1;
     for (uint32_t i = 0; count.load(cuda::memory_order_acquire) < gridDim.x; ++i) {

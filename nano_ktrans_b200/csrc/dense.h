@@ -59,7 +59,8 @@ struct MoeArgs {
   unsigned long long* bar;
   float* shared_open;        // [tokens]
   float* partial;            // [moe_pieces][tokens][hidden]
-  int h_cap;                 // set by the launcher
+  int h_cap;                 // set by the launcher, as is
+  uint64_t inter_inverse;    // 2^64 / inter
   int64_t ldx, ldr, ldo;
   int tokens, experts, top_k, hidden, inter, shared_inter, use_softmax, renorm;
 };

@@ -100,7 +100,6 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 template <bool GATED, int NT>
 struct LinearSrc {
-  static constexpr bool kWhole = false;
   struct Tile {
     const uint16_t *p, *u;  // this lane's first row, of each weight when gated
     int left;               // rows from there to the block's end

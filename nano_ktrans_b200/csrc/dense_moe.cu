@@ -178,7 +178,10 @@ struct Tables {
   uint32_t tokens[kMoePairs + 1];           // tokens of an active expert, one bit each; the shared expert's come last
   int active[kMoePairs];                    // routed experts, ascending
   uint32_t used[kMoeExperts / 32];          // routed experts, one bit each
-  int2 ranges[kMoePairs + 1];               // first and last range of an active expert's rows
+  int n_places[kMoeTokens];                 // a token's experts in ascending order: place in the active list,
+  int place[kMoeTokens][kMoeTopK + 1];      // first range of its rows,
+  int range[kMoeTokens][kMoeTopK + 1];
+  int pieces[kMoeTokens][kMoeTopK + 2];     // and pieces of the experts before it
   int n_active;
   int ok;
 };
@@ -204,12 +207,14 @@ struct Split {
   }
 };
 
+// Expert (place in the active list) of an intermediate row.
+MOE_DEV int place_of(const MoeArgs& a, int row) { return static_cast<int>(__umul64hi(static_cast<uint64_t>(row), a.inter_inverse)); }
+
 // Gate and up rows [lo, hi) of the list of intermediate rows (multiples of 8).
 // Tile i is its i-th group of 8 (a group never spans two experts: their sizes
 // are multiples of 16).
 template <int NT>
 struct GateUpSrc {
-  static constexpr bool kWhole = false;
   struct Tile {
     const uint16_t *g, *u;  // this lane's first gate and up row
   };
@@ -234,7 +239,7 @@ struct GateUpSrc {
   MOE_DEV Tile tile(int i) const {
     const int v = lo + 8 * i;
     if (v < routed) {
-      const int s = v / a.inter;
+      const int s = place_of(a, v);
       const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter) + q) * a.hidden;
       return {a.gate + at, a.up + at};
     }
@@ -284,7 +289,7 @@ struct DownStreamer {
   }
   MOE_DEV Piece piece(int v) const {
     if (v < routed) {
-      const int s = v / a.inter, off = v - s * a.inter;
+      const int s = place_of(a, v), off = v - s * a.inter;
       return {a.down + static_cast<int64_t>(tb.active[s]) * a.hidden * a.inter + off, a.inter, min(hi, (s + 1) * a.inter) - v,
               s, v};
     }
@@ -359,24 +364,36 @@ struct DownStreamer {
               x[j][0] = hrow[j] != nullptr && k + 8 * t4 < p.len ? *reinterpret_cast<const uint4*>(hrow[j] + k) : z;
               x[j][1] = hrow[j] != nullptr && k + 32 + 8 * t4 < p.len ? *reinterpret_cast<const uint4*>(hrow[j] + k + 32) : z;
             }
+          constexpr int P = RT >= 2 ? 2 : 1;  // slots at a time, as in the Streamer
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            copy_wait<D - 1>();
+          for (int i = 0; i < RT; i += P) {
+            copy_wait<D - P>();
             __syncwarp();
-            const uint32_t from = ring + (turn * RT + i) * kStepBytes;
-            const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
-            const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+            uint4 a0[P], a1[P], b0[P], b1[P];
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+              const uint32_t from = ring + (turn * RT + i + q) * kStepBytes;
+              a0[q] = ld_shared(from + frag0);
+              b0[q] = ld_shared(from + frag0 + 1024);
+              a1[q] = ld_shared(from + frag1);
+              b1[q] = ld_shared(from + frag1 + 1024);
+            }
             // a slot past the warp's last tile holds other bytes: its sums are not stored
 #pragma unroll
             for (int j = 0; j < ND; ++j)
               if (4 * j < n) {
-                T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
-                T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
-                T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
-                T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
+#pragma unroll
+                for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a0[q].x, b0[q].x, a0[q].y, b0[q].y, x[j][0].x, x[j][0].y);
+#pragma unroll
+                for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a0[q].z, b0[q].z, a0[q].w, b0[q].w, x[j][0].z, x[j][0].w);
+#pragma unroll
+                for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a1[q].x, b1[q].x, a1[q].y, b1[q].y, x[j][1].x, x[j][1].y);
+#pragma unroll
+                for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a1[q].z, b1[q].z, a1[q].w, b1[q].w, x[j][1].z, x[j][1].w);
               }
             __syncwarp();
-            load(turn, i);
+#pragma unroll
+            for (int q = 0; q < P; ++q) load(turn, i + q);
           }
           next_step();
           turn = turn + 1 == PD ? 0 : turn + 1;
@@ -459,8 +476,9 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     if (id >= 0) atomicOr(&tb.used[id >> 5], 1u << (id & 31));
   }
   __syncthreads();
+  int place = -1;
   if (id >= 0) {
-    int place = __popc(tb.used[id >> 5] & ((1u << (id & 31)) - 1u));
+    place = __popc(tb.used[id >> 5] & ((1u << (id & 31)) - 1u));
     for (int i = 0; i < id >> 5; ++i) place += __popc(tb.used[i]);
     tb.active[place] = id;
     tb.weight[place][warp] = wt;
@@ -490,7 +508,7 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     DownStreamer<T, ND, RD> down(a, tb, smem, hs, a.h_cap, r, lo, hi);
     up.prologue(src.tiles());
     up.run(a.tokens, [&](int tile, int row, int col, auto sum) {
-      const int v = lo + 8 * tile, place = v < src.routed ? v / a.inter : tb.n_active;
+      const int v = lo + 8 * tile, place = v < src.routed ? place_of(a, v) : tb.n_active;
       const uint32_t toks = tb.tokens[place], bit = 1u << col;
       if ((toks & bit) == 0) return;
       const float h = tb.weight[place][col] * (silu_f32(sum(row, col)) * sum(row + 8, col));
@@ -501,62 +519,89 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     down.run();
     __syncthreads();  // h may be written again
   }
-  const int places = tb.n_active + (a.shared_inter > 0 ? 1 : 0);
-  if (tid < places) {
-    const int begin = tid * a.inter, len = tid < tb.n_active ? a.inter : a.shared_inter;
-    tb.ranges[tid] = make_int2(split.of_row(begin), split.of_row(begin + len - 8));
+  // This block's partial sums are written; while the others finish, each token's
+  // list of pieces, by the warp that routed it.
+  ac::grid_arrive(a.bar);
+  if (warp < a.tokens) {
+    if (lane == a.top_k && a.shared_inter > 0) place = tb.n_active;
+    int rank = 0, before = 0, r0 = 0, count = 0;
+    if (place >= 0) {
+      const int begin = place * a.inter, len = place < tb.n_active ? a.inter : a.shared_inter;
+      r0 = split.of_row(begin);
+      count = split.of_row(begin + len - 8) - r0 + 1;
+    }
+    for (int j = 0; j <= a.top_k; ++j) {
+      const int other = __shfl_sync(kFullMask, place, j), c = __shfl_sync(kFullMask, count, j);
+      if (other >= 0 && other < place) {
+        ++rank;
+        before += c;
+      }
+    }
+    const int n = __popc(__ballot_sync(kFullMask, place >= 0));
+    if (lane == 0) tb.n_places[warp] = n;
+    if (place >= 0) {
+      tb.place[warp][rank] = place;
+      tb.range[warp][rank] = r0;
+      tb.pieces[warp][rank] = before;
+      if (rank == n - 1) tb.pieces[warp][n] = before + count;
+    }
   }
-  if (!ac::grid_sync_zeroed(a.bar, &tb.ok)) {
+  if (!ac::grid_wait(a.bar, &tb.ok)) {
     if (tid == 0) atomicOr(&g_dense_status, kStatusTimeout);
     return;
   }
 
-  // ---- out = r + the pieces' sums, experts ascending ----
-  // Four outputs of a token by `slices` threads, each adding every slices-th
-  // piece, then one thread the slices' sums.
+  // ---- out = r + the pieces' sums ----
+  // A warp adds up four outputs of a token: lane l takes its pieces l, l + 32,
+  // ... (experts ascending), then the lanes' sums are added in a fixed tree.
   const int quads = a.hidden / 4;
   const int64_t all = static_cast<int64_t>(quads) * a.tokens;
   const int q0 = static_cast<int>(all * blockIdx.x / gridDim.x), q1 = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x);
-  int slices = 1;
-  while (slices < 64 && 2 * slices * (q1 - q0) <= kSThreads) slices *= 2;
-  float4* sums = reinterpret_cast<float4*>(smem);
-  for (int base = q0; base < q1; base += kSThreads / slices) {
-    const int q = base + tid / slices, slice = tid % slices;
+  for (int q = q0 + warp; q < q1; q += kSW) {
+    const int tok = q / quads, col = q - tok * quads, n = tb.n_places[tok];
+    const int total = n > 0 ? tb.pieces[tok][n] : 0;
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (lane == 0 && a.res != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = T::to_f32(a.res[tok * a.ldr + 4 * col + i]);
+    }
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const int tok = q < q1 ? q / quads : 0, col = q - tok * quads;
-    if (q < q1) {
-      int before = 0;  // pieces of earlier experts
-      for (int place = 0; place < places; ++place) {
-        const uint32_t toks = tb.tokens[place];
-        if ((toks & (1u << tok)) == 0) continue;
-        const int r0 = tb.ranges[place].x, r1 = tb.ranges[place].y;
-        const float* p = a.partial + static_cast<int64_t>(__popc(toks & ((1u << tok) - 1u))) * a.hidden + 4 * col;
-        for (int r = r0 + ((slice - before) & (slices - 1)); r <= r1; r += slices) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(p + static_cast<int64_t>(r + place) * a.tokens * a.hidden));
-          s.x += f.x;
-          s.y += f.y;
-          s.z += f.z;
-          s.w += f.w;
+    int j = 0;
+    for (int p0 = 0; p0 < total; p0 += 128) {
+      float4 f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int p = p0 + 32 * u + lane;
+        f[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p < total) {
+          while (p >= tb.pieces[tok][j + 1]) ++j;
+          const int place_j = tb.place[tok][j], at = tb.range[tok][j] + p - tb.pieces[tok][j] + place_j;
+          const int i = __popc(tb.tokens[place_j] & ((1u << tok) - 1u));
+          f[u] = __ldcg(reinterpret_cast<const float4*>(
+              a.partial + (static_cast<int64_t>(at) * a.tokens + i) * a.hidden + 4 * col));
         }
-        before += r1 - r0 + 1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s.x += f[u].x;
+        s.y += f[u].y;
+        s.z += f[u].z;
+        s.w += f[u].w;
       }
     }
-    __syncthreads();
-    sums[tid] = s;
-    __syncthreads();
-    if (slice == 0 && q < q1) {
-      for (int i = 1; i < slices; ++i) {
-        const float4 f = sums[tid + i];
-        s.x += f.x;
-        s.y += f.y;
-        s.z += f.z;
-        s.w += f.w;
-      }
-      const float v[4] = {s.x, s.y, s.z, s.w};
-      uint16_t* o = a.out + tok * a.ldo + 4 * col;
-      const uint16_t* res = a.res ? a.res + tok * a.ldr + 4 * col : nullptr;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = T::from_f32(res ? v[i] + T::to_f32(res[i]) : v[i]);
+    for (int off = 16; off > 0; off >>= 1) {
+      s.x += __shfl_xor_sync(kFullMask, s.x, off);
+      s.y += __shfl_xor_sync(kFullMask, s.y, off);
+      s.z += __shfl_xor_sync(kFullMask, s.z, off);
+      s.w += __shfl_xor_sync(kFullMask, s.w, off);
+    }
+    if (lane == 0) {
+      uint16_t* o = a.out + tok * a.ldo + 4 * col;
+      o[0] = T::from_f32(s.x + r[0]);
+      o[1] = T::from_f32(s.y + r[1]);
+      o[2] = T::from_f32(s.z + r[2]);
+      o[3] = T::from_f32(s.w + r[3]);
     }
   }
 }
@@ -627,6 +672,7 @@ static cudaError_t moe_both(const MoeArgs& a, int sms, cudaStream_t st) {
 
 cudaError_t launch_dense_moe(MoeArgs a, int dtype, int sms, cudaStream_t st) {
   a.h_cap = moe_h_cap(a.tokens);
+  a.inter_inverse = ~0ull / static_cast<uint64_t>(a.inter) + 1;  // floor(row / inter) = high word of row * this, rows < 2^32
   return dtype == MOE_DTYPE_FP16 ? moe_both<Fp16>(a, sms, st) : moe_both<Bf16>(a, sms, st);
 }
 

@@ -3,11 +3,12 @@
 //
 // With a handful of tokens a projection is bound by reading its weights once.
 // A block owns a range of weight rows, cut into tiles of 16 (the mma's M;
-// tokens are its N, 8 per column tile).  The 16 warps split K evenly, in halves
-// of 32 elements, and each walks its part in steps of 64 elements; for a step
-// it takes up to RT tiles one after the other, so a token fragment is loaded
-// once for RT weight tiles (loading it for every tile cost 8 of 31 us at 118
-// MB of weights and 7 tokens: those loads queue behind the weights').  Lane
+// tokens are its N, 8 per column tile).  Groups of KW warps split K evenly, in
+// halves of 32 elements, and each warp walks its part in steps of 64 elements;
+// for a step it takes up to RT tiles one after the other, so a token fragment
+// is loaded once for RT weight tiles (loading it for every tile cost 8 of 31 us
+// at 118 MB of weights and 7 tokens: those loads queue behind the weights').
+// The 16 / KW groups work on different tiles (plan_warps).  Lane
 // (g, t) feeds the mma with 8 consecutive elements at 8 t and at 32 + 8 t of
 // rows g and g + 8 (A) and of token column g (B): an mma is unchanged by a
 // permutation of K that both operands share, so nothing is shuffled.
@@ -23,7 +24,7 @@
 // both worked out per slot the issue slots, not the memory, were the limit.
 //
 // Partial sums: a warp keeps RT tiles in registers over its part of K, puts the
-// 16 x 8 partial tiles into shared memory, and the block adds the 16 partials
+// 16 x 8 partial tiles into shared memory, and the block adds the KW partials
 // of each output in warp order (no atomics: the same bits every run) while the
 // next tiles' copies are in flight.
 #pragma once
@@ -70,20 +71,42 @@ constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
 constexpr int kSlots = 4;  // of a warp's ring
 
-// Tiles a warp keeps in registers when its block has `tiles`: as many as share
-// a token fragment, but no more than there are, since a ring slot of a tile
-// that does not exist is a copy less in flight (2048 x 2048, one token: 4.0 us,
-// with slots for four tiles where there is one 5.0).
+// Tiles that a warp keeps in registers when its block has `tiles`: as many as
+// share a token fragment, but no more than there are, since a ring slot of a
+// tile that does not exist is a copy less in flight (2048 x 2048, one token: 4.0
+// us, with slots for four tiles where there is one 5.0).
 template <int NT>
 inline int tiles_at_once(int tiles) {
   const int most = kSlots / NT;
   return tiles >= 3 && most >= 4 ? 4 : tiles >= 2 && most >= 2 ? 2 : 1;
 }
+
+// Warps that share K, for a block with `tiles` tiles of `halves` halves, RT of
+// them at once in a warp.  A warp's time is its steps times its group's tiles,
+// plus about three steps' worth for every round of RT tiles (two block
+// barriers and the sum over the group's partials): few warps on a tile make
+// the rounds long, many spread few tiles over all warps.  (26 tiles of 2048
+// elements, 16 tokens: 16 warps a tile 91 units by this count, 4 warps 68.)
+template <int RT>
+MOE_DEV int plan_warps(int tiles, int halves) {
+  int best = kSW, cost = 1 << 30;
+#pragma unroll
+  for (int l = 4; l >= 1; --l) {  // 1 << l warps; shifts, since this is on the way to the first load
+    const int each = (tiles + (kSW >> l) - 1) >> (4 - l), steps = (halves + (2 << l) - 1) >> (l + 1);
+    const int c = steps * each + 3 * ((each + RT - 1) / RT);
+    if (c < cost) {
+      cost = c;
+      best = 1 << l;
+    }
+  }
+  return best;
+}
+
 // Dynamic shared memory of a Streamer: the ring of four slots a warp, then the partials.
 constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * kSlots * kStepBytes + sizeof(float) * 4 * kSW * kPartTile;
 
 // NT column tiles of 8 tokens (1, 2 or 4), RT row tiles (RT * NT <= 4).  Src:
-//   halves()                  K in halves of 32 elements; kWhole: a warp's part starts on an even half
+//   halves()                  K in halves of 32 elements
 //   Tile tile(int)            what copying a tile's rows needs, rows (lane / 8) + 4 i
 //   Step step(int half)       what a step needs: where it is in K
 //   row(Tile, Step, i, p, n)  row i's address at the step's first element (null: zeros), elements from there to its end
@@ -100,9 +123,10 @@ struct Streamer {
   const Src& src;
   uint32_t ring;      // the warp's ring
   float* part;
-  int h0, h1, steps;  // the warp's halves and steps
+  int kw, groups;     // warps on a tile, and groups of them
+  int halves, steps;  // of K; the warp's steps
   int tiles;
-  int lb, ls;         // next to load: first tile of its round, step
+  int lb, ls;         // next to load: first tile of its group's round, step
   Tile lt[RT];
 
   MOE_DEV Streamer(const Src& source, unsigned char* smem) : src(source) {
@@ -112,12 +136,12 @@ struct Streamer {
 
   MOE_DEV void load_round() {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i, max(tiles - 1, 0)));
+    for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i * groups, max(tiles - 1, 0)));
   }
 
   // Slot i of the ring's `turn`: one group, empty past the last tile, so that the groups count the slots.
   MOE_DEV void load(const Step& at, bool both, int turn, int i) {
-    if (lb + i < tiles) {
+    if (lb + i * groups < tiles) {
       const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3;
       const uint32_t dst = ring + (turn * RT + i) * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
       const bool mine = piece < 4 || both;
@@ -132,32 +156,41 @@ struct Streamer {
     }
     copy_commit();
   }
-  // The second half of a warp's last step may belong to the next warp.
-  MOE_DEV bool both(int s) const { return h0 + 2 * s + 1 < h1; }
+  // Step s of the group's warps covers 2 kw adjacent halves of every row, two a
+  // warp; the last step shares out what is left, one half a warp if that is
+  // enough.  First half of this warp's step, and whether it has the second too.
+  MOE_DEV int half_at(int s) const {
+    const int w = (threadIdx.x >> 5) & (kw - 1), base = 2 * kw * s, left = halves - base;
+    if (left >= 2 * kw) return base + 2 * w;
+    const int twos = max(left - kw, 0);
+    return base + (w < twos ? 2 * w : twos + w);
+  }
+  MOE_DEV bool both(int s) const {
+    const int w = (threadIdx.x >> 5) & (kw - 1), left = halves - 2 * kw * s;
+    return left >= 2 * kw || w < left - kw;
+  }
   MOE_DEV void next_step() {
     if (++ls == steps) {
       ls = 0;
-      lb += RT;
+      lb += RT * groups;
       if (lb < tiles) load_round();
     }
   }
 
   MOE_DEV void prologue(int n_tiles) {
-    const int warp = threadIdx.x >> 5, halves = src.halves();
-    h0 = static_cast<int>(static_cast<int64_t>(halves) * warp / kSW);
-    h1 = static_cast<int>(static_cast<int64_t>(halves) * (warp + 1) / kSW);
-    if constexpr (Src::kWhole) {
-      h0 = (h0 + 1) & ~1;
-      h1 = warp == kSW - 1 ? halves : (h1 + 1) & ~1;
-    }
-    steps = h1 > h0 ? (h1 - h0 + 1) / 2 : 0;
+    halves = src.halves();
+    kw = plan_warps<RT>(n_tiles, halves);
+    groups = kSW / kw;
+    const int w = (threadIdx.x >> 5) & (kw - 1), full = halves >> __ffs(kw);
+    steps = full + (halves - 2 * kw * full > w ? 1 : 0);
     tiles = n_tiles;
-    lb = ls = 0;
-    if (steps == 0) return;
+    lb = (threadIdx.x >> 5) >> (__ffs(kw) - 1);
+    ls = 0;
+    if (steps == 0 || lb >= tiles) return;
     load_round();
 #pragma unroll
     for (int p = 0; p < PD; ++p) {
-      const Step at = src.step(h0 + 2 * ls);
+      const Step at = src.step(half_at(ls));
 #pragma unroll
       for (int i = 0; i < RT; ++i) load(at, both(ls), p, i);
       next_step();
@@ -171,7 +204,8 @@ struct Streamer {
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
     const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
     int turn = 0;
-    for (int base = 0; base < tiles; base += RT) {
+    const int round = RT * groups, shift = __ffs(groups) - 1;
+    for (int base = 0; base < tiles; base += round) {
       float acc[RT][NT][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -181,52 +215,67 @@ struct Streamer {
           for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
       uint4 next[NT][2];
       auto fetch = [&](int s) {
-        const Step at = src.step(h0 + 2 * s);
+        const Step at = src.step(half_at(s));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           src.tokens(at, j, next[j][0], next[j][1]);
           if (!both(s)) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
         }
       };
-      if (steps > 0) fetch(0);
+      const int mine = base + (warp >> (4 - shift)) < tiles ? steps : 0;  // a group without a tile in the last round
+      if (mine > 0) fetch(0);
 #pragma unroll 1
-      for (int s = 0; s < steps; ++s) {
+      for (int s = 0; s < mine; ++s) {
         uint4 x[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           x[j][0] = next[j][0];
           x[j][1] = next[j][1];
         }
-        if (s + 1 < steps) fetch(s + 1);
-        const Step at = src.step(h0 + 2 * ls);
+        if (s + 1 < mine) fetch(s + 1);
+        const Step at = src.step(half_at(ls));
         const bool whole = both(ls);
+        // Two slots at a time where there are two: their reads and mma chains overlap,
+        // and one pair of warp barriers serves both.
+        constexpr int P = RT >= 2 ? 2 : 1;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          copy_wait<D - 1>();
+        for (int i = 0; i < RT; i += P) {
+          copy_wait<D - P>();
           __syncwarp();
-          const uint32_t from = ring + (turn * RT + i) * kStepBytes;
-          const uint4 a0 = ld_shared(from + frag0), b0 = ld_shared(from + frag0 + 1024);
-          const uint4 a1 = ld_shared(from + frag1), b1 = ld_shared(from + frag1 + 1024);
+          uint4 a0[P], a1[P], b0[P], b1[P];
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            const uint32_t from = ring + (turn * RT + i + q) * kStepBytes;
+            a0[q] = ld_shared(from + frag0);
+            b0[q] = ld_shared(from + frag0 + 1024);
+            a1[q] = ld_shared(from + frag1);
+            b1[q] = ld_shared(from + frag1 + 1024);
+          }
           // a slot past the last tile holds an earlier tile's bytes: its sums are never read
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            T::mma(acc[i][j], a0.x, b0.x, a0.y, b0.y, x[j][0].x, x[j][0].y);
-            T::mma(acc[i][j], a0.z, b0.z, a0.w, b0.w, x[j][0].z, x[j][0].w);
-            T::mma(acc[i][j], a1.x, b1.x, a1.y, b1.y, x[j][1].x, x[j][1].y);
-            T::mma(acc[i][j], a1.z, b1.z, a1.w, b1.w, x[j][1].z, x[j][1].w);
+#pragma unroll
+            for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a0[q].x, b0[q].x, a0[q].y, b0[q].y, x[j][0].x, x[j][0].y);
+#pragma unroll
+            for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a0[q].z, b0[q].z, a0[q].w, b0[q].w, x[j][0].z, x[j][0].w);
+#pragma unroll
+            for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a1[q].x, b1[q].x, a1[q].y, b1[q].y, x[j][1].x, x[j][1].y);
+#pragma unroll
+            for (int q = 0; q < P; ++q) T::mma(acc[i + q][j], a1[q].z, b1[q].z, a1[q].w, b1[q].w, x[j][1].z, x[j][1].w);
           }
-          __syncwarp();  // every lane has read the slot
-          load(at, whole, turn, i);
+          __syncwarp();  // every lane has read the slots
+#pragma unroll
+          for (int q = 0; q < P; ++q) load(at, whole, turn, i + q);
         }
         next_step();
         turn = turn + 1 == PD ? 0 : turn + 1;
       }
-      const int nt = min(RT, tiles - base);
-      if (base + RT >= tiles) ahead();
+      const int nt = min(round, tiles - base);
+      if (base + round >= tiles) ahead();
       if (base > 0) __syncthreads();  // the last round's partials have been added
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        if (i < nt) {
+        if (i * groups < nt) {
           float* p = part + (i * kSW + warp) * (NT * kPartTile) + 2 * t4 * kPartCol + g;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -239,14 +288,16 @@ struct Streamer {
         }
       }
       __syncthreads();
-      const int per = FROWS * cols;
-      for (int o = threadIdx.x; o < nt * per; o += kSThreads) {
-        const int tl = o / per, rc = o - tl * per, col = rc / FROWS, row = rc % FROWS;
+      // o = (tile, column, row); o / cols by a 16-bit reciprocal, exact while (o / FROWS) cols < 2^16 (at most 32 x 32 x 32)
+      const uint32_t inverse = 65536u / static_cast<uint32_t>(cols) + 1u;
+      for (int o = threadIdx.x; o < nt * cols * FROWS; o += kSThreads) {
+        const int oc = o / FROWS, row = o % FROWS, tl = static_cast<int>((oc * inverse) >> 16), col = oc - tl * cols;
         fin(base + tl, row, col, [&](int r, int c) {
-          const float* p = part + tl * kSW * (NT * kPartTile) + (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
+          // tile tl of the round: the (tl / groups)-th of group tl % groups
+          const float* p = part + (((tl >> shift) << 4) + ((tl & (groups - 1)) << (4 - shift))) * (NT * kPartTile) +
+                           (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
           float v = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kSW; ++w) v += p[w * (NT * kPartTile)];
+          for (int w = 0; w < kw; w += 2) v += p[w * (NT * kPartTile)] + p[(w + 1) * (NT * kPartTile)];
           return v;
         });
       }
