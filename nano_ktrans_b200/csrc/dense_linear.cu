@@ -101,40 +101,46 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 template <bool GATED, int NT>
 struct LinearSrc {
   struct Tile {
-    const uint16_t *p, *u;  // this lane's first row, of each weight when gated
+    const uint16_t *p, *u;  // this lane's first row (the block's last one where there is none), of each weight when gated
     int left;               // rows from there to the block's end
   };
-  struct Step {
-    int k;
-  };
   const LinearArgs& a;
-  int r0, r1, q, t8;
+  int r0, r1, t8;
   const uint16_t* xrow[NT];
   MOE_DEV LinearSrc(const LinearArgs& args, int lo, int hi) : a(args), r0(lo), r1(hi) {
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    q = lane >> 3;
     t8 = 8 * (lane & 3);
 #pragma unroll
     for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.m ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
   }
-  MOE_DEV int halves() const { return (a.k + 31) / 32; }
-  MOE_DEV const uint16_t* any() const { return a.w; }
+  MOE_DEV int length() const { return a.k; }
   MOE_DEV Tile tile(int i) const {
-    const int r = r0 + (GATED ? 8 : 16) * i + q;
-    return {a.w + r * a.ldw, GATED ? a.w_up + r * a.ldwu : nullptr, r1 - r};
+    const int r = r0 + (GATED ? 8 : 16) * i + ((threadIdx.x & 31) >> 3), in = min(r, r1 - 1);
+    return {a.w + in * a.ldw, GATED ? a.w_up + in * a.ldwu : nullptr, r1 - r};
   }
-  MOE_DEV Step step(int half) const { return {32 * half}; }
-  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
-    n = a.k - s.k;
-    if constexpr (GATED)
-      p = t.left > 4 * (i & 1) ? (i < 2 ? t.p + (i & 1) * 4 * a.ldw : t.u + (i & 1) * 4 * a.ldwu) + s.k : nullptr;
-    else
-      p = t.left > 4 * i ? t.p + 4 * i * a.ldw + s.k : nullptr;
+  MOE_DEV void rows(const Tile& t, int k, const uint16_t* (&p)[4], uint32_t& valid) const {
+    if constexpr (GATED) {
+      const bool two = t.left > 4;
+      p[0] = t.p + k;
+      p[1] = p[0] + (two ? 4 * a.ldw : 0);
+      p[2] = t.u + k;
+      p[3] = p[2] + (two ? 4 * a.ldwu : 0);
+      valid = (t.left > 0 ? 5u : 0u) | (two ? 10u : 0u);
+    } else {
+      p[0] = t.p + k;
+      valid = t.left > 0 ? 1u : 0u;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        const bool in = t.left > 4 * i;
+        p[i] = p[0] + (in ? 4 * i * a.ldw : 0);
+        valid |= in ? 1u << i : 0u;
+      }
+    }
   }
-  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
+  MOE_DEV void tokens(int k, int j, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = xrow[j] != nullptr && s.k + t8 < a.k ? ld_tokens(xrow[j] + s.k) : z;
-    x1 = xrow[j] != nullptr && s.k + 32 + t8 < a.k ? ld_tokens(xrow[j] + s.k + 32) : z;
+    x0 = xrow[j] != nullptr && k + t8 < a.k ? ld_tokens(xrow[j] + k) : z;
+    x1 = xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
   }
 };
 

@@ -174,7 +174,8 @@ MOE_DEV void route_warp(const uint16_t* row, const MoeArgs& a, int& id, float& w
 
 // Routing of a call, in shared memory.
 struct Tables {
-  float weight[kMoePairs + 1][kMoeTokens];  // [place in the active list][token]; entries of routed pairs only
+  float weight[kMoePairs + 1][kMoeTokens];  // [place in the active list][i]: the expert's i-th token's weight,
+  uint8_t list[kMoePairs + 1][kMoeTokens];  // and which token that is
   uint32_t tokens[kMoePairs + 1];           // tokens of an active expert, one bit each; the shared expert's come last
   int active[kMoePairs];                    // routed experts, ascending
   uint32_t used[kMoeExperts / 32];          // routed experts, one bit each
@@ -212,32 +213,25 @@ MOE_DEV int place_of(const MoeArgs& a, int row) { return static_cast<int>(__umul
 
 // Gate and up rows [lo, hi) of the list of intermediate rows (multiples of 8).
 // Tile i is its i-th group of 8 (a group never spans two experts: their sizes
-// are multiples of 16).
-template <int NT>
+// are multiples of 16).  Column c is token list[c], or token c without a list.
 struct GateUpSrc {
   struct Tile {
     const uint16_t *g, *u;  // this lane's first gate and up row
   };
-  struct Step {
-    int k;
-  };
   const MoeArgs& a;
   const Tables& tb;
-  int lo, hi, routed, q, t8;
-  const uint16_t* xrow[NT];
-  MOE_DEV GateUpSrc(const MoeArgs& args, const Tables& tables, int lo_, int hi_)
+  int lo, hi, routed, t8;
+  const uint16_t* xrow;
+  MOE_DEV GateUpSrc(const MoeArgs& args, const Tables& tables, int lo_, int hi_, const uint8_t* list, int cols)
       : a(args), tb(tables), lo(lo_), hi(hi_), routed(tables.n_active * args.inter) {
     const int lane = threadIdx.x & 31, g = lane >> 2;
-    q = lane >> 3;
     t8 = 8 * (lane & 3);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) xrow[j] = 8 * j + g < a.tokens ? a.x + (8 * j + g) * a.ldx + t8 : nullptr;
+    xrow = g < cols ? a.x + (list != nullptr ? list[g] : g) * a.ldx + t8 : nullptr;
   }
-  MOE_DEV int halves() const { return (a.hidden + 31) / 32; }
+  MOE_DEV int length() const { return a.hidden; }
   MOE_DEV int tiles() const { return (hi - lo) / 8; }
-  MOE_DEV const uint16_t* any() const { return a.gate; }
   MOE_DEV Tile tile(int i) const {
-    const int v = lo + 8 * i;
+    const int v = lo + 8 * i, q = (threadIdx.x & 31) >> 3;
     if (v < routed) {
       const int s = place_of(a, v);
       const int64_t at = (static_cast<int64_t>(tb.active[s]) * a.inter + (v - s * a.inter) + q) * a.hidden;
@@ -246,15 +240,17 @@ struct GateUpSrc {
     const int64_t at = static_cast<int64_t>(v - routed + q) * a.hidden;
     return {a.shared_gate + at, a.shared_up + at};
   }
-  MOE_DEV Step step(int half) const { return {32 * half}; }
-  MOE_DEV void row(const Tile& t, const Step& s, int i, const uint16_t*& p, int& n) const {
-    n = a.hidden - s.k;
-    p = (i < 2 ? t.g : t.u) + (i & 1) * 4 * a.hidden + s.k;
+  MOE_DEV void rows(const Tile& t, int k, const uint16_t* (&p)[4], uint32_t& valid) const {
+    p[0] = t.g + k;
+    p[1] = p[0] + 4 * a.hidden;
+    p[2] = t.u + k;
+    p[3] = p[2] + 4 * a.hidden;
+    valid = 15u;
   }
-  MOE_DEV void tokens(const Step& s, int j, uint4& x0, uint4& x1) const {
+  MOE_DEV void tokens(int k, int, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
-    x0 = xrow[j] != nullptr && s.k + t8 < a.hidden ? ld_tokens(xrow[j] + s.k) : z;
-    x1 = xrow[j] != nullptr && s.k + 32 + t8 < a.hidden ? ld_tokens(xrow[j] + s.k + 32) : z;
+    x0 = xrow != nullptr && k + t8 < a.hidden ? ld_tokens(xrow + k) : z;
+    x1 = xrow != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow + k + 32) : z;
   }
 };
 
@@ -304,7 +300,7 @@ struct DownStreamer {
       const uint16_t* p = take ? lp.w + static_cast<int64_t>(r) * lp.ld + k : a.down;
       const int64_t four = take ? 4 * static_cast<int64_t>(lp.ld) : 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) copy16(dst + q * 512, p + q * four, take);
+      for (int q = 0; q < 4; ++q) copy16(dst + q * 512, p + q * four, take ? 16u : 0u);
     }
     copy_commit();
   }
@@ -424,9 +420,8 @@ MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
 }
 
-// NT column tiles hold the tokens of the gate / up phase; the down phase has up
-// to ND column tiles of 4 tokens and RD row tiles at once.
-template <typename T, int NT, int ND, int RD>
+// The down phase has up to ND column tiles of 4 tokens and takes RD row tiles at once.
+template <typename T, int ND, int RD>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Tables tb;
@@ -481,7 +476,6 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     place = __popc(tb.used[id >> 5] & ((1u << (id & 31)) - 1u));
     for (int i = 0; i < id >> 5; ++i) place += __popc(tb.used[i]);
     tb.active[place] = id;
-    tb.weight[place][warp] = wt;
     atomicOr(&tb.tokens[place], 1u << warp);
   }
   if (warp == kSW - 1) {  // 32 words of 32 experts
@@ -491,8 +485,17 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     if (lane == 0) tb.n_active = n;
     if (a.shared_inter > 0) {  // every token's, in the place after the last routed expert
       if (lane == 0) tb.tokens[n] = (1u << a.tokens) - 1u;
-      if (lane < a.tokens) tb.weight[n][lane] = __ldcg(a.shared_open + lane);
+      if (lane < a.tokens) {
+        tb.weight[n][lane] = __ldcg(a.shared_open + lane);
+        tb.list[n][lane] = static_cast<uint8_t>(lane);
+      }
     }
+  }
+  __syncthreads();
+  if (place >= 0) {
+    const int i = __popc(tb.tokens[place] & ((1u << warp) - 1u));
+    tb.weight[place][i] = wt;
+    tb.list[place][i] = static_cast<uint8_t>(warp);
   }
   __syncthreads();
 
@@ -503,18 +506,44 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   const int last = min(first + split.per_block, split.ranges);
   for (int r = first; r < last; ++r) {
     const int lo = split.begin(r), hi = split.begin(r + 1);
-    const GateUpSrc<NT> src(a, tb, lo, hi);
-    Streamer<T, NT, kSlots / NT, 8, GateUpSrc<NT>> up(src, smem);
     DownStreamer<T, ND, RD> down(a, tb, smem, hs, a.h_cap, r, lo, hi);
-    up.prologue(src.tiles());
-    up.run(a.tokens, [&](int tile, int row, int col, auto sum) {
-      const int v = lo + 8 * tile, place = v < src.routed ? place_of(a, v) : tb.n_active;
-      const uint32_t toks = tb.tokens[place], bit = 1u << col;
-      if ((toks & bit) == 0) return;
-      const float h = tb.weight[place][col] * (silu_f32(sum(row, col)) * sum(row + 8, col));
-      uint16_t* p = hs + __popc(toks & (bit - 1u)) * a.h_cap + 8 * tile + row;
-      store_split<T>(p, p + a.tokens * a.h_cap, h);
-    }, [&] { down.prologue(); });
+    const auto put = [&](int place, int i, int v, float gate, float up) {
+      uint16_t* p = hs + i * a.h_cap + (v - lo);
+      store_split<T>(p, p + a.tokens * a.h_cap, tb.weight[place][i] * (silu_f32(gate) * up));
+    };
+    if constexpr (ND <= 2) {
+      // at most 8 tokens: one column tile holds them all, for all rows of the range at once
+      const GateUpSrc src(a, tb, lo, hi, nullptr, a.tokens);
+      Streamer<T, 1, kSlots, 8, GateUpSrc> up(src, smem);
+      up.prologue(src.tiles());
+      up.run(a.tokens, [&](int tile, int row, int col, auto sum) {
+        const int v = lo + 8 * tile, place = v < src.routed ? place_of(a, v) : tb.n_active;
+        const uint32_t toks = tb.tokens[place], bit = 1u << col;
+        if (toks & bit) put(place, __popc(toks & (bit - 1u)), v + row, sum(row, col), sum(row + 8, col));
+      }, [&] { down.prologue(); });
+    } else {
+      // Expert by expert, only the tokens routed there as columns, 8 at a time:
+      // with all 16 as columns of every expert the token fragments were as many
+      // bytes as the weights (16 tokens, 128 x 768 experts: 178 us).
+      const int routed = tb.n_active * a.inter;
+      for (int v = lo; v < hi;) {
+        const int place = v < routed ? place_of(a, v) : tb.n_active;
+        const int end = v < routed ? min(hi, (place + 1) * a.inter) : hi, n = __popc(tb.tokens[place]);
+        for (int c0 = 0; c0 < n; c0 += 8) {
+          const int cols = min(8, n - c0);
+          const GateUpSrc src(a, tb, v, end, &tb.list[place][c0], cols);
+          Streamer<T, 1, kSlots, 8, GateUpSrc> up(src, smem);
+          up.prologue(src.tiles());
+          up.run(cols, [&](int tile, int row, int col, auto sum) {
+            put(place, c0 + col, v + 8 * tile + row, sum(row, col), sum(row + 8, col));
+          }, [&] {
+            if (end == hi && c0 + 8 >= n) down.prologue();
+          });
+          __syncthreads();  // the partials may be overwritten
+        }
+        v = end;
+      }
+    }
     __syncthreads();  // h is complete
     down.run();
     __syncthreads();  // h may be written again
@@ -621,9 +650,9 @@ int64_t moe_pieces(const MoeArgs& a, int sms) {
   return sms * (per_block > 0 ? per_block : 1) + most + 1;
 }
 
-template <typename T, int NT, int ND, int RD>
+template <typename T, int ND, int RD>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
-  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, NT, ND, RD>);
+  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, ND, RD>);
   constexpr size_t smem = kStreamBytes + kHBytes;
   static_assert(smem + sizeof(Tables) + 1024 <= 232448, "shared-memory plan");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
@@ -639,17 +668,17 @@ static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, NT, ND, RD>, a);
+  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, ND, RD>, a);
 }
 
-template <typename T, int NT, int ND>
+template <typename T, int ND>
 static cudaError_t moe_tiles(const MoeArgs& a, int sms, cudaStream_t st) {
   const int rd = tiles_at_once<ND>((a.hidden / 16 + kSW - 1) / kSW);  // a warp's tiles
   if constexpr (ND == 1)
-    if (rd == 4) return moe_main<T, NT, ND, 4>(a, sms, st);
+    if (rd == 4) return moe_main<T, ND, 4>(a, sms, st);
   if constexpr (ND <= 2)
-    if (rd == 2) return moe_main<T, NT, ND, 2>(a, sms, st);
-  return moe_main<T, NT, ND, 1>(a, sms, st);
+    if (rd == 2) return moe_main<T, ND, 2>(a, sms, st);
+  return moe_main<T, ND, 1>(a, sms, st);
 }
 
 template <typename T>
@@ -665,9 +694,9 @@ static cudaError_t moe_both(const MoeArgs& a, int sms, cudaStream_t st) {
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, dense_router_kernel<T>, a);
   if (e != cudaSuccess) return e;
-  if (a.tokens <= 4) return moe_tiles<T, 1, 1>(a, sms, st);
-  if (a.tokens <= 8) return moe_tiles<T, 1, 2>(a, sms, st);
-  return moe_tiles<T, 2, 4>(a, sms, st);
+  if (a.tokens <= 4) return moe_tiles<T, 1>(a, sms, st);
+  if (a.tokens <= 8) return moe_tiles<T, 2>(a, sms, st);
+  return moe_tiles<T, 4>(a, sms, st);
 }
 
 cudaError_t launch_dense_moe(MoeArgs a, int dtype, int sms, cudaStream_t st) {

@@ -40,9 +40,9 @@ constexpr int kPartCol = 20;            // floats per column of a partial tile: 
                                         // of a store fall into different banks
 constexpr int kPartTile = 8 * kPartCol;
 
-// 16 bytes global -> shared, past L1; zeros where !take (nothing is read then).
-MOE_DEV void copy16(uint32_t dst, const uint16_t* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+// 16 bytes global -> shared, past L1; zeros where bytes is 0 instead of 16.
+MOE_DEV void copy16(uint32_t dst, const uint16_t* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 MOE_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -106,12 +106,12 @@ MOE_DEV int plan_warps(int tiles, int halves) {
 constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * kSlots * kStepBytes + sizeof(float) * 4 * kSW * kPartTile;
 
 // NT column tiles of 8 tokens (1, 2 or 4), RT row tiles (RT * NT <= 4).  Src:
-//   halves()                  K in halves of 32 elements
-//   Tile tile(int)            what copying a tile's rows needs, rows (lane / 8) + 4 i
-//   Step step(int half)       what a step needs: where it is in K
-//   row(Tile, Step, i, p, n)  row i's address at the step's first element (null: zeros), elements from there to its end
-//   tokens(Step, j, x0, x1)   column 8 j + g at 8 t and 32 + 8 t of the step (zeros outside)
-//   fin(tile, row, col, sum)  one output; sum(row, col) adds the partials
+//   length()                 K
+//   Tile tile(int)           what copying a tile's rows needs
+//   rows(Tile, k, p, valid)  addresses at element k of rows (lane / 8) + 4 i, i < 4, and a bit for each that exists (every
+//                            address has to be readable for k < K)
+//   tokens(k, j, x0, x1)     column 8 j + g at elements k + 8 t and k + 32 + 8 t (zeros outside)
+//   fin(tile, row, col, sum) one output; sum(row, col) adds the partials
 // FROWS outputs per column and tile (16, or 8 where rows g and g + 8 belong to
 // one output), `cols` columns.
 template <typename T, int NT, int RT, int FROWS, class Src>
@@ -119,7 +119,6 @@ struct Streamer {
   static constexpr int D = kSlots, PD = D / RT;  // steps ahead
   static_assert(RT * NT <= 4, "partials");
   using Tile = typename Src::Tile;
-  using Step = typename Src::Step;
   const Src& src;
   uint32_t ring;      // the warp's ring
   float* part;
@@ -139,20 +138,27 @@ struct Streamer {
     for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i * groups, max(tiles - 1, 0)));
   }
 
+  // Where this lane's pieces of step s are: element offset (0 where there is
+  // nothing to copy), and whether there is.
+  struct At {
+    int k;
+    uint32_t bytes;
+  };
+  MOE_DEV At at_step(int s) const {
+    const int piece = threadIdx.x & 7, k = 32 * half_at(s) + 8 * piece;
+    const bool ok = (piece < 4 || both(s)) && k < src.length();
+    return {ok ? k : 0, ok ? 16u : 0u};
+  }
   // Slot i of the ring's `turn`: one group, empty past the last tile, so that the groups count the slots.
-  MOE_DEV void load(const Step& at, bool both, int turn, int i) {
+  MOE_DEV void load(const At& at, int turn, int i) {
     if (lb + i * groups < tiles) {
       const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3;
       const uint32_t dst = ring + (turn * RT + i) * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
-      const bool mine = piece < 4 || both;
+      const uint16_t* p[4];
+      uint32_t valid;
+      src.rows(lt[i], at.k, p, valid);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint16_t* p;
-        int n;
-        src.row(lt[i], at, r, p, n);
-        const bool take = p != nullptr && 8 * piece < n && mine;
-        copy16(dst + r * 512, take ? p + 8 * piece : src.any(), take);
-      }
+      for (int r = 0; r < 4; ++r) copy16(dst + r * 512, p[r], (valid >> r & 1u) ? at.bytes : 0u);
     }
     copy_commit();
   }
@@ -178,7 +184,7 @@ struct Streamer {
   }
 
   MOE_DEV void prologue(int n_tiles) {
-    halves = src.halves();
+    halves = (src.length() + 31) / 32;
     kw = plan_warps<RT>(n_tiles, halves);
     groups = kSW / kw;
     const int w = (threadIdx.x >> 5) & (kw - 1), full = halves >> __ffs(kw);
@@ -190,9 +196,9 @@ struct Streamer {
     load_round();
 #pragma unroll
     for (int p = 0; p < PD; ++p) {
-      const Step at = src.step(half_at(ls));
+      const At at = at_step(ls);
 #pragma unroll
-      for (int i = 0; i < RT; ++i) load(at, both(ls), p, i);
+      for (int i = 0; i < RT; ++i) load(at, p, i);
       next_step();
     }
   }
@@ -215,10 +221,10 @@ struct Streamer {
           for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
       uint4 next[NT][2];
       auto fetch = [&](int s) {
-        const Step at = src.step(half_at(s));
+        const int k = 32 * half_at(s);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          src.tokens(at, j, next[j][0], next[j][1]);
+          src.tokens(k, j, next[j][0], next[j][1]);
           if (!both(s)) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
         }
       };
@@ -233,8 +239,7 @@ struct Streamer {
           x[j][1] = next[j][1];
         }
         if (s + 1 < mine) fetch(s + 1);
-        const Step at = src.step(half_at(ls));
-        const bool whole = both(ls);
+        const At at = at_step(ls);
         // Two slots at a time where there are two: their reads and mma chains overlap,
         // and one pair of warp barriers serves both.
         constexpr int P = RT >= 2 ? 2 : 1;
@@ -265,7 +270,7 @@ struct Streamer {
           }
           __syncwarp();  // every lane has read the slots
 #pragma unroll
-          for (int q = 0; q < P; ++q) load(at, whole, turn, i + q);
+          for (int q = 0; q < P; ++q) load(at, turn, i + q);
         }
         next_step();
         turn = turn + 1 == PD ? 0 : turn + 1;
