@@ -193,7 +193,7 @@ static cudaError_t stream_launch(const LinearArgs& a, int sms, cudaStream_t st) 
 template <typename T, bool GATED, int NT>
 static cudaError_t stream_tiles(const LinearArgs& a, int sms, cudaStream_t st) {
   const int rows = (a.n + sms - 1) / sms, tile = GATED ? 8 : 16;  // a block's rows
-  const int rt = tiles_at_once<NT>((rows + tile - 1) / tile);
+  const int rt = tiles_at_once<NT>((rows + tile - 1) / tile, a.k);
   if constexpr (NT == 1)
     if (rt == 4) return stream_launch<T, GATED, NT, 4>(a, sms, st);
   if constexpr (NT <= 2)

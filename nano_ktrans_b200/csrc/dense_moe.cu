@@ -420,8 +420,8 @@ MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
 }
 
-// The down phase has up to ND column tiles of 4 tokens and takes RD row tiles at once.
-template <typename T, int ND, int RD>
+// The gate / up phase takes RG row tiles at once, the down phase RD, with up to ND column tiles of 4 tokens.
+template <typename T, int ND, int RG, int RD>
 __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_constant__ MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Tables tb;
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     if constexpr (ND <= 2) {
       // at most 8 tokens: one column tile holds them all, for all rows of the range at once
       const GateUpSrc src(a, tb, lo, hi, nullptr, a.tokens);
-      Streamer<T, 1, kSlots, 8, GateUpSrc> up(src, smem);
+      Streamer<T, 1, RG, 8, GateUpSrc> up(src, smem);
       up.prologue(src.tiles());
       up.run(a.tokens, [&](int tile, int row, int col, auto sum) {
         const int v = lo + 8 * tile, place = v < src.routed ? place_of(a, v) : tb.n_active;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
         for (int c0 = 0; c0 < n; c0 += 8) {
           const int cols = min(8, n - c0);
           const GateUpSrc src(a, tb, v, end, &tb.list[place][c0], cols);
-          Streamer<T, 1, kSlots, 8, GateUpSrc> up(src, smem);
+          Streamer<T, 1, RG, 8, GateUpSrc> up(src, smem);
           up.prologue(src.tiles());
           up.run(cols, [&](int tile, int row, int col, auto sum) {
             put(place, c0 + col, v + 8 * tile + row, sum(row, col), sum(row + 8, col));
@@ -581,33 +581,32 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   }
 
   // ---- out = r + the pieces' sums ----
-  // A warp adds up four outputs of a token: lane l takes its pieces l, l + 32,
-  // ... (experts ascending), then the lanes' sums are added in a fixed tree.
+  // `lanes` neighbouring lanes add up a quad, four outputs of a token: lane l of
+  // them takes pieces l, l + lanes, ... (experts ascending), four reads under way
+  // at once, then their sums are added in a fixed tree.  As many lanes as let the
+  // block take all its quads in one pass, but 8 at least.
   const int quads = a.hidden / 4;
   const int64_t all = static_cast<int64_t>(quads) * a.tokens;
   const int q0 = static_cast<int>(all * blockIdx.x / gridDim.x), q1 = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x);
-  for (int q = q0 + warp; q < q1; q += kSW) {
-    const int tok = q / quads, col = q - tok * quads, n = tb.n_places[tok];
-    const int total = n > 0 ? tb.pieces[tok][n] : 0;
-    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (lane == 0 && a.res != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = T::to_f32(a.res[tok * a.ldr + 4 * col + i]);
-    }
+  int lanes = 32;
+  while (lanes > 8 && kSThreads / lanes < q1 - q0) lanes /= 2;
+  for (int qb = q0; qb < q1; qb += kSThreads / lanes) {
+    const int q = qb + tid / lanes, tok = min(q, q1 - 1) / quads, col = min(q, q1 - 1) - tok * quads;
+    const int total = q < q1 && tb.n_places[tok] > 0 ? tb.pieces[tok][tb.n_places[tok]] : 0;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    int j = 0;
-    for (int p0 = 0; p0 < total; p0 += 128) {
+    int j = 0;  // place in the token's list
+    for (int p0 = tid & (lanes - 1); p0 < total; p0 += 4 * lanes) {
       float4 f[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int p = p0 + 32 * u + lane;
+        const int p = p0 + u * lanes;
         f[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p < total) {
           while (p >= tb.pieces[tok][j + 1]) ++j;
-          const int place_j = tb.place[tok][j], at = tb.range[tok][j] + p - tb.pieces[tok][j] + place_j;
-          const int i = __popc(tb.tokens[place_j] & ((1u << tok) - 1u));
-          f[u] = __ldcg(reinterpret_cast<const float4*>(
-              a.partial + (static_cast<int64_t>(at) * a.tokens + i) * a.hidden + 4 * col));
+          const int at_place = tb.place[tok][j], at = tb.range[tok][j] + p - tb.pieces[tok][j] + at_place;
+          const int i = __popc(tb.tokens[at_place] & ((1u << tok) - 1u));
+          f[u] = __ldcg(reinterpret_cast<const float4*>(a.partial + (static_cast<int64_t>(at) * a.tokens + i) * a.hidden +
+                                                        4 * col));
         }
       }
 #pragma unroll
@@ -618,19 +617,23 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
         s.w += f[u].w;
       }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
+    __syncwarp();
+    for (int off = lanes / 2; off > 0; off >>= 1) {
       s.x += __shfl_xor_sync(kFullMask, s.x, off);
       s.y += __shfl_xor_sync(kFullMask, s.y, off);
       s.z += __shfl_xor_sync(kFullMask, s.z, off);
       s.w += __shfl_xor_sync(kFullMask, s.w, off);
     }
-    if (lane == 0) {
+    if (q < q1 && (tid & (lanes - 1)) == 0) {
+      const float v[4] = {s.x, s.y, s.z, s.w};
       uint16_t* o = a.out + tok * a.ldo + 4 * col;
-      o[0] = T::from_f32(s.x + r[0]);
-      o[1] = T::from_f32(s.y + r[1]);
-      o[2] = T::from_f32(s.z + r[2]);
-      o[3] = T::from_f32(s.w + r[3]);
+      float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (a.res != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = T::to_f32(a.res[tok * a.ldr + 4 * col + i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = T::from_f32(v[i] + r[i]);
     }
   }
 }
@@ -650,9 +653,9 @@ int64_t moe_pieces(const MoeArgs& a, int sms) {
   return sms * (per_block > 0 ? per_block : 1) + most + 1;
 }
 
-template <typename T, int ND, int RD>
+template <typename T, int ND, int RG, int RD>
 static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
-  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, ND, RD>);
+  const void* kern = reinterpret_cast<const void*>(dense_moe_kernel<T, ND, RG, RD>);
   constexpr size_t smem = kStreamBytes + kHBytes;
   static_assert(smem + sizeof(Tables) + 1024 <= 232448, "shared-memory plan");
   if (!ensure_dynamic_smem(kern, smem, kSThreads)) return cudaErrorInvalidConfiguration;
@@ -668,17 +671,22 @@ static cudaError_t moe_main(const MoeArgs& a, int sms, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, ND, RD>, a);
+  return cudaLaunchKernelEx(&cfg, dense_moe_kernel<T, ND, RG, RD>, a);
+}
+
+template <typename T, int ND, int RG>
+static cudaError_t moe_down(const MoeArgs& a, int sms, cudaStream_t st) {
+  const int rd = tiles_at_once<ND>((a.hidden / 16 + kSW - 1) / kSW, kLongK);  // a warp's tiles
+  if constexpr (ND == 1)
+    if (rd == 4) return moe_main<T, ND, RG, 4>(a, sms, st);
+  if constexpr (ND <= 2)
+    if (rd == 2) return moe_main<T, ND, RG, 2>(a, sms, st);
+  return moe_main<T, ND, RG, 1>(a, sms, st);
 }
 
 template <typename T, int ND>
 static cudaError_t moe_tiles(const MoeArgs& a, int sms, cudaStream_t st) {
-  const int rd = tiles_at_once<ND>((a.hidden / 16 + kSW - 1) / kSW);  // a warp's tiles
-  if constexpr (ND == 1)
-    if (rd == 4) return moe_main<T, ND, 4>(a, sms, st);
-  if constexpr (ND <= 2)
-    if (rd == 2) return moe_main<T, ND, 2>(a, sms, st);
-  return moe_main<T, ND, 1>(a, sms, st);
+  return tiles_at_once<1>(kSlots, a.hidden) == 4 ? moe_down<T, ND, 4>(a, sms, st) : moe_down<T, ND, 2>(a, sms, st);
 }
 
 template <typename T>

@@ -3,28 +3,30 @@
 //
 // With a handful of tokens a projection is bound by reading its weights once.
 // A block owns a range of weight rows, cut into tiles of 16 (the mma's M;
-// tokens are its N, 8 per column tile).  Groups of KW warps split K evenly, in
-// halves of 32 elements, and each warp walks its part in steps of 64 elements;
-// for a step it takes up to RT tiles one after the other, so a token fragment
-// is loaded once for RT weight tiles (loading it for every tile cost 8 of 31 us
-// at 118 MB of weights and 7 tokens: those loads queue behind the weights').
-// The 16 / KW groups work on different tiles (plan_warps).  Lane
-// (g, t) feeds the mma with 8 consecutive elements at 8 t and at 32 + 8 t of
-// rows g and g + 8 (A) and of token column g (B): an mma is unchanged by a
-// permutation of K that both operands share, so nothing is shuffled.
+// tokens are its N, 8 per column tile).  The 16 warps share K: in a step they
+// cover 16 adjacent stretches of 64 elements of every row, one a warp, and what
+// K leaves over is shared out in halves of 32, so that the warps differ by one
+// half at most.  (Fewer warps on a tile and several tiles at once need fewer
+// sums, but read DRAM in shorter runs: 8 experts of 14336, 5 tokens, 419 us with
+// 16 warps on a tile, 447 with 4.)  For a step a warp takes up to RT tiles, so a
+// token fragment is loaded once for RT weight tiles; the first step's, the same
+// in every round of tiles, is kept.  Lane (g, t) feeds the mma with 8 consecutive
+// elements at 8 t and at 32 + 8 t of rows g and g + 8 (A) and of token column g
+// (B): an mma is unchanged by a permutation of K that both operands share, so
+// nothing is shuffled.
 //
 // Weights in flight: a warp copies a step's 16 rows x 128 bytes of each tile
 // into its own ring of D = PD x RT slots in shared memory with cp.async, whole
 // 128-byte lines at a time, PD steps ahead, and waits for its own copies only;
-// 16 warps x D x 2 KB = 128 KB per SM are under way (6.5 TB/s x 1 us / 148 SMs
-// is 44 KB).  Rows are stored with the 64-byte halves of odd rows swapped, so
+// 16 warps x D x 2 KB = 128 KB per SM are under way (7 TB/s x 1 us / 148 SMs
+// is 47 KB).  Rows are stored with the 64-byte halves of odd rows swapped, so
 // that the fragment reads (two rows a phase) meet no bank conflict.  Addresses
 // are split into a part per tile (kept in registers for a round of RT tiles)
 // and a part per step, so that a slot costs a few tens of instructions: with
 // both worked out per slot the issue slots, not the memory, were the limit.
 //
 // Partial sums: a warp keeps RT tiles in registers over its part of K, puts the
-// 16 x 8 partial tiles into shared memory, and the block adds the KW partials
+// 16 x 8 partial tiles into shared memory, and the block adds the 16 partials
 // of each output in warp order (no atomics: the same bits every run) while the
 // next tiles' copies are in flight.
 #pragma once
@@ -71,35 +73,17 @@ constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
 constexpr int kSlots = 4;  // of a warp's ring
 
-// Tiles that a warp keeps in registers when its block has `tiles`: as many as
-// share a token fragment, but no more than there are, since a ring slot of a
-// tile that does not exist is a copy less in flight (2048 x 2048, one token: 4.0
-// us, with slots for four tiles where there is one 5.0).
+// Tiles that a warp keeps in registers when its block has `tiles` of K `k`: as
+// many as share a token fragment, but no more than there are, since a ring slot
+// of a tile that does not exist is a copy less in flight (2048 x 2048, one token:
+// 4.0 us, with slots for four tiles where there is one 5.0); and two where a
+// round of four would be over after two steps (128 x 768 experts, hidden 2048,
+// 16 tokens: 149 us with two, 164 with four; 8 x 14336, hidden 4096: 439 and 424).
+constexpr int kLongK = 2 * 64 * kSW + 1;
 template <int NT>
-inline int tiles_at_once(int tiles) {
+inline int tiles_at_once(int tiles, int k) {
   const int most = kSlots / NT;
-  return tiles >= 3 && most >= 4 ? 4 : tiles >= 2 && most >= 2 ? 2 : 1;
-}
-
-// Warps that share K, for a block with `tiles` tiles of `halves` halves, RT of
-// them at once in a warp.  A warp's time is its steps times its group's tiles,
-// plus about three steps' worth for every round of RT tiles (two block
-// barriers and the sum over the group's partials): few warps on a tile make
-// the rounds long, many spread few tiles over all warps.  (26 tiles of 2048
-// elements, 16 tokens: 16 warps a tile 91 units by this count, 4 warps 68.)
-template <int RT>
-MOE_DEV int plan_warps(int tiles, int halves) {
-  int best = kSW, cost = 1 << 30;
-#pragma unroll
-  for (int l = 4; l >= 1; --l) {  // 1 << l warps; shifts, since this is on the way to the first load
-    const int each = (tiles + (kSW >> l) - 1) >> (4 - l), steps = (halves + (2 << l) - 1) >> (l + 1);
-    const int c = steps * each + 3 * ((each + RT - 1) / RT);
-    if (c < cost) {
-      cost = c;
-      best = 1 << l;
-    }
-  }
-  return best;
+  return tiles >= 3 && most >= 4 && k >= kLongK ? 4 : tiles >= 2 && most >= 2 ? 2 : 1;
 }
 
 // Dynamic shared memory of a Streamer: the ring of four slots a warp, then the partials.
@@ -122,10 +106,9 @@ struct Streamer {
   const Src& src;
   uint32_t ring;      // the warp's ring
   float* part;
-  int kw, groups;     // warps on a tile, and groups of them
   int halves, steps;  // of K; the warp's steps
   int tiles;
-  int lb, ls;         // next to load: first tile of its group's round, step
+  int lb, ls;         // next to load: first tile of its round, step
   Tile lt[RT];
 
   MOE_DEV Streamer(const Src& source, unsigned char* smem) : src(source) {
@@ -135,7 +118,7 @@ struct Streamer {
 
   MOE_DEV void load_round() {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i * groups, max(tiles - 1, 0)));
+    for (int i = 0; i < RT; ++i) lt[i] = src.tile(min(lb + i, tiles - 1));
   }
 
   // Where this lane's pieces of step s are: element offset (0 where there is
@@ -151,7 +134,7 @@ struct Streamer {
   }
   // Slot i of the ring's `turn`: one group, empty past the last tile, so that the groups count the slots.
   MOE_DEV void load(const At& at, int turn, int i) {
-    if (lb + i * groups < tiles) {
+    if (lb + i < tiles) {
       const int lane = threadIdx.x & 31, piece = lane & 7, row = lane >> 3;
       const uint32_t dst = ring + (turn * RT + i) * kStepBytes + row * 128 + ((piece ^ ((row & 1) << 2)) << 4);
       const uint16_t* p[4];
@@ -162,37 +145,33 @@ struct Streamer {
     }
     copy_commit();
   }
-  // Step s of the group's warps covers 2 kw adjacent halves of every row, two a
-  // warp; the last step shares out what is left, one half a warp if that is
-  // enough.  First half of this warp's step, and whether it has the second too.
+  // First half of this warp's step s (the last step shares out what is left, one
+  // half a warp if that is enough), and whether the step has a second.
   MOE_DEV int half_at(int s) const {
-    const int w = (threadIdx.x >> 5) & (kw - 1), base = 2 * kw * s, left = halves - base;
-    if (left >= 2 * kw) return base + 2 * w;
-    const int twos = max(left - kw, 0);
+    const int w = threadIdx.x >> 5, base = 2 * kSW * s, left = halves - base;
+    if (left >= 2 * kSW) return base + 2 * w;
+    const int twos = max(left - kSW, 0);
     return base + (w < twos ? 2 * w : twos + w);
   }
   MOE_DEV bool both(int s) const {
-    const int w = (threadIdx.x >> 5) & (kw - 1), left = halves - 2 * kw * s;
-    return left >= 2 * kw || w < left - kw;
+    const int w = threadIdx.x >> 5, left = halves - 2 * kSW * s;
+    return left >= 2 * kSW || w < left - kSW;
   }
   MOE_DEV void next_step() {
     if (++ls == steps) {
       ls = 0;
-      lb += RT * groups;
+      lb += RT;
       if (lb < tiles) load_round();
     }
   }
 
   MOE_DEV void prologue(int n_tiles) {
     halves = (src.length() + 31) / 32;
-    kw = plan_warps<RT>(n_tiles, halves);
-    groups = kSW / kw;
-    const int w = (threadIdx.x >> 5) & (kw - 1), full = halves >> __ffs(kw);
-    steps = full + (halves - 2 * kw * full > w ? 1 : 0);
+    const int w = threadIdx.x >> 5, full = halves / (2 * kSW);
+    steps = full + (halves - 2 * kSW * full > w ? 1 : 0);
     tiles = n_tiles;
-    lb = (threadIdx.x >> 5) >> (__ffs(kw) - 1);
-    ls = 0;
-    if (steps == 0 || lb >= tiles) return;
+    lb = ls = 0;
+    if (steps == 0 || tiles == 0) return;
     load_round();
 #pragma unroll
     for (int p = 0; p < PD; ++p) {
@@ -210,8 +189,17 @@ struct Streamer {
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
     const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
     int turn = 0;
-    const int round = RT * groups, shift = __ffs(groups) - 1;
-    for (int base = 0; base < tiles; base += round) {
+    uint4 first[NT][2];
+    const auto fetch = [&](int s, uint4 (&x)[NT][2]) {
+      const int k = 32 * half_at(s);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        src.tokens(k, j, x[j][0], x[j][1]);
+        if (!both(s)) x[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
+      }
+    };
+    if (steps > 0) fetch(0, first);
+    for (int base = 0; base < tiles; base += RT) {
       float acc[RT][NT][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -220,25 +208,20 @@ struct Streamer {
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
       uint4 next[NT][2];
-      auto fetch = [&](int s) {
-        const int k = 32 * half_at(s);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          src.tokens(k, j, next[j][0], next[j][1]);
-          if (!both(s)) next[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
-        }
-      };
-      const int mine = base + (warp >> (4 - shift)) < tiles ? steps : 0;  // a group without a tile in the last round
-      if (mine > 0) fetch(0);
+      for (int j = 0; j < NT; ++j) {
+        next[j][0] = first[j][0];
+        next[j][1] = first[j][1];
+      }
 #pragma unroll 1
-      for (int s = 0; s < mine; ++s) {
+      for (int s = 0; s < steps; ++s) {
         uint4 x[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           x[j][0] = next[j][0];
           x[j][1] = next[j][1];
         }
-        if (s + 1 < mine) fetch(s + 1);
+        if (s + 1 < steps) fetch(s + 1, next);
         const At at = at_step(ls);
         // Two slots at a time where there are two: their reads and mma chains overlap,
         // and one pair of warp barriers serves both.
@@ -275,12 +258,12 @@ struct Streamer {
         next_step();
         turn = turn + 1 == PD ? 0 : turn + 1;
       }
-      const int nt = min(round, tiles - base);
-      if (base + round >= tiles) ahead();
+      const int nt = min(RT, tiles - base);
+      if (base + RT >= tiles) ahead();
       if (base > 0) __syncthreads();  // the last round's partials have been added
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        if (i * groups < nt) {
+        if (i < nt) {
           float* p = part + (i * kSW + warp) * (NT * kPartTile) + 2 * t4 * kPartCol + g;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -293,16 +276,15 @@ struct Streamer {
         }
       }
       __syncthreads();
-      // o = (tile, column, row); o / cols by a 16-bit reciprocal, exact while (o / FROWS) cols < 2^16 (at most 32 x 32 x 32)
+      // o = (tile, column, row); o / cols by a 16-bit reciprocal, exact while (o / FROWS) cols < 2^16 (at most 4 x 32 x 32)
       const uint32_t inverse = 65536u / static_cast<uint32_t>(cols) + 1u;
       for (int o = threadIdx.x; o < nt * cols * FROWS; o += kSThreads) {
         const int oc = o / FROWS, row = o % FROWS, tl = static_cast<int>((oc * inverse) >> 16), col = oc - tl * cols;
         fin(base + tl, row, col, [&](int r, int c) {
-          // tile tl of the round: the (tl / groups)-th of group tl % groups
-          const float* p = part + (((tl >> shift) << 4) + ((tl & (groups - 1)) << (4 - shift))) * (NT * kPartTile) +
-                           (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
+          const float* p = part + tl * kSW * (NT * kPartTile) + (c >> 3) * kPartTile + (c & 7) * kPartCol + r;
           float v = 0.0f;
-          for (int w = 0; w < kw; w += 2) v += p[w * (NT * kPartTile)] + p[(w + 1) * (NT * kPartTile)];
+#pragma unroll
+          for (int w = 0; w < kSW; ++w) v += p[w * (NT * kPartTile)];
           return v;
         });
       }
