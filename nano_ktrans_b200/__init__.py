@@ -26,23 +26,20 @@ __all__ = [
 ]
 
 
+_MODULES = {
+    "CudaMoEBackend": "cuda_moe", "HybridMoE": "hybrid_moe", "MoeLayer": "moe_layer",
+    "EpMoeLayer": "expert_parallel", "plan_placement": "expert_parallel", "shard_layer": "expert_parallel",
+    "TorchDistComm": "expert_parallel", "PeerExchange": "expert_parallel",
+    "linear": "dense", "gated_linear": "dense", "DenseMLP": "dense", "DenseMoeLayer": "dense_moe",
+}
+
+
 def __getattr__(name):
-    if name == "CudaMoEBackend":
-        from .cuda_moe import CudaMoEBackend
-        return CudaMoEBackend
-    if name == "HybridMoE":
-        from .hybrid_moe import HybridMoE
-        return HybridMoE
-    if name == "MoeLayer":
-        from .moe_layer import MoeLayer
-        return MoeLayer
-    if name in ("EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange"):
-        from . import expert_parallel
-        return getattr(expert_parallel, name)
-    if name in ("linear", "gated_linear", "DenseMLP"):
-        from . import dense
-        return getattr(dense, name)
-    if name == "DenseMoeLayer":
-        from .dense_moe import DenseMoeLayer
-        return DenseMoeLayer
-    raise AttributeError(name)
+    module = _MODULES.get(name)
+    if module is None:
+        raise AttributeError(name)
+    from importlib import import_module
+
+    # kept as a plain attribute: the next use is not looked up again
+    value = globals()[name] = getattr(import_module("." + module, __name__), name)
+    return value

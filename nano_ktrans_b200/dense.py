@@ -22,6 +22,19 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _tls = threading.local()
+_Desc = _lib.MoeLinearDesc
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_entry = None
+
+
+def _moe_linear():
+    """The library's entry point, looked up once."""
+    global _entry
+    if _entry is None:
+        _entry = _lib.lib().moe_linear
+    return _entry
+
+
 
 
 def _err_buffer():
@@ -48,52 +61,64 @@ def _empty_on(shape, dtype, device, stream) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _matrix(t: torch.Tensor, name: str, rows: Optional[int], cols: int, like: torch.Tensor) -> int:
-    """Row stride of a [rows, cols] tensor after its checks."""
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
-    if t.dtype is not like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+def _row_stride(t: torch.Tensor, name: str, rows: Optional[int], cols: int, dtype, dev: int) -> int:
+    """Row stride of a [rows, cols] tensor after its checks.  The first test is the usual case in as few attribute
+    reads as it takes: these checks are most of what a small call costs on the host."""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == cols and shape[0] == rows and t.dtype is dtype and t.get_device() == dev \
+            and t.is_contiguous():
+        return cols
+    if t.dim() != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {tuple(shape)}")
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be {dtype} on cuda:{dev}, got {t.dtype} on {t.device}")
     ld, inner = t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name} must have unit stride along its rows")
-    return ld if t.shape[0] > 1 else cols
+    return ld if shape[0] > 1 else cols
 
 
 def _project(x, weight, up, bias, activation, residual, out, stream) -> torch.Tensor:
-    dtype = _DTYPES.get(x.dtype)
-    if dtype is None or not x.is_cuda or x.dim() != 2:
-        raise ValueError(f"x must be a bf16 or fp16 [m, k] CUDA tensor, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    dtype = x.dtype
+    code = _DTYPES.get(dtype)
+    if code is None or not x.is_cuda or x.dim() != 2 or weight.dim() != 2:
+        raise ValueError(f"x must be a bf16 or fp16 [m, k] CUDA tensor and the weight [n, k], got {x.dtype} "
+                         f"{tuple(x.shape)} on {x.device} and {tuple(weight.shape)}")
     act = _lib.ACTIVATIONS.get(activation, -1)
     if act < 0:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(k for k in _lib.ACTIVATIONS if k)}")
+    dev = x.get_device()
     m, k = x.shape
-    ldx = _matrix(x, "x", m, k, x)
-    ldw = _matrix(weight, "weight" if up is None else "gate_weight", None, k, x)
     n = weight.shape[0]
+    ldx = _row_stride(x, "x", m, k, dtype, dev)
+    ldw = _row_stride(weight, "weight" if up is None else "gate_weight", n, k, dtype, dev)
     if n < 1 or k < 1:
         raise ValueError(f"empty weight {tuple(weight.shape)}")
-    ldu = 0 if up is None else _matrix(up, "up_weight", n, k, x)
-    if bias is not None and (bias.shape != (n,) or bias.dtype is not x.dtype or bias.device != x.device
-                             or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous {x.dtype} [{n}] tensor on {x.device}")
-    ldr = 0 if residual is None else _matrix(residual, "residual", m, n, x)
+    up_ptr = bias_ptr = res_ptr = None
+    ldu = ldr = 0
+    if up is not None:
+        ldu, up_ptr = _row_stride(up, "up_weight", n, k, dtype, dev), up.data_ptr()
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype is not dtype or bias.get_device() != dev or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous {dtype} [{n}] tensor on {x.device}")
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        ldr, res_ptr = _row_stride(residual, "residual", m, n, dtype, dev), residual.data_ptr()
     if out is None:
-        out = _empty_on((m, n), x.dtype, x.device, stream)
-    ldo = _matrix(out, "out", m, n, x)
+        out = _empty_on((m, n), dtype, x.device, stream)
+        ldo = n
+    else:
+        ldo = _row_stride(out, "out", m, n, dtype, dev)
     if m == 0:
         return out
-    dev = x.get_device()
-    desc = _lib.MoeLinearDesc(x.data_ptr(), weight.data_ptr(), None if up is None else up.data_ptr(),
-                              None if bias is None else bias.data_ptr(),
-                              None if residual is None else residual.data_ptr(), out.data_ptr(),
-                              ldx, ldw, ldu, ldr, ldo, m, n, k, dtype, act)
+    desc = _Desc(x.data_ptr(), weight.data_ptr(), up_ptr, bias_ptr, res_ptr, out.data_ptr(), ldx, ldw, ldu, ldr, ldo,
+                 m, n, k, code, act)
     err = _err_buffer()
-    if dev == torch.cuda.current_device():
-        rc = _lib.lib().moe_linear(ctypes.byref(desc), _stream_on(dev, stream), err, 512)
+    if dev == torch._C._cuda_getDevice():
+        rc = _moe_linear()(desc, _raw_stream(dev) if stream is None else _stream_on(dev, stream), err, 512)
     else:
         with torch.cuda.device(dev):
-            rc = _lib.lib().moe_linear(ctypes.byref(desc), _stream_on(dev, stream), err, 512)
+            rc = _moe_linear()(desc, _stream_on(dev, stream), err, 512)
     if rc != _lib.MOE_OK:
         raise _lib.MoeError(rc, err.value.decode(errors="replace"))
     return out

@@ -121,7 +121,7 @@ class DenseMoeLayer:
             ws = _empty_on(n, torch.uint8, self.device, stream)
             d.workspace_dev = ws.data_ptr()
         err = _err_buffer()
-        if self._dev == torch.cuda.current_device():
+        if self._dev == torch._C._cuda_getDevice():
             rc = _lib.lib().moe_dense_forward(ctypes.byref(d), _stream_on(self._dev, stream), err, 512)
         else:
             with torch.cuda.device(self._dev):
