@@ -73,8 +73,11 @@ MOE_DEV uint32_t map_rank(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+MOE_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+MOE_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 MOE_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 MOE_DEV void st_cluster(uint32_t addr, float x, float y, float z, float w) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
@@ -160,6 +163,28 @@ MOE_DEV void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// N groups of 8 columns, `apart` columns from one to the next, in one round trip.
+template <int N>
+MOE_DEV void tmem_ld8_all(uint32_t taddr, int apart, float (&v)[N][8]) {
+  uint32_t r[N][8];
+#pragma unroll
+  for (int g = 0; g < N; ++g)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[g][0]), "=r"(r[g][1]), "=r"(r[g][2]), "=r"(r[g][3]), "=r"(r[g][4]), "=r"(r[g][5]), "=r"(r[g][6]),
+                   "=r"(r[g][7])
+                 : "r"(taddr + g * apart));
+  // the registers pass through the wait, so that nothing uses them before it
+#pragma unroll
+  for (int g = 0; g < N; ++g)
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[g][0]), "+r"(r[g][1]), "+r"(r[g][2]), "+r"(r[g][3]), "+r"(r[g][4]), "+r"(r[g][5]), "+r"(r[g][6]),
+                   "+r"(r[g][7])::"memory");
+#pragma unroll
+  for (int g = 0; g < N; ++g)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[g][i] = __uint_as_float(r[g][i]);
 }
 
 template <int N>
@@ -525,6 +550,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_s;
+  if (p.splits > 1) cluster_arrive();  // this block runs: its shared memory may be written (waited for before the exchange)
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // One thread walks the stages in each role, so what it does per step is paid in
@@ -634,30 +660,52 @@ __global__ void __launch_bounds__(kQThreads, 1)
   if (p.splits > 1) {
     // Chunk c belongs to block c % splits of the cluster.  Every block sends its
     // partial sums of a chunk to the owner's shared memory, [sender][chunk]
-    // [4 columns][row], once all blocks are past their MMAs; the owner adds them
-    // in sender order.
+    // [4 columns][row], beside the owner's stages; the owner adds them in sender
+    // order.
     constexpr int kSub = GATED ? 4 : 2;  // quads of columns of a chunk
-    const int own = (chunks + p.splits - 1) / p.splits, quad_bytes = valid * 16;
-    __syncthreads();
-    cluster_sync();
+    const int log = __ffs(p.splits) - 1, own = (chunks + p.splits - 1) >> log, quad_bytes = valid * 16;
+    unsigned char* exchange = smem + p.stages * stage_bytes;
+    __syncwarp();
+    cluster_wait();
     if (warp >= 2 && !*aborted) {
       fence_after();
-      const uint32_t mine = smem_u32(smem) + static_cast<uint32_t>(rank * own * kSub * quad_bytes);
+      const uint32_t mine = smem_u32(exchange) + static_cast<uint32_t>(rank * own * kSub * quad_bytes);
+      constexpr int kAtOnce = GATED ? 2 : 4;  // chunks read from tensor memory in one round trip
       for (int r = 0; r < row_tiles; ++r) {
         const int row = r * 128 + q * 32 + lane;
         if (r * 128 + q * 32 >= valid) continue;  // warp-uniform
-        for (int c = half; c < chunks; c += 2) {
-          const uint32_t at = tmem + r * cols + 8 * c + (static_cast<uint32_t>(q * 32) << 16);
-          float v[8], u[8];
-          tmem_ld8(at, v);
-          if constexpr (GATED) tmem_ld8(at + p.width, u);
+        for (int c0 = half; c0 < chunks; c0 += 2 * kAtOnce) {
+          // chunks past the last one are padding of the tile: read and not sent
+          const int last = (cols - 8) / 8;
+          const uint32_t at = tmem + r * cols + (static_cast<uint32_t>(q * 32) << 16);
+          float v[kAtOnce][8], u[kAtOnce][8];
+          if (c0 + 2 * (kAtOnce - 1) <= (GATED ? p.width / 8 - 1 : last)) {
+            tmem_ld8_all<kAtOnce>(at + 8 * c0, 16, v);
+            if constexpr (GATED) tmem_ld8_all<kAtOnce>(at + p.width + 8 * c0, 16, u);
+          } else {
+            for (int g = 0; g < kAtOnce; ++g) {
+              const int c = min(c0 + 2 * g, chunks - 1);
+#pragma unroll
+              for (int h = 0; h < kAtOnce; ++h)
+                if (h == g) {
+                  tmem_ld8(at + 8 * c, v[h]);
+                  if constexpr (GATED) tmem_ld8(at + p.width + 8 * c, u[h]);
+                }
+            }
+          }
           if (row < valid) {
-            const uint32_t to = map_rank(mine + (c / p.splits) * kSub * quad_bytes + row * 16, c % p.splits);
-            st_cluster(to, v[0], v[1], v[2], v[3]);
-            st_cluster(to + quad_bytes, v[4], v[5], v[6], v[7]);
-            if constexpr (GATED) {
-              st_cluster(to + 2 * quad_bytes, u[0], u[1], u[2], u[3]);
-              st_cluster(to + 3 * quad_bytes, u[4], u[5], u[6], u[7]);
+#pragma unroll
+            for (int g = 0; g < kAtOnce; ++g) {
+              const int c = c0 + 2 * g;
+              if (c < chunks) {
+                const uint32_t to = map_rank(mine + (c >> log) * kSub * quad_bytes + row * 16, c & (p.splits - 1));
+                st_cluster(to, v[g][0], v[g][1], v[g][2], v[g][3]);
+                st_cluster(to + quad_bytes, v[g][4], v[g][5], v[g][6], v[g][7]);
+                if constexpr (GATED) {
+                  st_cluster(to + 2 * quad_bytes, u[g][0], u[g][1], u[g][2], u[g][3]);
+                  st_cluster(to + 3 * quad_bytes, u[g][4], u[g][5], u[g][6], u[g][7]);
+                }
+              }
             }
           }
         }
@@ -683,7 +731,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
         if (row >= valid) continue;
         float v[8] = {}, u[8] = {};
         for (int s = 0; s < p.splits; ++s) {
-          const unsigned char* from = smem + static_cast<size_t>((s * own + slot) * kSub) * quad_bytes + row * 16;
+          const unsigned char* from = exchange + static_cast<size_t>((s * own + slot) * kSub) * quad_bytes + row * 16;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 f = *reinterpret_cast<const float4*>(from + h * quad_bytes);
@@ -776,17 +824,16 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
         const int cols = width * mul;
         if (cols > 256 || rows / 128 * cols > 512) continue;
         const int stage = (box + cols) * 128;
-        int stages = static_cast<int>((kSmemLimit - 2048 - kQTail) / stage);
-        if (stages > 16) stages = 16;
-        if (stages < 2) continue;
-        // partial sums that a block receives: its chunks of 8 columns from every block
+        const int steps = (nk + splits - 1) / splits, real_waves = (slices * mg * splits + cap - 1) / cap;
+        // partial sums that a block receives, beside its stages: its chunks of 8 columns from every block
         const int valid = a.m < rows ? a.m : rows, own = ((width + 7) / 8 + splits - 1) / splits;
         const int64_t part = splits > 1 ? 32LL * mul * valid * own * splits : 0;
-        int64_t smem = static_cast<int64_t>(stages) * stage;
-        if (part > smem) smem = part;
-        smem += kQTail;
-        if (smem > static_cast<int64_t>(kSmemLimit) - 2048) continue;
-        const int steps = (nk + splits - 1) / splits, real_waves = (slices * mg * splits + cap - 1) / cap;
+        const int64_t room = static_cast<int64_t>(kSmemLimit) - 2048 - kQTail - part;
+        int stages = room > 0 ? static_cast<int>(room / stage) : 0;
+        if (stages > 16) stages = 16;
+        if (stages > steps) stages = steps;
+        if (stages < steps && stages < 3) continue;
+        const int64_t smem = static_cast<int64_t>(stages) * stage + part + kQTail;
         const double load = stage / 50.0, mma = 2.0 * cols * (box > 128 ? 2 : 1);
         const double items = (valid + 31) / 32 * ((width + 7) / 8) * mul / 8.0;  // 32 rows x 8 columns a warp
         const double join = splits > 1 ? 2500.0 + 90.0 * items + 60.0 * items : 110.0 * items;
