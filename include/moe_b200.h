@@ -445,7 +445,8 @@ int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_
  * ids_out_dev / weights_out_dev (may be NULL) receive the routing in the first
  * two forms.
  * 0 <= num_tokens <= MOE_DENSE_MAX_TOKENS (above: MOE_ERANGE), num_experts in
- * [1, 1024], top_k in [1, min(16, num_experts)], hidden and inter multiples of
+ * [1, 1024], top_k in [1, 16] (at most num_experts unless the routing is
+ * given), hidden, inter and shared_inter at most 65536 and multiples of
  * 16, x rows and all weights on 16-byte boundaries.  out may be x or residual
  * itself, and overlaps nothing else.
  * workspace_dev: moe_dense_workspace bytes, 256-byte aligned, for this call
@@ -483,8 +484,9 @@ typedef struct moe_dense_desc {
 } moe_dense_desc;
 int moe_dense_workspace(const moe_dense_desc* desc, int64_t* bytes, char* err, size_t err_len);
 int moe_dense_forward(const moe_dense_desc* desc, void* stream, char* err, size_t err_len);
-/* Copy the current device's status word of the dense calls (bits as
- * moe_read_status) to *status and clear it; synchronises `stream`. */
+/* Copy the current device's status word of the dense calls (moe_linear and
+ * moe_dense_forward; bits as moe_read_status) to *status and clear it;
+ * synchronises `stream`. */
 int moe_dense_read_status(int32_t* status, void* stream, char* err, size_t err_len);
 
 #ifdef __cplusplus

@@ -22,7 +22,7 @@ __all__ = [
     "ExpertOffloadBackend", "normalize_offload_backend_name", "GPTQLinearWeight", "LayerWeights",
     "quantize_symmetric", "stack_layer", "CudaMoEBackend", "HybridMoE", "MoeLayer",
     "EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange",
-    "linear", "gated_linear", "DenseMLP", "DenseMoeLayer",
+    "linear", "gated_linear", "DenseMLP", "DenseMoeLayer", "stack_expert_modules",
 ]
 
 
@@ -31,6 +31,7 @@ _MODULES = {
     "EpMoeLayer": "expert_parallel", "plan_placement": "expert_parallel", "shard_layer": "expert_parallel",
     "TorchDistComm": "expert_parallel", "PeerExchange": "expert_parallel",
     "linear": "dense", "gated_linear": "dense", "DenseMLP": "dense", "DenseMoeLayer": "dense_moe",
+    "stack_expert_modules": "dense_moe",
 }
 
 

@@ -138,8 +138,7 @@ MoeSpace moe_space(const moe_dense_desc& d, int sms) {
 const char* check_layer(const moe_dense_desc& d) {
   if (d.dtype != MOE_DTYPE_BF16 && d.dtype != MOE_DTYPE_FP16) return "dtype must be MOE_DTYPE_BF16 or MOE_DTYPE_FP16";
   if (d.num_experts < 1 || d.num_experts > moe::dense::kMoeExperts) return "num_experts must be in [1, 1024]";
-  if (d.top_k < 1 || d.top_k > moe::dense::kMoeTopK || d.top_k > d.num_experts)
-    return "top_k must be in [1, min(16, num_experts)]";
+  if (d.top_k < 1 || d.top_k > moe::dense::kMoeTopK) return "top_k must be in [1, 16]";
   const int32_t big = 1 << 16;
   if (d.hidden_size < 16 || d.hidden_size % 16 || d.hidden_size > big) return "hidden_size must be a positive multiple of 16";
   if (d.inter_size < 16 || d.inter_size % 16 || d.inter_size > big) return "inter_size must be a positive multiple of 16";
@@ -180,6 +179,7 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
     return refuse(err, err_len, MOE_EINVAL, "%s: given routing needs ids and weights, and no router or logits", me);
   if (!given && d->router_w_dev == nullptr && d->logits_dev == nullptr)
     return refuse(err, err_len, MOE_EINVAL, "%s: no routing: router weights, logits or ids", me);
+  if (!given && d->top_k > E) return refuse(err, err_len, MOE_EINVAL, "%s: top_k above num_experts", me);
   if (given && (d->ids_out_dev || d->weights_out_dev))
     return refuse(err, err_len, MOE_EINVAL, "%s: given routing is not written out again", me);
   const void* wide[] = {d->gate_dev, d->up_dev, d->down_dev, d->x_dev, d->router_w_dev,

@@ -21,6 +21,30 @@ from .dense import _DTYPES, _empty_on, _err_buffer, _stream_on
 MAX_TOKENS = _lib.DENSE_MAX_TOKENS
 
 
+# Attribute names of an expert's gate, up and down projection: the reference's SparseExpertMLP
+# (nano_ktrans/layers/expert_mlp.py:9-23), and the checkpoints' own.
+_PROJECTIONS = (("w1", "w3", "w2"), ("gate_proj", "up_proj", "down_proj"))
+
+
+def stack_expert_modules(modules) -> tuple:
+    """``(gate [E, I, H], up [E, I, H], down [E, H, I])`` of expert modules with ``w1`` / ``w3`` / ``w2`` (or
+    ``gate_proj`` / ``up_proj`` / ``down_proj``) linear layers without bias.  The modules' parameters are made views of
+    the stacks, so the weights are held once."""
+    parts = []
+    for m in modules:
+        names = next((n for n in _PROJECTIONS if all(hasattr(m, a) for a in n)), None)
+        if names is None or any(getattr(getattr(m, a), "bias", None) is not None for a in names):
+            raise ValueError(f"{type(m).__name__} is not a gated expert of three linear layers without bias")
+        parts.append([getattr(m, a) for a in names])
+    if not parts:
+        raise ValueError("no expert modules")
+    stacks = tuple(torch.stack([p[j].weight.detach() for p in parts]).contiguous() for j in range(3))
+    for e, p in enumerate(parts):
+        for j in range(3):
+            p[j].weight.data = stacks[j][e]
+    return stacks
+
+
 class DenseMoeLayer:
     """``gate`` / ``up`` [E, I, H], ``down`` [E, H, I] (bf16 or fp16, contiguous, on one CUDA device; H and I
     multiples of 16); ``shared``: ``{"gate", "up": [S, H], "down": [H, S], "gate_vec": [H]}`` or None."""
@@ -57,13 +81,14 @@ class DenseMoeLayer:
                                        int(self.normalize_topk_prob), _DTYPES[gate.dtype])
         self._space = []  # workspace bytes by token count
         err = _err_buffer()
-        for t in range(MAX_TOKENS + 1):
-            self._desc.num_tokens = t
-            n = ctypes.c_int64(0)
-            rc = _lib.lib().moe_dense_workspace(ctypes.byref(self._desc), ctypes.byref(n), err, 512)
-            if rc != _lib.MOE_OK:
-                raise _lib.MoeError(rc, err.value.decode(errors="replace"))
-            self._space.append(n.value)
+        with torch.cuda.device(self._dev):  # the workspace goes by the device's SMs
+            for t in range(MAX_TOKENS + 1):
+                self._desc.num_tokens = t
+                n = ctypes.c_int64(0)
+                rc = _lib.lib().moe_dense_workspace(ctypes.byref(self._desc), ctypes.byref(n), err, 512)
+                if rc != _lib.MOE_OK:
+                    raise _lib.MoeError(rc, err.value.decode(errors="replace"))
+                self._space.append(n.value)
         self._layer_bytes = bytes(self._desc)
 
     # ------------------------------------------------------------------

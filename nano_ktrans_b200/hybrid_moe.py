@@ -5,7 +5,7 @@ router_logits)`` contract (nano_ktrans/layers/hybrid_moe.py:54-290,
 :3310-3570).  Routing semantics are the reference's (:3321-3329), computed by
 the router kernel; the offloaded experts go through the backend's
 ``submit_forward`` / ``sync_forward`` (:3373-3378, :3563-3567); experts marked
-GPU-resident in ``gpu_experts_mask`` are served one of two ways, chosen by
+GPU-resident in ``gpu_experts_mask`` are served one of three ways, chosen by
 ``resident_experts``:
 
 * ``"kernels"`` (default): by the same kernels, from the backend's quantized
@@ -15,7 +15,11 @@ GPU-resident in ``gpu_experts_mask`` are served one of two ways, chosen by
   the weights, not how the output is computed;
 * ``"modules"``: as dense ``nn.Module``s in the reference's per-expert loop
   (:3501-3533, with its host reads of the routed ids), summed with the
-  backend's part (:3570) — bit-for-bit the reference's split semantics.
+  backend's part (:3570) — bit-for-bit the reference's split semantics;
+* ``"dense"``: the modules' bf16 weights stacked once (the modules keep views of
+  them) and run by ``DenseMoeLayer`` — for up to 16 tokens all resident experts,
+  the weighted sum and the addition of the backend's part are two launches
+  without a host read and one rounding; larger batches take the ``"modules"`` loop.
 
 The reference's residency machinery (migration queues, prefetch caches,
 schedulers; hybrid_moe.py:109-254, :2841-3300) is not part of this path; its
@@ -30,6 +34,8 @@ import torch
 from torch import nn
 
 from .cuda_moe import CudaMoEBackend
+from .dense_moe import MAX_TOKENS as DENSE_MAX_TOKENS
+from .dense_moe import DenseMoeLayer, stack_expert_modules
 from .offload_backend import normalize_offload_backend_name
 
 
@@ -70,14 +76,14 @@ class HybridMoE(nn.Module):
         self.normalize_topk_prob = normalize_topk_prob
         self.experts_are_packed = experts_are_packed
         self.hidden_act = hidden_act
-        if resident_experts not in ("kernels", "modules"):
-            raise ValueError("resident_experts must be 'kernels' or 'modules'")
+        if resident_experts not in ("kernels", "modules", "dense"):
+            raise ValueError("resident_experts must be 'kernels', 'modules' or 'dense'")
         self.resident_experts = resident_experts
         self.has_cpu_experts = bool((~gpu_experts_mask.bool()).any().item())
         self.offload_backend_name = normalize_offload_backend_name(offload_backend)
         if self.offload_backend_name != "cuda":
             raise NotImplementedError(f"this package provides the 'cuda' backend, not '{self.offload_backend_name}'")
-        if not self.has_cpu_experts and resident_experts == "modules":
+        if not self.has_cpu_experts and resident_experts != "kernels":
             raise ValueError("every expert is GPU-resident: there is no routed-expert work for the cuda backend")
         kwargs = dict(layer_idx=layer_idx, num_experts=num_experts, top_k=top_k, hidden_size=hidden_size,
                       intermediate_size=moe_intermediate_size, gpu_experts_mask=gpu_experts_mask,
@@ -87,6 +93,16 @@ class HybridMoE(nn.Module):
                       router_use_softmax=router_use_softmax, normalize_topk_prob=normalize_topk_prob)
         kwargs.update(offload_backend_kwargs or {})
         self.offload_backend = CudaMoEBackend(**kwargs)
+        self._dense: Optional[DenseMoeLayer] = None
+        self._dense_slot: Optional[torch.Tensor] = None  # expert -> its place in the stack, -1: not resident
+        resident = [e for e in range(num_experts) if bool(gpu_experts_mask[e]) and str(e) in gpu_experts]
+        if resident_experts == "dense" and resident:
+            device = self.offload_backend.device
+            stacks = [w.to(device) for w in stack_expert_modules([gpu_experts[str(e)] for e in resident])]
+            self._dense = DenseMoeLayer(*stacks, top_k=top_k)
+            slot = torch.full((num_experts,), -1, dtype=torch.int64)
+            slot[resident] = torch.arange(len(resident))
+            self._dense_slot = slot.to(device)
         self.last_topk_ids: Optional[torch.Tensor] = None
         self.last_topk_weights: Optional[torch.Tensor] = None
 
@@ -106,6 +122,10 @@ class HybridMoE(nn.Module):
         self.last_topk_ids, self.last_topk_weights = topk_ids, topk_weights
         stream = torch.cuda.current_stream(hidden_states.device).cuda_stream
         self.offload_backend.submit_forward(hidden_states, topk_ids, topk_weights, stream)
+
+        if self._dense is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
+            offloaded = self.offload_backend.sync_forward(hidden_states, stream)
+            return self._dense.experts_forward(hidden_states, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
 
         final_gpu_states = torch.zeros_like(hidden_states)
         mask_host = self.gpu_experts_mask.bool().cpu().tolist()

@@ -138,3 +138,30 @@ def test_dense_moe_layer_refuses_host_weights():
         DenseMoeLayer(g, g, d, top_k=2)
     with pytest.raises(ValueError, match="gate and up"):
         DenseMoeLayer(g, d, d, top_k=2)
+
+
+def test_stack_expert_modules():
+    """The stacks hold the modules' weights and the modules keep views of them."""
+    from nano_ktrans_b200 import stack_expert_modules
+
+    class Expert(torch.nn.Module):
+        def __init__(self, names, bias=False):
+            super().__init__()
+            for n, (o, i) in zip(names, [(3, 4), (3, 4), (4, 3)]):
+                setattr(self, n, torch.nn.Linear(i, o, bias=bias))
+
+    mods = [Expert(("w1", "w3", "w2")), Expert(("gate_proj", "up_proj", "down_proj"))]
+    want = [[getattr(m, n).weight.detach().clone() for n in names]
+            for m, names in zip(mods, (("w1", "w3", "w2"), ("gate_proj", "up_proj", "down_proj")))]
+    gate, up, down = stack_expert_modules(mods)
+    for e in range(2):
+        for stack, w in zip((gate, up, down), want[e]):
+            assert torch.equal(stack[e], w)
+    down[1].mul_(2)
+    assert torch.equal(mods[1].down_proj.weight, want[1][2] * 2)
+    with pytest.raises(ValueError, match="without bias"):
+        stack_expert_modules([Expert(("w1", "w3", "w2"), bias=True)])
+    with pytest.raises(ValueError, match="gated expert"):
+        stack_expert_modules([torch.nn.Linear(2, 2)])
+    with pytest.raises(ValueError, match="no expert"):
+        stack_expert_modules([])

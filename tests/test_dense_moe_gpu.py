@@ -237,6 +237,76 @@ def test_no_tokens_and_refusals(cuda_device):
     with pytest.raises(ValueError, match="contiguous"):
         DenseMoeLayer(g, u, g.transpose(1, 2), top_k=2)
     with pytest.raises(MoeError, match="top_k"):
-        DenseMoeLayer(g, u, d, top_k=9)
+        DenseMoeLayer(g, u, d, top_k=17)
+    with pytest.raises(MoeError, match="top_k"):
+        DenseMoeLayer(g, u, d, top_k=9).forward_x(x, wr)
     with pytest.raises(MoeError, match="inter_size"):
         DenseMoeLayer(g[:, :24].contiguous(), u[:, :24].contiguous(), d[:, :, :24].contiguous(), top_k=2)
+
+
+class Expert(torch.nn.Module):
+    """The reference's expert: w2(silu(w1 x) * w3 x)."""
+
+    def __init__(self, gate, up, down):
+        super().__init__()
+        for name, w in (("w1", gate), ("w3", up), ("w2", down)):
+            lin = torch.nn.Linear(w.shape[1], w.shape[0], bias=False, device=w.device, dtype=w.dtype)
+            lin.weight.data.copy_(w)
+            setattr(self, name, lin)
+
+    def forward(self, x):
+        return self.w2(torch.nn.functional.silu(self.w1(x)) * self.w3(x))
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 16, 40])
+@pytest.mark.parametrize("resident", [2, 9])
+def test_hybrid_moe_with_dense_resident_experts(tokens, resident, cuda_device):
+    """Resident experts from their bf16 modules and the others from their codes, in one forward: the dense path against
+    the 64-bit form over the backend's own part, without a host sync; above its token limit the module loop."""
+    from nano_ktrans_b200.hybrid_moe import HybridMoE
+    from tests import helpers as hp
+
+    e, k, h, i = 16, 4, 256, 128
+    lw = hp.device_layer({n: hp.make_expert(5, n, h, i, 4, 128) for n in range(e)}, e, h, i, 4, 128, cuda_device)
+    on = list(range(1, 1 + resident))
+    mods = torch.nn.ModuleDict()
+    for n in on:
+        mods[str(n)] = Expert(*(rnd(cuda_device, 100 + 3 * n + j, *s, scale=0.05) for j, s in enumerate([(i, h), (i, h), (h, i)])))
+    mask = torch.zeros(e, dtype=torch.bool)
+    mask[on] = True
+    kw = dict(num_experts=e, top_k=k, hidden_size=h, moe_intermediate_size=i, gpu_experts=mods, gpu_experts_mask=mask,
+              layer_idx=0, weight_path="", router_use_softmax=True, normalize_topk_prob=True,
+              offload_backend_kwargs={"device": cuda_device, "max_tokens": 64, "layer_weights": lw})
+    before = [mods[str(n)].w2.weight.clone() for n in on]
+    moe, loop = HybridMoE(resident_experts="dense", **kw), HybridMoE(resident_experts="modules", **kw)
+    for n, w in zip(on, before):
+        assert torch.equal(mods[str(n)].w2.weight, w), "stacking changed a module's weights"
+    assert mods[str(on[0])].w1.weight.data_ptr() == moe._dense.gate.data_ptr()
+    x, lg = rnd(cuda_device, 1, tokens, h), rnd(cuda_device, 2, tokens, e)
+    want = loop(x, lg)
+    moe(x, lg)
+    torch.cuda.synchronize()
+    if tokens <= 16:
+        torch.cuda.set_sync_debug_mode("error")
+    try:
+        out = moe(x, lg)
+    finally:
+        torch.cuda.set_sync_debug_mode(0)
+    if tokens > 16:
+        assert torch.equal(out, want)
+        return
+    assert torch.equal(moe.last_topk_ids, loop.last_topk_ids)
+    offloaded = moe.offload_backend.layer.experts_forward(x, moe.last_topk_ids, moe.last_topk_weights, offload_mask=~mask)
+    slots = moe._dense_slot[moe.last_topk_ids]
+    d = moe._dense
+    dr.assert_within(out, dr.moe64(x, slots, moe.last_topk_weights, d.gate, d.up, d.down, None, offloaded))
+    assert d.read_status() == 0
+
+
+def test_given_routing_on_fewer_experts_than_picks(cuda_device):
+    """Two stacked experts under a top-8 routing, as when two of a layer's experts are resident."""
+    layer, _ = make(cuda_device, 2, 8, 128, 64)
+    x, w = rnd(cuda_device, 1, 3, 128), torch.rand(3, 8, device=cuda_device).to(BF16)
+    ids = torch.full((3, 8), -1, device=cuda_device)
+    ids[0, 5], ids[2, 0], ids[2, 7] = 1, 1, 0
+    check(layer, None, layer.experts_forward(x, ids, w), x, ids, w)
