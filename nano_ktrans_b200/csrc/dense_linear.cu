@@ -137,10 +137,10 @@ struct LinearSrc {
       }
     }
   }
-  MOE_DEV void tokens(int k, int j, uint4& x0, uint4& x1) const {
+  MOE_DEV void tokens(int k, bool two, int j, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
     x0 = xrow[j] != nullptr && k + t8 < a.k ? ld_tokens(xrow[j] + k) : z;
-    x1 = xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
+    x1 = two && xrow[j] != nullptr && k + 32 + t8 < a.k ? ld_tokens(xrow[j] + k + 32) : z;
   }
 };
 

@@ -247,10 +247,10 @@ struct GateUpSrc {
     p[3] = p[2] + 4 * a.hidden;
     valid = 15u;
   }
-  MOE_DEV void tokens(int k, int, uint4& x0, uint4& x1) const {
+  MOE_DEV void tokens(int k, bool two, int, uint4& x0, uint4& x1) const {
     const uint4 z = make_uint4(0, 0, 0, 0);
     x0 = xrow != nullptr && k + t8 < a.hidden ? ld_tokens(xrow + k) : z;
-    x1 = xrow != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow + k + 32) : z;
+    x1 = two && xrow != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow + k + 32) : z;
   }
 };
 

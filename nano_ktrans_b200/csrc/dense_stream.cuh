@@ -94,7 +94,8 @@ constexpr size_t kStreamBytes = static_cast<size_t>(kSW) * kSlots * kStepBytes +
 //   Tile tile(int)           what copying a tile's rows needs
 //   rows(Tile, k, p, valid)  addresses at element k of rows (lane / 8) + 4 i, i < 4, and a bit for each that exists (every
 //                            address has to be readable for k < K)
-//   tokens(k, j, x0, x1)     column 8 j + g at elements k + 8 t and k + 32 + 8 t (zeros outside)
+//   tokens(k, two, j, x0, x1) column 8 j + g at elements k + 8 t and, with `two`, k + 32 + 8 t (zeros otherwise: that
+//                            half is the next warp's, and 0 x inf must not appear here)
 //   fin(tile, row, col, sum) one output; sum(row, col) adds the partials
 // FROWS outputs per column and tile (16, or 8 where rows g and g + 8 belong to
 // one output), `cols` columns.
@@ -110,6 +111,7 @@ struct Streamer {
   int tiles;
   int lb, ls;         // next to load: first tile of its round, step
   Tile lt[RT];
+  uint4 first[NT][2]; // token fragments of the first step: the same in every round
 
   MOE_DEV Streamer(const Src& source, unsigned char* smem) : src(source) {
     ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x >> 5) * (D * kStepBytes);
@@ -157,6 +159,13 @@ struct Streamer {
     const int w = threadIdx.x >> 5, left = halves - 2 * kSW * s;
     return left >= 2 * kSW || w < left - kSW;
   }
+  MOE_DEV void fetch(int s, uint4 (&x)[NT][2]) const {
+    const int k = 32 * half_at(s);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      src.tokens(k, both(s), j, x[j][0], x[j][1]);
+    }
+  }
   MOE_DEV void next_step() {
     if (++ls == steps) {
       ls = 0;
@@ -171,7 +180,10 @@ struct Streamer {
     steps = full + (halves - 2 * kSW * full > w ? 1 : 0);
     tiles = n_tiles;
     lb = ls = 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) first[j][0] = first[j][1] = make_uint4(0, 0, 0, 0);
     if (steps == 0 || tiles == 0) return;
+    fetch(0, first);  // ahead of the weights, or it would queue behind 128 KB of them (3.6 us at the start of a kernel)
     load_round();
 #pragma unroll
     for (int p = 0; p < PD; ++p) {
@@ -189,16 +201,6 @@ struct Streamer {
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4);      // first half of row g in a step
     const uint32_t frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);  // second half
     int turn = 0;
-    uint4 first[NT][2];
-    const auto fetch = [&](int s, uint4 (&x)[NT][2]) {
-      const int k = 32 * half_at(s);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        src.tokens(k, j, x[j][0], x[j][1]);
-        if (!both(s)) x[j][1] = make_uint4(0, 0, 0, 0);  // the next warp's half: 0 x inf must not appear here
-      }
-    };
-    if (steps > 0) fetch(0, first);
     for (int base = 0; base < tiles; base += RT) {
       float acc[RT][NT][4];
 #pragma unroll
