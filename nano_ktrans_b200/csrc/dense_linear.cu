@@ -93,8 +93,8 @@ cudaError_t launch_generic(const LinearArgs& a, int dtype, cudaStream_t st) {
 
 // ---------------------------------------------------------------------------
 // A few tokens: weight rows streamed past the token columns (dense_stream.cuh).
-// One block per SM; block c owns features [n c / G, n (c + 1) / G), so the SMs
-// have the same number of rows to within one.  A plain tile is 16 features; a
+// One block per SM, each with a range of features; the ranges differ by one
+// feature at most.  A plain tile is 16 features; a
 // gated tile is 8 gate rows (mma rows 0-7) and the same 8 up rows (mma rows
 // 8-15), so gate and up of a feature meet in one thread.
 // ---------------------------------------------------------------------------
@@ -150,8 +150,9 @@ __global__ void __launch_bounds__(kSThreads, 1) stream_linear_kernel(const __gri
   // A launch that may start early reads nothing before its predecessor is done
   // (weights too: they may be that kernel's output), and lets none start early.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int r0 = static_cast<int>(static_cast<int64_t>(a.n) * blockIdx.x / gridDim.x);
-  const int r1 = static_cast<int>(static_cast<int64_t>(a.n) * (blockIdx.x + 1) / gridDim.x);
+  // the first n % blocks blocks have a row more (one 32-bit division: this is on the way to the first load)
+  const uint32_t blocks = gridDim.x, b = blockIdx.x, each = static_cast<uint32_t>(a.n) / blocks, more = a.n - each * blocks;
+  const int r0 = static_cast<int>(each * b + min(b, more)), r1 = r0 + static_cast<int>(each + (b < more ? 1u : 0u));
   constexpr int kRows = GATED ? 8 : 16;
   const int tiles = (r1 - r0 + kRows - 1) / kRows;
   const LinearSrc<GATED, NT> src(a, r0, r1);

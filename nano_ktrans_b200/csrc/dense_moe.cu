@@ -586,8 +586,8 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
   // at once, then their sums are added in a fixed tree.  As many lanes as let the
   // block take all its quads in one pass, but 8 at least.
   const int quads = a.hidden / 4;
-  const int64_t all = static_cast<int64_t>(quads) * a.tokens;
-  const int q0 = static_cast<int>(all * blockIdx.x / gridDim.x), q1 = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x);
+  const uint32_t all = static_cast<uint32_t>(quads) * a.tokens, b = blockIdx.x;  // at most 16384 x 16
+  const int q0 = static_cast<int>(all * b / gridDim.x), q1 = static_cast<int>(all * (b + 1) / gridDim.x);
   int lanes = 32;
   while (lanes > 8 && kSThreads / lanes < q1 - q0) lanes /= 2;
   for (int qb = q0; qb < q1; qb += kSThreads / lanes) {
