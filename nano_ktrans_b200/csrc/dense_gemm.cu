@@ -223,37 +223,74 @@ MOE_DEV void give_up(volatile int* flag) {
 // ---------------------------------------------------------------------------
 constexpr int kPStages = 6, kPTile = 128 * 128, kPStage = 2 * kPTile;  // A and B half of one SM: 16 KB each
 constexpr int kPBarOff = kPStages * kPStage;
-constexpr size_t kPSmem = kPBarOff + 8 * (2 * kPStages + 4) + 16 + 1024;
+constexpr int kPTurnOff = kPBarOff + 8 * (2 * kPStages + 4) + 16;  // 32 rows x 16 columns of each epilogue warp
+constexpr int kPTurnRow = 17;
+constexpr size_t kPSmem = kPTurnOff + 4 * 32 * kPTurnRow * sizeof(float) + 1024;
 constexpr int kPThreads = 256;
 static_assert(kPSmem <= kSmemLimit, "shared-memory plan");
 
-// 16 output columns of one row from n on: wide stores where the row allows.
+// Residual of 64 columns of a row, read well ahead of the sums it joins: a read
+// per 16 columns when they are stored waits out a memory latency each time
+// (4000 x 5000 outputs, K = 1024, with bias: 148 us, so 76).
+struct Ahead64 {
+  uint4 r[8];
+  MOE_DEV void load(const LinearArgs& a, int64_t m, int n, bool row) {
+    const uint16_t* p = a.res + m * a.ldr + n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r[i] = row && n + 8 * i + 8 <= a.n ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
+  }
+};
+
+// 16 output columns of one row from n on, all of them there, rows on 16-byte
+// boundaries; r0 and r1: their residual (zeros without one).
 template <typename T>
-MOE_DEV void store16(const LinearArgs& a, int64_t m, int n, float (&v)[16], bool wide) {
-  uint16_t* o = a.out + m * a.ldo + n;
-  const uint16_t* r = a.res ? a.res + m * a.ldr + n : nullptr;
-  if (wide && n + 16 <= a.n) {
+MOE_DEV void store16(const LinearArgs& a, int64_t m, int n, float (&v)[16], uint4 r0, uint4 r1) {
+  uint4* o = reinterpret_cast<uint4*>(a.out + m * a.ldo + n);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (r) {
-        const uint4 q = *reinterpret_cast<const uint4*>(r + 8 * h);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  for (int h = 0; h < 2; ++h) {
+    const uint4 q = h == 0 ? r0 : r1;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = T::unpack(w[i]);
-          v[8 * h + 2 * i] += f.x;
-          v[8 * h + 2 * i + 1] += f.y;
-        }
-      }
-      uint32_t p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = T::pack(v[8 * h + 2 * i], v[8 * h + 2 * i + 1]);
-      *reinterpret_cast<uint4*>(o + 8 * h) = make_uint4(p[0], p[1], p[2], p[3]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = T::unpack(w[i]);
+      p[i] = T::pack(v[8 * h + 2 * i] + f.x, v[8 * h + 2 * i + 1] + f.y);
     }
+    o[h] = make_uint4(p[0], p[1], p[2], p[3]);
+  }
+}
+
+// The same for any row alignment and a ragged last column, by the whole warp:
+// 32 rows from m0 on, this lane's row in v.  The values are turned through
+// `turn` (32 x kPTurnRow), so that 16 lanes write neighbouring elements of a row;
+// a store of one element in each of 32 rows cost 32 sectors (3765 x 5789 gated outputs
+// of K = 152: 245 us, so 169).
+template <typename T>
+MOE_DEV void store_any(const LinearArgs& a, int64_t m0, int n, const float (&v)[16], float* turn) {
+  const int lane = threadIdx.x & 31, col = lane & 15;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) turn[lane * kPTurnRow + i] = v[i];
+  __syncwarp();
+  // this lane's 16 elements: rows lane / 16, + 2, ...; all residuals are read before anything is stored
+  const int64_t first = m0 + (lane >> 4);
+  const int rows = n + col < a.n ? static_cast<int>(min(static_cast<int64_t>(16), (a.m - first + 1) / 2)) : 0;
+  const float* mine = turn + (lane >> 4) * kPTurnRow + col;
+  uint16_t* o = a.out + first * a.ldo + n + col;
+  const int64_t step = 2 * a.ldo;
+  if (a.res != nullptr) {
+    const uint16_t* p = a.res + first * a.ldr + n + col;
+    uint16_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i, p += 2 * a.ldr) r[i] = i < rows ? *p : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i, o += step)
+      if (i < rows) *o = T::from_f32(mine[2 * i * kPTurnRow] + T::to_f32(r[i]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (n + i < a.n) o[i] = T::from_f32(r ? v[i] + T::to_f32(r[i]) : v[i]);
+    for (int i = 0; i < 16; ++i, o += step)
+      if (i < rows) *o = T::from_f32(mine[2 * i * kPTurnRow]);
   }
 }
 
@@ -379,40 +416,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
   } else if (warp >= 4) {
     const int q = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    float* turn = reinterpret_cast<float*>(smem + kPTurnOff) + q * 32 * kPTurnRow;
+    const bool wide_bias = reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
     int ti = 0;
     for (int i = pair; i < total; i += pairs, ++ti) {
       int mi, ni;
       place(i, mi, ni);
-      const int acc = ti & 1;
+      const int acc = ti & 1, n0 = ni * kTN;
+      const int64_t m = static_cast<int64_t>(mi) * 256 + 128 * rank + q * 32 + lane;
+      const bool ahead = !GATED && wide != 0 && a.res != nullptr;
+      Ahead64 cur, next;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cur.r[j] = next.r[j] = make_uint4(0, 0, 0, 0);
+      if (ahead) cur.load(a, m, n0, m < a.m);  // while the tile's MMAs still run
       const bool ok = mbar_wait(smem_u32(&acc_full[acc]), (ti >> 1) & 1);
       if (!__all_sync(kFullMask, ok)) {
         give_up(aborted);
         break;
       }
       fence_after();
-      const int64_t m = static_cast<int64_t>(mi) * 256 + 128 * rank + q * 32 + lane;
       const uint32_t base = tmem + acc * 256 + lanes;
 #pragma unroll 1
-      for (int c = 0; c < kTN; c += 16) {
-        const int n = ni * kTN + c;
-        if (n >= a.n) break;  // warp-uniform
-        float v[16];
-        tmem_ld16(base + c, v);
-        if constexpr (GATED) {
-          float u[16];
-          tmem_ld16(base + 128 + c, u);
-          activate_all(a.act, v);
+      for (int c = 0; c < kTN && n0 + c < a.n; c += 64) {  // warp-uniform
+        if (ahead && c + 64 < kTN) next.load(a, m, n0 + c + 64, m < a.m);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] *= u[j];
-        } else {
-          if (a.bias) {
+        for (int j = 0; j < 4; ++j) {
+          const int n = n0 + c + 16 * j;
+          if (n >= a.n) break;
+          float v[16];
+          tmem_ld16(base + c + 16 * j, v);
+          if constexpr (GATED) {
+            float u[16];
+            tmem_ld16(base + 128 + c + 16 * j, u);
+            activate_all(a.act, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (n + j < a.n) v[j] += T::to_f32(__ldg(a.bias + n + j));
+            for (int i = 0; i < 16; ++i) v[i] *= u[i];
+          } else {
+            if (a.bias && wide_bias && n + 16 <= a.n) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(a.bias + n + 8 * h));
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = T::unpack(w[i]);
+                  v[8 * h + 2 * i] += f.x;
+                  v[8 * h + 2 * i + 1] += f.y;
+                }
+              }
+            } else if (a.bias) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (n + i < a.n) v[i] += T::to_f32(__ldg(a.bias + n + i));
+            }
+            activate_all(a.act, v);
           }
-          activate_all(a.act, v);
+          if (wide != 0 && n + 16 <= a.n) {
+            if (m < a.m) store16<T>(a, m, n, v, cur.r[2 * j], cur.r[2 * j + 1]);
+          } else {
+            store_any<T>(a, m - lane, n, v, turn);
+          }
         }
-        if (m < a.m) store16<T>(a, m, n, v, wide != 0);
+        cur = next;
       }
       fence_before();
       __syncwarp();

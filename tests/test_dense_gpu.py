@@ -18,7 +18,7 @@ def rnd(dev, seed, *shape, dtype=BF16, scale=1.0):
 SHAPES = [(1, 2048, 2048), (1, 1, 1), (1, 5, 64), (2, 64, 8), (3, 7, 24), (7, 130, 1000), (8, 2048, 1408), (9, 257, 512),
           (15, 301, 4096), (16, 1024, 2048), (17, 1001, 1000), (31, 64, 14336), (33, 2050, 264), (64, 128, 64),
           (65, 129, 72), (100, 1408, 2048), (128, 2048, 1408), (129, 255, 136), (200, 2048, 1408), (256, 256, 256),
-          (257, 513, 520), (333, 1001, 1000), (640, 768, 2048), (1025, 2100, 1032), (2048, 4096, 1024),
+          (257, 513, 520), (333, 1001, 1000), (640, 768, 2048), (1025, 2100, 1032), (2048, 4096, 1024), (3001, 2777, 152),
           # rows that no wide load can take
           (1, 100, 77), (5, 33, 7), (40, 70, 129), (200, 130, 1001)]
 
