@@ -62,13 +62,6 @@ MOE_DEV uint4 ld_tokens(const uint16_t* p) {
   asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
-// Written by other blocks of the same launch: from L2, where they are coherent.
-MOE_DEV uint4 ld_l2(const uint16_t* p) {
-  uint4 r;
-  asm volatile("ld.global.cg.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
-  return r;
-}
-
 constexpr int kStepBytes = 2048;  // 16 rows x 64 elements
 
 constexpr int kSlots = 4;  // of a warp's ring

@@ -45,7 +45,9 @@ def run_x(layer, x, wr, **kw):
 SHAPES = [(1, 128, 8, 2048, 768, 0), (3, 128, 8, 2048, 768, 0), (16, 128, 8, 2048, 768, 0), (6, 60, 4, 2048, 1408, 5632),
           (5, 8, 2, 1024, 3584, 0), (1, 1, 1, 16, 16, 0), (16, 1, 1, 16, 16, 16), (4, 33, 16, 48, 80, 0), (5, 33, 5, 80, 48, 112),
           (16, 40, 16, 272, 144, 0), (8, 1024, 16, 256, 32, 0), (9, 7, 7, 528, 1040, 16), (12, 31, 3, 2064, 16, 0),
-          (2, 64, 6, 16, 2064, 32)]
+          (2, 64, 6, 16, 2064, 32),
+          # more intermediate rows than the blocks hold at a time
+          (16, 8, 2, 64, 16384, 1600)]
 
 
 @pytest.mark.parametrize("dtype,softmax,renorm", [(BF16, True, True), (BF16, True, False), (FP16, False, True), (FP16, True, True)])
