@@ -52,13 +52,17 @@ struct Fp16 {
 };
 
 // Activations in fp32 (the accumulator's type); the result is rounded once,
-// after the residual.
+// after the residual.  Where a GELU is small its factor is computed as the small
+// number that it is: 1 + erf and 1 + tanh cancel there, down to nothing below -5.5.
 template <int ACT>
 MOE_DEV float activate(float v) {
   if constexpr (ACT == MOE_ACT_SILU) return silu_f32(v);
-  if constexpr (ACT == MOE_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-  if constexpr (ACT == MOE_ACT_GELU_TANH)
-    return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+  if constexpr (ACT == MOE_ACT_GELU) return 0.5f * v * erfcf(v * -0.70710678118654752f);
+  if constexpr (ACT == MOE_ACT_GELU_TANH) {
+    // (1 + tanh y) / 2 = 1 / (1 + e^-2y), the exponential of the negative side on both, which cannot overflow
+    const float y = 0.79788456080286536f * (v + 0.044715f * v * v * v), e = expf(-2.0f * fabsf(y));
+    return v * ((y < 0.0f ? e : 1.0f) / (1.0f + e));
+  }
   if constexpr (ACT == MOE_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
   return v;
 }
