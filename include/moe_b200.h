@@ -429,7 +429,9 @@ int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_
  *   out[t] = round(residual[t] + sum_e w[t][e] * down_e(silu(gate_e(x[t])) * up_e(x[t]))
  *                  + sigmoid(x[t] . shared_gate_vec) * shared(x[t]))
  * in fp32, e over the experts that token t is routed to (and offload_mask
- * keeps).  Weights of one type: gate, up [num_experts][inter][hidden], down
+ * keeps).  Between the projections w * silu(gate) * up is held to 2^-16 of
+ * itself for bf16; for fp16 to 2^-22 of itself or 2^-39 of the largest one of its
+ * token and expert, whatever fp16's own range.  Weights of one type: gate, up [num_experts][inter][hidden], down
  * [num_experts][hidden][inter], shared likewise with shared_inter, router_w
  * [num_experts][hidden], all contiguous.  All weights have to be finite.
  * Routing, one of:

@@ -30,7 +30,10 @@
 // h is kept as hi + lo, two values of the layer's type (hi = round(h), lo =
 // round(h - hi): relative error 2^-16 for bf16, 2^-22 for fp16), each a column
 // of its own: the tensor cores have room, since the kernel is bound by reading
-// each routed expert's weights once.
+// each routed expert's weights once.  bf16 has fp32's range.  fp16 has not: there
+// h is first multiplied by a power of two that brings the largest |h| of a
+// token's piece into [2^14, 2^15) and that the partial sums are divided by, so an
+// h of any size is kept to 2^-22 of itself or 2^-39 of that largest one.
 #include "async_copy.cuh"
 #include "dense_stream.cuh"
 #include "kernels.h"
@@ -183,6 +186,9 @@ struct Tables {
   int place[kMoeTokens][kMoeTopK + 1];      // first range of its rows,
   int range[kMoeTokens][kMoeTopK + 1];
   int pieces[kMoeTokens][kMoeTopK + 2];     // and pieces of the experts before it
+  // fp16: bits of the largest finite |h| of a range's [piece][i-th token of its expert].  Experts have 16 rows at least,
+  // so a range of cap rows meets cap / 16 + 2 of them at most.
+  uint32_t top[kHBytes / 64 + 2 * kMoeTokens];
   int n_active;
   int ok;
 };
@@ -253,6 +259,11 @@ struct GateUpSrc {
     x1 = two && xrow != nullptr && k + 32 + t8 < a.hidden ? ld_tokens(xrow + k + 32) : z;
   }
 };
+
+// Power of two that brings a largest |h| (its bits) into [2^14, 2^15), and its
+// inverse.  Below 2^-111 the scale stays at 2^125: both are normal numbers then.
+MOE_DEV float h_scale(uint32_t top) { return __uint_as_float((268u - max(top >> 23, 16u)) << 23); }
+MOE_DEV float h_unscale(uint32_t top) { return __uint_as_float((max(top >> 23, 16u) - 14u) << 23); }
 
 // The down projection's columns of rows [lo, hi), all output rows: every warp
 // takes whole tiles of 16 output rows (tile w, w + 16, ...), RT at a time, over
@@ -332,6 +343,7 @@ struct DownStreamer {
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const uint32_t frag0 = g * 128 + ((t4 ^ ((g & 1) << 2)) << 4), frag1 = g * 128 + ((t4 ^ 4 ^ ((g & 1) << 2)) << 4);
     int turn = 0;
+    const int first = lo < routed ? place_of(a, lo) : tb.n_active;  // place of the range's first piece
     for (int v = lo; v < hi;) {
       const Piece p = piece(v);
       const int n = __popc(tb.tokens[p.place]);  // the expert's tokens
@@ -342,6 +354,13 @@ struct DownStreamer {
         hrow[j] = i < n ? hs + ((g & 1) * a.tokens + i) * cap + (v - lo) + 8 * t4 : nullptr;
       }
       float* out = a.partial + (static_cast<int64_t>(range + p.place) * a.tokens + t4) * a.hidden + g;
+      float back[ND];  // what the scale of the 4 j + t4-th token's h is undone by
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        back[j] = 1.0f;
+        if constexpr (!T::kBf16)
+          if (4 * j + t4 < n) back[j] = h_unscale(tb.top[(p.place - first) * a.tokens + 4 * j + t4]);
+      }
       for (int grp = 0; grp < count; grp += RT) {
         float acc[RT][ND][4];
 #pragma unroll
@@ -401,8 +420,8 @@ struct DownStreamer {
 #pragma unroll
             for (int j = 0; j < ND; ++j)
               if (4 * j + t4 < n) {
-                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden, acc[i][j][0] + acc[i][j][1]);
-                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden + 8, acc[i][j][2] + acc[i][j][3]);
+                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden, (acc[i][j][0] + acc[i][j][1]) * back[j]);
+                __stcg(o + static_cast<int64_t>(4 * j) * a.hidden + 8, (acc[i][j][2] + acc[i][j][3]) * back[j]);
               }
           }
       }
@@ -411,13 +430,48 @@ struct DownStreamer {
   }
 };
 
-// h = hi + lo in the layer's type.  An h beyond fp16's range stays infinite.
+// h = hi + lo in the layer's type; infinities and NaN stay what they are.
 template <typename T>
 MOE_DEV void store_split(uint16_t* hi, uint16_t* lo, float h) {
   const uint16_t b = T::from_f32(h);
   const float rest = h - T::to_f32(b);
   *hi = b;
   *lo = T::from_f32(isfinite(rest) ? rest : 0.0f);
+}
+
+// fp16: the fp32 values h [token of the expert][cap] of rows [lo, hi) become scaled
+// hi [token][cap] and lo [token][cap] in the same bytes.  The whole block's, which
+// holds all of h in registers between the two (13 values a thread).
+template <typename T>
+MOE_DEV void split_scaled(const MoeArgs& a, Tables& tb, float* hf, int cap, int lo, int hi) {
+  constexpr int kEach = kHBytes / 4 / kSThreads;
+  static_assert(kEach * 4 * kSThreads == kHBytes, "h is shared out evenly");
+  const int routed = tb.n_active * a.inter, first = lo < routed ? place_of(a, lo) : tb.n_active;
+  float h[kEach];
+  int slot[kEach];  // of the largest |h|, -1: no element here
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int e = threadIdx.x + kSThreads * j, i = e / cap, v = lo + e - i * cap;
+    slot[j] = -1;
+    h[j] = 0.0f;
+    if (i < a.tokens && v < hi) {
+      const int place = v < routed ? place_of(a, v) : tb.n_active;
+      if (i < __popc(tb.tokens[place])) {
+        slot[j] = (place - first) * a.tokens + i;
+        h[j] = hf[e];
+        if (isfinite(h[j])) atomicMax(&tb.top[slot[j]], __float_as_uint(fabsf(h[j])));
+      }
+    }
+  }
+  __syncthreads();
+  uint16_t* out = reinterpret_cast<uint16_t*>(hf);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (slot[j] >= 0) {
+      uint16_t* p = out + threadIdx.x + kSThreads * j;
+      store_split<T>(p, p + a.tokens * cap, h[j] * h_scale(tb.top[slot[j]]));
+    }
+  __syncthreads();
 }
 
 // The gate / up phase takes RG row tiles at once, the down phase RD, with up to ND column tiles of 4 tokens.
@@ -508,9 +562,13 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
     const int lo = split.begin(r), hi = split.begin(r + 1);
     DownStreamer<T, ND, RD> down(a, tb, smem, hs, a.h_cap, r, lo, hi);
     const auto put = [&](int place, int i, int v, float gate, float up) {
-      uint16_t* p = hs + i * a.h_cap + (v - lo);
-      store_split<T>(p, p + a.tokens * a.h_cap, tb.weight[place][i] * (silu_f32(gate) * up));
+      const float h = tb.weight[place][i] * (silu_f32(gate) * up);
+      const int at = i * a.h_cap + (v - lo);
+      if constexpr (T::kBf16) store_split<T>(hs + at, hs + at + a.tokens * a.h_cap, h);
+      else reinterpret_cast<float*>(hs)[at] = h;
     };
+    if constexpr (!T::kBf16)  // read again after the barriers of the gate / up phase
+      for (int i = tid; i < static_cast<int>(sizeof(tb.top) / sizeof(tb.top[0])); i += kSThreads) tb.top[i] = 0;
     if constexpr (ND <= 2) {
       // at most 8 tokens: one column tile holds them all, for all rows of the range at once
       const GateUpSrc src(a, tb, lo, hi, nullptr, a.tokens);
@@ -545,6 +603,7 @@ __global__ void __launch_bounds__(kSThreads, 1) dense_moe_kernel(const __grid_co
       }
     }
     __syncthreads();  // h is complete
+    if constexpr (!T::kBf16) split_scaled<T>(a, tb, reinterpret_cast<float*>(hs), a.h_cap, lo, hi);
     down.run();
     __syncthreads();  // h may be written again
   }
