@@ -5,8 +5,9 @@ layers/hybrid_moe.py:3321-3329, :3442-3533): router projection, routing, gated e
 sum, shared expert and the decoder layer's residual, in two kernel launches and without a host
 read.  ``MoeLayer`` is its counterpart on quantised weights.
 
-The layer borrows its weight tensors and keeps no other state: every call takes its workspace from
-the caching allocator of the stream it runs on, so calls on several streams are independent.
+The layer borrows its weight tensors and goes by where they are when it is called; it keeps no
+other state: every call takes its workspace from the caching allocator of the stream it runs on,
+so calls on several streams are independent.
 """
 from __future__ import annotations
 
@@ -45,12 +46,33 @@ def stack_expert_modules(modules) -> tuple:
     return stacks
 
 
+# A shared expert's weights, in the order of the layer's description.
+_SHARED = ("gate", "up", "down", "gate_vec")
+
+
 class DenseMoeLayer:
     """``gate`` / ``up`` [E, I, H], ``down`` [E, H, I] (bf16 or fp16, contiguous, on one CUDA device; H and I
     multiples of 16); ``shared``: ``{"gate", "up": [S, H], "down": [H, S], "gate_vec": [H]}`` or None."""
 
     def __init__(self, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *, top_k: int,
                  router_use_softmax: bool = True, normalize_topk_prob: bool = True, shared: Optional[dict] = None):
+        self.top_k = int(top_k)
+        self.router_use_softmax, self.normalize_topk_prob = bool(router_use_softmax), bool(normalize_topk_prob)
+        self.gate, self.up, self.down = gate, up, down
+        self.shared = dict(shared) if shared is not None else None
+        self._bind()
+
+    def _weights(self) -> list:
+        """The weight tensors as they are now, in the order of the description's pointers."""
+        held = [self.gate, self.up, self.down]
+        if self.shared is not None:
+            held += [self.shared[n] for n in _SHARED]
+        return held
+
+    def _bind(self) -> None:
+        """Check the weights and describe the layer by their present addresses.  Done again by the first call that finds
+        a weight elsewhere (a parameter given another ``data``, a module moved): the memory it left may be freed."""
+        gate, up, down, shared = self.gate, self.up, self.down, self.shared
         if gate.dim() != 3 or up.shape != gate.shape or down.shape != (gate.shape[0], gate.shape[2], gate.shape[1]):
             raise ValueError(f"gate and up must be [E, I, H] and down [E, H, I], got {tuple(gate.shape)}, "
                              f"{tuple(up.shape)}, {tuple(down.shape)}")
@@ -58,38 +80,33 @@ class DenseMoeLayer:
             raise ValueError(f"expert weights must be bf16 or fp16 CUDA tensors, got {gate.dtype} on {gate.device}")
         self.num_experts, self.inter_size, self.hidden_size = gate.shape
         self.dtype, self.device, self._dev = gate.dtype, gate.device, gate.get_device()
-        self.top_k = int(top_k)
-        self.router_use_softmax, self.normalize_topk_prob = bool(router_use_softmax), bool(normalize_topk_prob)
-        self.gate, self.up, self.down = gate, up, down
-        self.shared = dict(shared) if shared is not None else None
         self.shared_inter = 0
         h = self.hidden_size
         named = [("gate", gate), ("up", up), ("down", down)]
         if shared is not None:
             s = self.shared_inter = int(shared["gate"].shape[0])
-            for name, shape in (("gate", (s, h)), ("up", (s, h)), ("down", (h, s)), ("gate_vec", (h,))):
+            for name, shape in zip(_SHARED, ((s, h), (s, h), (h, s), (h,))):
                 if tuple(shared[name].shape) != shape or s < 1:
                     raise ValueError(f"shared {name} must be {shape}, got {tuple(shared[name].shape)}")
                 named.append((f"shared {name}", shared[name]))
         for name, w in named:
             if w.dtype is not gate.dtype or w.device != gate.device or not w.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous {gate.dtype} tensor on {gate.device}")
-        ptr = (lambda n: self.shared[n].data_ptr()) if self.shared is not None else (lambda n: None)
-        self._desc = _lib.MoeDenseDesc(gate.data_ptr(), up.data_ptr(), down.data_ptr(), ptr("gate"), ptr("up"),
-                                       ptr("down"), ptr("gate_vec"), self.num_experts, self.top_k, h,
-                                       self.inter_size, self.shared_inter, int(self.router_use_softmax),
-                                       int(self.normalize_topk_prob), _DTYPES[gate.dtype])
-        self._space = []  # workspace bytes by token count
+        at = [w.data_ptr() for w in self._weights()]
+        desc = _lib.MoeDenseDesc(*at, *([None] * (3 + len(_SHARED) - len(at))), self.num_experts, self.top_k, h,
+                                 self.inter_size, self.shared_inter, int(self.router_use_softmax),
+                                 int(self.normalize_topk_prob), _DTYPES[gate.dtype])
+        space = []  # workspace bytes by token count
         err = _err_buffer()
         with torch.cuda.device(self._dev):  # the workspace goes by the device's SMs
             for t in range(MAX_TOKENS + 1):
-                self._desc.num_tokens = t
+                desc.num_tokens = t
                 n = ctypes.c_int64(0)
-                rc = _lib.lib().moe_dense_workspace(ctypes.byref(self._desc), ctypes.byref(n), err, 512)
+                rc = _lib.lib().moe_dense_workspace(ctypes.byref(desc), ctypes.byref(n), err, 512)
                 if rc != _lib.MOE_OK:
                     raise _lib.MoeError(rc, err.value.decode(errors="replace"))
-                self._space.append(n.value)
-        self._layer_bytes = bytes(self._desc)
+                space.append(n.value)
+        self._at, self._space, self._layer_bytes = at, space, bytes(desc)
 
     # ------------------------------------------------------------------
     def _rows(self, t: torch.Tensor, name: str, rows: Optional[int], cols: int) -> int:
@@ -111,6 +128,8 @@ class DenseMoeLayer:
 
     def _run(self, x, residual, out, offload_mask, add_shared, stream, *, router=None, logits=None, ids=None,
              weights=None, out_ids=None, out_weights=None) -> torch.Tensor:
+        if [w.data_ptr() for w in self._weights()] != self._at:
+            self._bind()
         ldx = self._rows(x, "x", None, self.hidden_size)
         t = x.shape[0]
         d = _lib.MoeDenseDesc.from_buffer_copy(self._layer_bytes)
