@@ -27,22 +27,33 @@ MAX_TOKENS = _lib.DENSE_MAX_TOKENS
 _PROJECTIONS = (("w1", "w3", "w2"), ("gate_proj", "up_proj", "down_proj"))
 
 
+def _projections(module) -> list:
+    """An expert module's gate, up and down layers; a ValueError where they are not three linear layers without bias whose
+    weights are parameters of their own."""
+    names = next((n for n in _PROJECTIONS if all(hasattr(module, a) for a in n)), None)
+    layers = [getattr(module, a) for a in names or ()]
+    if names is None or any(getattr(p, "bias", None) is not None or "weight" not in getattr(p, "_parameters", ()) for p in layers):
+        raise ValueError(f"{type(module).__name__} is not a gated expert of three linear layers without bias")
+    return layers
+
+
 def stack_expert_modules(modules) -> tuple:
     """``(gate [E, I, H], up [E, I, H], down [E, H, I])`` of expert modules with ``w1`` / ``w3`` / ``w2`` (or
-    ``gate_proj`` / ``up_proj`` / ``down_proj``) linear layers without bias.  The modules' parameters are made views of
-    the stacks, so the weights are held once."""
-    parts = []
-    for m in modules:
-        names = next((n for n in _PROJECTIONS if all(hasattr(m, a) for a in n)), None)
-        if names is None or any(getattr(getattr(m, a), "bias", None) is not None for a in names):
-            raise ValueError(f"{type(m).__name__} is not a gated expert of three linear layers without bias")
-        parts.append([getattr(m, a) for a in names])
+    ``gate_proj`` / ``up_proj`` / ``down_proj``) linear layers without bias, of one size, type and device.  The modules'
+    parameters are made views of the stacks, so the weights are held once."""
+    parts = [_projections(m) for m in modules]
     if not parts:
         raise ValueError("no expert modules")
-    stacks = tuple(torch.stack([p[j].weight.detach() for p in parts]).contiguous() for j in range(3))
-    for e, p in enumerate(parts):
+    weights = [[p.weight for p in layers] for layers in parts]
+    kind = {(w.dtype, w.device) for ws in weights for w in ws}
+    if len(kind) > 1 or any(ws[j].shape != weights[0][j].shape for ws in weights for j in range(3)):
+        raise ValueError("the experts differ in size, type or device: one stack cannot hold them")
+    if len({id(w) for ws in weights for w in ws}) < 3 * len(weights):
+        raise ValueError("two experts share a weight: it cannot be a view of two places")
+    stacks = tuple(torch.stack([ws[j].detach() for ws in weights]).contiguous() for j in range(3))
+    for e, ws in enumerate(weights):
         for j in range(3):
-            p[j].weight.data = stacks[j][e]
+            ws[j].data = stacks[j][e]
     return stacks
 
 
