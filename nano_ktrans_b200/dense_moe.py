@@ -12,6 +12,7 @@ so calls on several streams are independent.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional
 
 import torch
@@ -215,3 +216,60 @@ class DenseMoeLayer:
         if rc != _lib.MOE_OK:
             raise _lib.MoeError(rc, err.value.decode(errors="replace"))
         return int(st.value)
+
+
+class ResidentExperts:
+    """Expert modules run by a ``DenseMoeLayer``: their weights are stacked (``stack_expert_modules``) and stacked anew by the
+    first call that finds one of them to be elsewhere than in the stack, whatever put it there: a module moved or cast, a
+    parameter given other ``data`` or replaced, a layer or an expert exchanged."""
+
+    def __init__(self, modules, resident, num_experts: int, top_k: int, device, make_layer=DenseMoeLayer):
+        self._modules, self._resident, self._num_experts, self._top_k = modules, list(resident), num_experts, top_k
+        self._device, self._make_layer = device, make_layer
+        self.layer = None                          # None: the modules are to be called themselves
+        self.slot: Optional[torch.Tensor] = None   # expert -> its place in the stack, -1: not in it
+        self._stack()
+
+    def current(self, modules):
+        """The layer on the present weights of ``modules``, or None where it cannot run them (they are on another device, or
+        have become something else than gated experts of one size and type)."""
+        if modules is not self._modules or not self._unchanged():
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the resident experts' weights have changed since they were stacked: call the layer once "
+                                   "outside the capture first")
+            self._modules = modules
+            try:
+                self._stack()
+            except (ValueError, _lib.MoeError):
+                pass
+        return self.layer
+
+    def _stack(self) -> None:
+        self.layer = self.slot = None
+        here = [e for e in self._resident if str(e) in self._modules]
+        experts = [self._modules[str(e)] for e in here]
+        try:
+            weights = [p.weight for m in experts for p in _projections(m)]
+            if weights and all(w.device == self._device for w in weights):
+                layer = self._make_layer(*stack_expert_modules(experts), top_k=self._top_k)
+                slot = torch.full((self._num_experts,), -1, dtype=torch.int64)
+                slot[here] = torch.arange(len(here))
+                self.layer, self.slot = layer, slot.to(self._device)
+        finally:
+            self._watch(experts)
+
+    def _watch(self, experts) -> None:
+        """What has to stay the same: objects under their names, and addresses.  Kept as columns, so that the comparison
+        of a call runs in a few C loops."""
+        children = [c for m in experts for c in m._modules.values() if c is not None]
+        held = [(getattr(self._modules, "_modules", self._modules), str(e)) for e in self._resident]
+        held += [(m._modules, n) for m in experts for n in m._modules]
+        held += [(c._parameters, n) for c in children for n in c._parameters]
+        self._dicts, self._names = [d for d, _ in held], [n for _, n in held]
+        self._objects = list(map(dict.get, self._dicts, self._names))
+        self._params = [w for c in children for w in c._parameters.values() if w is not None]
+        self._at = list(map(torch.Tensor.data_ptr, self._params))
+
+    def _unchanged(self) -> bool:
+        return (all(map(operator.is_, map(dict.get, self._dicts, self._names), self._objects))
+                and list(map(torch.Tensor.data_ptr, self._params)) == self._at)

@@ -16,10 +16,11 @@ GPU-resident in ``gpu_experts_mask`` are served one of three ways, chosen by
 * ``"modules"``: as dense ``nn.Module``s in the reference's per-expert loop
   (:3501-3533, with its host reads of the routed ids), summed with the
   backend's part (:3570) — bit-for-bit the reference's split semantics;
-* ``"dense"``: the modules' bf16 weights stacked once (the modules keep views of
-  them) and run by ``DenseMoeLayer`` — for up to 16 tokens all resident experts,
-  the weighted sum and the addition of the backend's part are two launches
-  without a host read and one rounding; larger batches take the ``"modules"`` loop.
+* ``"dense"``: the modules' bf16 weights stacked (the modules keep views of the
+  stack, and are stacked anew when they have been moved or given other weights) and
+  run by ``DenseMoeLayer`` — for up to 16 tokens all resident experts, the weighted
+  sum and the addition of the backend's part are two launches without a host read
+  and one rounding; larger batches take the ``"modules"`` loop.
 
 The reference's residency machinery (migration queues, prefetch caches,
 schedulers; hybrid_moe.py:109-254, :2841-3300) is not part of this path; its
@@ -35,7 +36,7 @@ from torch import nn
 
 from .cuda_moe import CudaMoEBackend
 from .dense_moe import MAX_TOKENS as DENSE_MAX_TOKENS
-from .dense_moe import DenseMoeLayer, stack_expert_modules
+from .dense_moe import ResidentExperts
 from .offload_backend import normalize_offload_backend_name
 
 
@@ -93,18 +94,20 @@ class HybridMoE(nn.Module):
                       router_use_softmax=router_use_softmax, normalize_topk_prob=normalize_topk_prob)
         kwargs.update(offload_backend_kwargs or {})
         self.offload_backend = CudaMoEBackend(**kwargs)
-        self._dense: Optional[DenseMoeLayer] = None
-        self._dense_slot: Optional[torch.Tensor] = None  # expert -> its place in the stack, -1: not resident
-        resident = [e for e in range(num_experts) if bool(gpu_experts_mask[e]) and str(e) in gpu_experts]
-        if resident_experts == "dense" and resident:
-            device = self.offload_backend.device
-            stacks = [w.to(device) for w in stack_expert_modules([gpu_experts[str(e)] for e in resident])]
-            self._dense = DenseMoeLayer(*stacks, top_k=top_k)
-            slot = torch.full((num_experts,), -1, dtype=torch.int64)
-            slot[resident] = torch.arange(len(resident))
-            self._dense_slot = slot.to(device)
+        self._resident: Optional[ResidentExperts] = None
+        if resident_experts == "dense":
+            resident = [e for e in range(num_experts) if bool(gpu_experts_mask[e])]
+            self._resident = ResidentExperts(gpu_experts, resident, num_experts, top_k, self.offload_backend.layer.device)
         self.last_topk_ids: Optional[torch.Tensor] = None
         self.last_topk_weights: Optional[torch.Tensor] = None
+
+    @property
+    def _dense(self):
+        return self._resident.layer if self._resident is not None else None
+
+    @property
+    def _dense_slot(self):
+        return self._resident.slot if self._resident is not None else None
 
     def forward(self, hidden_states: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         layer = self.offload_backend.layer
@@ -118,14 +121,18 @@ class HybridMoE(nn.Module):
             self.last_topk_ids, self.last_topk_weights = ids, w
             return out
 
+        dense = None
+        if self._resident is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
+            dense = self._resident.current(self.gpu_experts)
+
         topk_ids, topk_weights = layer.route(router_logits)
         self.last_topk_ids, self.last_topk_weights = topk_ids, topk_weights
         stream = torch.cuda.current_stream(hidden_states.device).cuda_stream
         self.offload_backend.submit_forward(hidden_states, topk_ids, topk_weights, stream)
 
-        if self._dense is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
+        if dense is not None:
             offloaded = self.offload_backend.sync_forward(hidden_states, stream)
-            return self._dense.experts_forward(hidden_states, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
+            return dense.experts_forward(hidden_states, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
 
         final_gpu_states = torch.zeros_like(hidden_states)
         mask_host = self.gpu_experts_mask.bool().cpu().tolist()
