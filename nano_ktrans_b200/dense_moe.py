@@ -218,31 +218,55 @@ class DenseMoeLayer:
         return int(st.value)
 
 
+def _version(t: torch.Tensor) -> int:
+    return 0 if t.is_inference() else t._version  # tensors made in inference mode count no changes
+
+
 class ResidentExperts:
     """Expert modules run by a ``DenseMoeLayer``: their weights are stacked (``stack_expert_modules``) and stacked anew by the
     first call that finds one of them to be elsewhere than in the stack, whatever put it there: a module moved or cast, a
-    parameter given other ``data`` or replaced, a layer or an expert exchanged."""
+    parameter given other ``data`` or replaced, a layer or an expert exchanged, another residency mask."""
 
-    def __init__(self, modules, resident, num_experts: int, top_k: int, device, make_layer=DenseMoeLayer):
-        self._modules, self._resident, self._num_experts, self._top_k = modules, list(resident), num_experts, top_k
+    def __init__(self, modules, mask: torch.Tensor, top_k: int, device, make_layer=DenseMoeLayer):
+        self._modules, self._top_k = modules, top_k
         self._device, self._make_layer = device, make_layer
         self.layer = None                          # None: the modules are to be called themselves
         self.slot: Optional[torch.Tensor] = None   # expert -> its place in the stack, -1: not in it
+        self._read(mask)
         self._stack()
 
-    def current(self, modules):
+    @property
+    def some(self) -> bool:
+        """Whether the mask of the last call named any expert as resident."""
+        return len(self._resident) > 0
+
+    def current(self, modules, mask: torch.Tensor):
         """The layer on the present weights of ``modules``, or None where it cannot run them (they are on another device, or
         have become something else than gated experts of one size and type)."""
-        if modules is not self._modules or not self._unchanged():
+        same = self._same_mask(mask)
+        if not same or modules is not self._modules or not self._unchanged():
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the resident experts' weights have changed since they were stacked: call the layer once "
-                                   "outside the capture first")
+                raise RuntimeError("the resident experts' weights or mask have changed since they were stacked: call the "
+                                   "layer once outside the capture first")
+            if not same:
+                self._read(mask)
             self._modules = modules
             try:
                 self._stack()
             except (ValueError, _lib.MoeError):
                 pass
         return self.layer
+
+    def _read(self, mask: torch.Tensor) -> None:
+        self._mask, self._mask_version = mask, _version(mask)
+        self._mask_host = mask.bool().cpu().clone()
+        self._resident = torch.nonzero(self._mask_host).flatten().tolist()
+
+    def _same_mask(self, mask: torch.Tensor) -> bool:
+        """Without a host read: a mask on a device is the same while the tensor is and counts no change."""
+        if mask.device.type == "cpu":
+            return torch.equal(mask.bool(), self._mask_host)
+        return mask is self._mask and _version(mask) == self._mask_version
 
     def _stack(self) -> None:
         self.layer = self.slot = None
@@ -252,7 +276,7 @@ class ResidentExperts:
             weights = [p.weight for m in experts for p in _projections(m)]
             if weights and all(w.device == self._device for w in weights):
                 layer = self._make_layer(*stack_expert_modules(experts), top_k=self._top_k)
-                slot = torch.full((self._num_experts,), -1, dtype=torch.int64)
+                slot = torch.full((self._mask_host.numel(),), -1, dtype=torch.int64)
                 slot[here] = torch.arange(len(here))
                 self.layer, self.slot = layer, slot.to(self._device)
         finally:

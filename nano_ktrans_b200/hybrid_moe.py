@@ -96,8 +96,7 @@ class HybridMoE(nn.Module):
         self.offload_backend = CudaMoEBackend(**kwargs)
         self._resident: Optional[ResidentExperts] = None
         if resident_experts == "dense":
-            resident = [e for e in range(num_experts) if bool(gpu_experts_mask[e])]
-            self._resident = ResidentExperts(gpu_experts, resident, num_experts, top_k, self.offload_backend.layer.device)
+            self._resident = ResidentExperts(gpu_experts, gpu_experts_mask, top_k, self.offload_backend.layer.device)
         self.last_topk_ids: Optional[torch.Tensor] = None
         self.last_topk_weights: Optional[torch.Tensor] = None
 
@@ -111,7 +110,13 @@ class HybridMoE(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         layer = self.offload_backend.layer
-        if self.resident_experts == "kernels" or not bool(self.gpu_experts_mask.bool().any()):
+        if self._resident is not None:
+            dense = self._resident.current(self.gpu_experts, self.gpu_experts_mask)
+            some_resident = self._resident.some
+        else:
+            dense = None
+            some_resident = self.resident_experts != "kernels" and bool(self.gpu_experts_mask.bool().any())
+        if not some_resident:
             t = hidden_states.shape[0]
             ids = torch.empty(t, self.top_k, dtype=torch.int64, device=hidden_states.device)
             w = torch.empty(t, self.top_k, dtype=torch.bfloat16, device=hidden_states.device)
@@ -121,16 +126,12 @@ class HybridMoE(nn.Module):
             self.last_topk_ids, self.last_topk_weights = ids, w
             return out
 
-        dense = None
-        if self._resident is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
-            dense = self._resident.current(self.gpu_experts)
-
         topk_ids, topk_weights = layer.route(router_logits)
         self.last_topk_ids, self.last_topk_weights = topk_ids, topk_weights
         stream = torch.cuda.current_stream(hidden_states.device).cuda_stream
         self.offload_backend.submit_forward(hidden_states, topk_ids, topk_weights, stream)
 
-        if dense is not None:
+        if dense is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
             offloaded = self.offload_backend.sync_forward(hidden_states, stream)
             return dense.experts_forward(hidden_states, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
 

@@ -126,6 +126,36 @@ def test_weights_that_are_replaced(how, t, codes, cuda_device):
     check(moe, t)
 
 
+@pytest.mark.parametrize("t", TOKENS)
+@pytest.mark.parametrize("mask_device", ["cpu", "cuda"])
+def test_residency_that_changes(mask_device, t, codes, cuda_device):
+    mods = modules(cuda_device, on=[1, 2, 4, 7])
+    moe = build(codes, mods, mask_device=mask_device)
+    check(moe, t)
+    for on in ([1, 4], [1, 2, 4, 7], [2], [1, 4, 7]):
+        mask = torch.zeros(E, dtype=torch.bool, device=mask_device)
+        mask[on] = True
+        moe.gpu_experts_mask = mask
+        moe.offload_backend.update_gpu_expert_mask(mask)
+        check(moe, t, on)
+    mask[[1, 4]] = False  # the same tensor, in place
+    moe.offload_backend.update_gpu_expert_mask(mask)
+    check(moe, t, [7])
+
+
+def test_no_host_read_whatever_device_the_mask_is_on(codes, cuda_device):
+    for mask_device in ("cpu", "cuda"):
+        moe = build(codes, modules(cuda_device), mask_device=mask_device)
+        x, lg = inputs(6)
+        moe(x, lg)
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            moe(x, lg)
+        finally:
+            torch.cuda.set_sync_debug_mode(0)
+
+
 def test_a_capture_finds_changed_weights(codes, cuda_device):
     """The stack cannot be made anew inside a capture: refused, and right after one call outside."""
     moe = build(codes, modules(cuda_device))

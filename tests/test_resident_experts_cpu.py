@@ -28,12 +28,18 @@ class Stacks:
 
 def make(on=(1, 4, 7), device="cpu"):
     mods = torch.nn.ModuleDict({str(n): Expert(n, device=device) for n in on})
-    return mods, ResidentExperts(mods, on, 9, 2, torch.device("cpu"), make_layer=Stacks)
+    return mods, ResidentExperts(mods, mask_of(on), 2, torch.device("cpu"), make_layer=Stacks)
+
+
+def mask_of(on):
+    mask = torch.zeros(9, dtype=torch.bool)
+    mask[list(on)] = True
+    return mask
 
 
 def holds(res, mods, on=(1, 4, 7)):
     """The stack has the modules' weights, and is where they are."""
-    layer = res.current(mods)
+    layer = res.current(mods, mask_of(on))
     assert res.slot.tolist() == [on.index(n) if n in on else -1 for n in range(9)]
     for j, name in enumerate(NAMES):
         for n in on:
@@ -90,30 +96,30 @@ def test_another_dict_of_modules():
     other = torch.nn.ModuleDict({str(n): Expert(30 + n) for n in (1, 4, 7)})
     holds(res, other)
     del other["4"]
-    assert res.current(other) is not None and res.slot.tolist() == [-1, 0, -1, -1, -1, -1, -1, 1, -1]
+    assert res.current(other, mask_of((1, 4, 7))) is not None and res.slot.tolist() == [-1, 0, -1, -1, -1, -1, -1, 1, -1]
     other["4"] = Expert(50)
     holds(res, other)
 
 
 def test_modules_on_another_device_are_called_themselves():
     mods, res = make(device="meta")
-    assert res.current(mods) is None
+    assert res.current(mods, mask_of((1, 4, 7))) is None
     mods.to_empty(device="cpu")
     mods.load_state_dict({k: torch.randn(v.shape).to(v.dtype) for k, v in mods.state_dict().items()})
     holds(res, mods)
     mods["4"].to("meta")
-    assert res.current(mods) is None and res.slot is None
+    assert res.current(mods, mask_of((1, 4, 7))) is None and res.slot is None
 
 
 def test_modules_that_become_something_else_are_called_themselves():
     mods, res = make()
     holds(res, mods)
     mods["4"].w1 = torch.nn.Linear(H, I, dtype=torch.bfloat16)  # with a bias
-    assert res.current(mods) is None and res.current(mods) is None
+    assert res.current(mods, mask_of((1, 4, 7))) is None and res.current(mods, mask_of((1, 4, 7))) is None
     mods["4"].w1.bias = None
     holds(res, mods)
     mods["1"].w2.float()
-    assert res.current(mods) is None
+    assert res.current(mods, mask_of((1, 4, 7))) is None
     mods["1"].w2.bfloat16()
     holds(res, mods)
 
@@ -122,9 +128,45 @@ def test_a_capture_makes_nothing_anew(monkeypatch):
     mods, res = make()
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-    layer = res.current(mods)
+    layer = res.current(mods, mask_of((1, 4, 7)))
     data(mods)
     with pytest.raises(RuntimeError, match="outside the capture"):
-        res.current(mods)
+        res.current(mods, mask_of((1, 4, 7)))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     assert holds(res, mods) is not layer
+
+
+def test_the_mask_changes():
+    mods, res = make()
+    layer = holds(res, mods)
+    for on in ((1, 4), (7,), (1, 4, 7)):
+        mask = mask_of(on)
+        again = res.current(mods, mask)
+        assert again is not layer and res.some and res.current(mods, mask.clone()) is again
+        holds(res, mods, on)
+        layer = again
+    mask[4] = False  # in place
+    assert res.current(mods, mask) is not layer
+    holds(res, mods, (1, 7))
+    assert res.current(mods, mask_of(())) is None and not res.some
+    mods["2"] = Expert(60)
+    holds(res, mods, (1, 2))
+
+
+def test_a_resident_expert_without_a_module():
+    """It has no place in the stack, until it gets a module."""
+    mods, res = make()
+    res.current(mods, mask_of((1, 3, 4)))
+    assert res.slot.tolist() == [-1, 0, -1, -1, 1, -1, -1, -1, -1]
+    mods["3"] = Expert(70)
+    holds(res, mods, (1, 3, 4))
+
+
+def test_masks_of_other_types_and_of_inference_mode():
+    mods, res = make()
+    layer = holds(res, mods)
+    assert res.current(mods, mask_of((1, 4, 7)).to(torch.uint8)) is layer
+    with torch.inference_mode():
+        mask = mask_of((1, 4))
+    res.current(mods, mask)
+    holds(res, mods, (1, 4))
