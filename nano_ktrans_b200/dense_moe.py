@@ -222,6 +222,31 @@ def _version(t: torch.Tensor) -> int:
     return 0 if t.is_inference() else t._version  # tensors made in inference mode count no changes
 
 
+def _shows_silu(module, layers) -> bool:
+    """Whether the module, whatever its weights, computes ``down(silu(gate(x)) * up(x))``: called on weights that show its
+    activation value by value (gate and up hold a value each in the column that x picks, down is the identity), so that an
+    activation of another kind, a limit, a scale or a term beside the product is seen."""
+    names = {p: n for n, p in module.named_children()}
+    if any(type(p).forward is not torch.nn.Linear.forward or "forward" in p.__dict__ or p not in names for p in layers):
+        return False
+    w = layers[0].weight
+    inter, hidden = w.shape
+    gate, up = torch.zeros_like(w, requires_grad=False), torch.zeros_like(w, requires_grad=False)
+    gate[:, 0] = torch.linspace(-12.0, 12.0, inter, device=w.device)
+    up[:, 0] = torch.linspace(-9.0, 10.0, inter, device=w.device).roll(inter // 3)
+    down = torch.eye(hidden, inter, dtype=w.dtype, device=w.device)
+    x = torch.zeros(3, hidden, dtype=w.dtype, device=w.device)
+    x[0, 0], x[1, 0] = 1.0, -1.0
+    with torch.no_grad():
+        out = torch.func.functional_call(module, {f"{names[p]}.weight": v for p, v in zip(layers, (gate, up, down))}, (x,))
+    n = min(hidden, inter)
+    g, u = gate[:n, 0].double(), up[:n, 0].double()
+    want = torch.zeros(3, hidden, dtype=torch.float64, device=w.device)
+    want[0, :n], want[1, :n] = g * torch.sigmoid(g) * u, g * torch.sigmoid(-g) * u
+    # roundings to the type of sigmoid, silu and the product, half a unit each
+    return out.shape == want.shape and bool(((out.double() - want).abs() <= 2 * torch.finfo(w.dtype).eps * want.abs()).all())
+
+
 class ResidentExperts:
     """Expert modules run by a ``DenseMoeLayer``: their weights are stacked (``stack_expert_modules``) and stacked anew by the
     first call that finds one of them to be elsewhere than in the stack, whatever put it there: a module moved or cast, a
@@ -241,10 +266,11 @@ class ResidentExperts:
         return len(self._resident) > 0
 
     def current(self, modules, mask: torch.Tensor):
-        """The layer on the present weights of ``modules``, or None where it cannot run them (they are on another device, or
-        have become something else than gated experts of one size and type)."""
+        """The layer on the present weights of ``modules``, or None where they have to be called themselves: on another
+        device, with hooks, or since they have become something else than bf16 experts of the layer's function."""
         same = self._same_mask(mask)
-        if not same or modules is not self._modules or not self._unchanged():
+        if (not same or modules is not self._modules or not self._unchanged()
+                or (self._put_off and not any(self._hooks))):
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the resident experts' weights or mask have changed since they were stacked: call the "
                                    "layer once outside the capture first")
@@ -255,7 +281,7 @@ class ResidentExperts:
                 self._stack()
             except (ValueError, _lib.MoeError):
                 pass
-        return self.layer
+        return None if any(self._hooks) else self.layer
 
     def _read(self, mask: torch.Tensor) -> None:
         self._mask, self._mask_version = mask, _version(mask)
@@ -272,9 +298,19 @@ class ResidentExperts:
         self.layer = self.slot = None
         here = [e for e in self._resident if str(e) in self._modules]
         experts = [self._modules[str(e)] for e in here]
+        self._watch(experts)
+        self._put_off = any(self._hooks)  # the check below would run them
+        if self._put_off:
+            return
         try:
-            weights = [p.weight for m in experts for p in _projections(m)]
+            parts = [_projections(m) for m in experts]
+            weights = [p.weight for layers in parts for p in layers]
             if weights and all(w.device == self._device for w in weights):
+                if any(w.dtype is not torch.bfloat16 for w in weights):
+                    raise ValueError("resident experts must be torch.bfloat16, the type of the routing weights")
+                for m, layers in zip(experts, parts):
+                    if not _shows_silu(m, layers):
+                        raise ValueError(f"{type(m).__name__} does not compute w2(silu(w1 x) * w3 x) of its weights")
                 layer = self._make_layer(*stack_expert_modules(experts), top_k=self._top_k)
                 slot = torch.full((self._mask_host.numel(),), -1, dtype=torch.int64)
                 slot[here] = torch.arange(len(here))
@@ -289,10 +325,12 @@ class ResidentExperts:
         held = [(getattr(self._modules, "_modules", self._modules), str(e)) for e in self._resident]
         held += [(m._modules, n) for m in experts for n in m._modules]
         held += [(c._parameters, n) for c in children for n in c._parameters]
+        held += [(m.__dict__, "forward") for m in experts + children]  # an instance's own, as wrappers set it
         self._dicts, self._names = [d for d, _ in held], [n for _, n in held]
         self._objects = list(map(dict.get, self._dicts, self._names))
         self._params = [w for c in children for w in c._parameters.values() if w is not None]
         self._at = list(map(torch.Tensor.data_ptr, self._params))
+        self._hooks = [h for m in experts + children for h in (m._forward_hooks, m._forward_pre_hooks)]
 
     def _unchanged(self) -> bool:
         return (all(map(operator.is_, map(dict.get, self._dicts, self._names), self._objects))

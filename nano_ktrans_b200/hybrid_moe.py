@@ -20,7 +20,9 @@ GPU-resident in ``gpu_experts_mask`` are served one of three ways, chosen by
   stack, and are stacked anew when they have been moved or given other weights) and
   run by ``DenseMoeLayer`` — for up to 16 tokens all resident experts, the weighted
   sum and the addition of the backend's part are two launches without a host read
-  and one rounding; larger batches take the ``"modules"`` loop.
+  and one rounding; larger batches take the ``"modules"`` loop, and so do all calls
+  while a module has forward hooks.  Modules that do not compute
+  ``w2(silu(w1 x) * w3 x)`` are refused.  Forward only.
 
 The reference's residency machinery (migration queues, prefetch caches,
 schedulers; hybrid_moe.py:109-254, :2841-3300) is not part of this path; its
@@ -79,6 +81,8 @@ class HybridMoE(nn.Module):
         self.hidden_act = hidden_act
         if resident_experts not in ("kernels", "modules", "dense"):
             raise ValueError("resident_experts must be 'kernels', 'modules' or 'dense'")
+        if resident_experts == "dense" and hidden_act not in ("silu", "swish"):
+            raise ValueError(f"resident_experts='dense' runs gated SiLU experts, not hidden_act {hidden_act!r}")
         self.resident_experts = resident_experts
         self.has_cpu_experts = bool((~gpu_experts_mask.bool()).any().item())
         self.offload_backend_name = normalize_offload_backend_name(offload_backend)

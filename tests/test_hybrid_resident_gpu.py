@@ -156,6 +156,58 @@ def test_no_host_read_whatever_device_the_mask_is_on(codes, cuda_device):
             torch.cuda.set_sync_debug_mode(0)
 
 
+def test_experts_of_another_kind_are_refused(codes, cuda_device):
+    with pytest.raises(ValueError, match="hidden_act"):
+        build(codes, modules(cuda_device), hidden_act="gelu")
+    with pytest.raises(ValueError, match="silu"):
+        build(codes, modules(cuda_device, act=torch.nn.functional.gelu))
+    with pytest.raises(ValueError, match="silu"):
+        build(codes, modules(cuda_device, act=lambda v: torch.nn.functional.silu(v).clamp(max=7)))
+    with pytest.raises(ValueError, match="bfloat16"):
+        build(codes, modules(cuda_device, dtype=torch.float16))
+    with pytest.raises(ValueError, match="bfloat16"):
+        build(codes, modules(cuda_device, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("where", ["expert", "linear"])
+@pytest.mark.parametrize("when", ["before", "after"])
+def test_hooks_are_run(when, where, codes, cuda_device):
+    """A module with hooks is called, on small batches too."""
+    mods = modules(cuda_device)
+    seen = []
+    target = mods["4"] if where == "expert" else mods["4"].w2
+    if when == "before":
+        handle = target.register_forward_hook(lambda m, a, y: seen.append(1) or y * 0)
+    moe = build(codes, mods)
+    if when == "after":
+        handle = target.register_forward_hook(lambda m, a, y: seen.append(1) or y * 0)
+    x, lg = inputs(8)
+    lg[:, 4] = 9.0
+    seen.clear()
+    got = moe(x, lg)
+    want = build(codes, mods, resident="modules")(x, lg)
+    assert len(seen) == 2 and torch.equal(got, want)
+    handle.remove()
+    seen.clear()
+    check(moe, 8)
+    assert not seen
+
+
+@pytest.mark.parametrize("t", [1, 8])
+def test_a_module_whose_function_changes(t, codes, cuda_device):
+    """Its own forward replaced, as adapters do: the module is called."""
+    mods = modules(cuda_device)
+    moe = build(codes, mods)
+    check(moe, t)
+    inner = mods["4"].forward
+    mods["4"].forward = lambda x: 0.5 * inner(x)
+    x, lg = inputs(t)
+    lg[:, 4] = 9.0
+    assert torch.equal(moe(x, lg), build(codes, mods, resident="modules")(x, lg))
+    del mods["4"].forward
+    check(moe, t)
+
+
 def test_a_capture_finds_changed_weights(codes, cuda_device):
     """The stack cannot be made anew inside a capture: refused, and right after one call outside."""
     moe = build(codes, modules(cuda_device))

@@ -170,3 +170,110 @@ def test_masks_of_other_types_and_of_inference_mode():
         mask = mask_of((1, 4))
     res.current(mods, mask)
     holds(res, mods, (1, 4))
+
+
+def biased(m):
+    m.w2.bias = torch.nn.Parameter(torch.ones(H, dtype=torch.bfloat16))
+
+
+def own_forward(m):
+    inner = m.forward
+    m.forward = lambda x: 0.5 * inner(x)
+
+
+def linear_forward(m):
+    inner = m.w3.forward
+    m.w3.forward = lambda x: inner(x) + 1
+
+
+class Another(Expert):
+    def __init__(self, function):
+        super().__init__(80)
+        self.function = function
+
+    def forward(self, x):
+        return self.function(self, x)
+
+
+F = torch.nn.functional
+OTHERS = dict(
+    gelu=lambda m, x: m.w2(F.gelu(m.w1(x)) * m.w3(x)),
+    quick_gelu=lambda m, x: m.w2(m.w1(x) * torch.sigmoid(1.702 * m.w1(x)) * m.w3(x)),
+    hardswish=lambda m, x: m.w2(F.hardswish(m.w1(x)) * m.w3(x)),
+    mish=lambda m, x: m.w2(F.mish(m.w1(x)) * m.w3(x)),
+    relu=lambda m, x: m.w2(F.relu(m.w1(x)) * m.w3(x)),
+    limited=lambda m, x: m.w2(F.silu(m.w1(x).clamp(max=7)) * m.w3(x)),
+    limited_up=lambda m, x: m.w2(F.silu(m.w1(x)) * m.w3(x).clamp(-7, 7)),
+    plus_one=lambda m, x: m.w2(F.silu(m.w1(x)) * (m.w3(x) + 1)),
+    exchanged=lambda m, x: m.w2(m.w1(x) * F.silu(m.w3(x))),
+    not_gated=lambda m, x: m.w2(F.silu(m.w1(x))),
+    scaled=lambda m, x: 2.5 * m.w2(F.silu(m.w1(x)) * m.w3(x)),
+    skip=lambda m, x: x + m.w2(F.silu(m.w1(x)) * m.w3(x)),
+)
+SAME = dict(
+    sigmoid=lambda m, x: m.w2(m.w1(x) * torch.sigmoid(m.w1(x)) * m.w3(x)),
+    wide=lambda m, x: m.w2((F.silu(m.w1(x).float()) * m.w3(x).float()).to(x.dtype)),
+    module=lambda m, x: m.w2(torch.nn.SiLU()(m.w1(x)) * m.w3(x)),
+)
+
+
+@pytest.mark.parametrize("name", sorted(OTHERS))
+def test_other_functions_are_refused(name):
+    mods = torch.nn.ModuleDict({"1": Expert(1), "4": Another(OTHERS[name])})
+    with pytest.raises(ValueError, match="silu"):
+        ResidentExperts(mods, mask_of((1, 4)), 2, torch.device("cpu"), make_layer=Stacks)
+
+
+@pytest.mark.parametrize("name", sorted(SAME))
+def test_the_same_function_written_otherwise(name):
+    mods = torch.nn.ModuleDict({"1": Expert(1), "4": Another(SAME[name])})
+    before = [p.detach().clone() for p in mods.parameters()]
+    holds(ResidentExperts(mods, mask_of((1, 4)), 2, torch.device("cpu"), make_layer=Stacks), mods, (1, 4))
+    assert all(torch.equal(p, q) for p, q in zip(mods.parameters(), before))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_types_that_the_routing_weights_do_not_have(dtype):
+    mods = torch.nn.ModuleDict({"1": Expert(1, dtype)})
+    with pytest.raises(ValueError, match="bfloat16"):
+        ResidentExperts(mods, mask_of((1,)), 2, torch.device("cpu"), make_layer=Stacks)
+    mods, res = make()
+    mods.half()
+    assert res.current(mods, mask_of((1, 4, 7))) is None
+    mods.bfloat16()
+    holds(res, mods)
+
+
+@pytest.mark.parametrize("change", [own_forward, linear_forward, biased])
+def test_a_function_that_changes(change):
+    mods, res = make()
+    holds(res, mods)
+    change(mods["4"])
+    for _ in range(2):
+        assert res.current(mods, mask_of((1, 4, 7))) is None
+    mods["4"].w2.bias = None
+    for m in (mods["4"], mods["4"].w3):
+        m.__dict__.pop("forward", None)
+    holds(res, mods)
+
+
+@pytest.mark.parametrize("before", [True, False])
+@pytest.mark.parametrize("where", ["expert", "w1", "pre"])
+def test_hooks(where, before):
+    """While there are any the modules are called themselves; nothing else runs them."""
+    mods = torch.nn.ModuleDict({str(n): Expert(n) for n in (1, 4, 7)})
+    seen = []
+
+    def hook():
+        if where == "pre":
+            return mods["4"].register_forward_pre_hook(lambda m, a: seen.append(1))
+        return (mods["4"] if where == "expert" else mods["4"].w1).register_forward_hook(lambda m, a, y: seen.append(1))
+
+    h = hook() if before else None
+    res = ResidentExperts(mods, mask_of((1, 4, 7)), 2, torch.device("cpu"), make_layer=Stacks)
+    h = h or hook()
+    assert res.current(mods, mask_of((1, 4, 7))) is None and res.some
+    assert res.current(mods, mask_of(())) is None and not res.some  # the mask is followed all the same
+    h.remove()
+    holds(res, mods)
+    assert not seen
