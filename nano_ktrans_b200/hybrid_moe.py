@@ -137,7 +137,10 @@ class HybridMoE(nn.Module):
 
         if dense is not None and hidden_states.shape[0] <= DENSE_MAX_TOKENS:
             offloaded = self.offload_backend.sync_forward(hidden_states, stream)
-            return dense.experts_forward(hidden_states, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
+            x = hidden_states
+            if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8) or x.stride(-1) != 1:
+                x = x.clone(memory_format=torch.contiguous_format)  # rows off the kernels' 16-byte boundaries
+            return dense.experts_forward(x, self._dense_slot[topk_ids], topk_weights, residual=offloaded)
 
         final_gpu_states = torch.zeros_like(hidden_states)
         mask_host = self.gpu_experts_mask.bool().cpu().tolist()

@@ -226,3 +226,13 @@ def test_a_capture_finds_changed_weights(codes, cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, moe(x, lg))
+
+
+def test_hidden_states_at_any_alignment(codes, cuda_device):
+    moe = build(codes, modules(cuda_device))
+    x, lg = inputs(5)
+    want = moe(x, lg)
+    for off, width in ((1, H + 3), (8, H + 20), (4, H + 8)):
+        wide = torch.zeros(5, width, dtype=BF16, device=cuda_device)
+        wide[:, off:off + H] = x
+        assert torch.equal(moe(wide[:, off:off + H], lg), want)
