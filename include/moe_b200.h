@@ -422,6 +422,24 @@ typedef struct moe_linear_desc {
 } moe_linear_desc;
 int moe_linear(const moe_linear_desc* desc, void* stream, char* err, size_t err_len);
 
+/* Which kernel a moe_linear call takes on the current device, and its plan; on
+ * a host without a device, on a B200 whose clusters all fit.  Refuses what
+ * moe_linear refuses; launches and reads nothing. */
+enum moe_linear_kernel {
+  MOE_LINEAR_NONE = 0,    /* m == 0 */
+  MOE_LINEAR_GENERIC = 1, /* rows that no 16-byte load can take */
+  MOE_LINEAR_STREAM = 2,  /* a few tokens: weights streamed past them */
+  MOE_LINEAR_SPLIT = 3,   /* tcgen05, one SM per tile, K over a cluster */
+  MOE_LINEAR_PAIR = 4     /* tcgen05, SM pairs */
+};
+typedef struct moe_linear_plan {
+  int32_t kernel;
+  int32_t rows, splits, slices, width, stages; /* of the tcgen05 kernels: token rows and features of a tile, blocks that
+                                                  share K, feature slices, K steps held */
+  int32_t smem_bytes, tmem_columns;            /* of a block */
+} moe_linear_plan;
+int moe_linear_query(const moe_linear_desc* desc, moe_linear_plan* plan, char* err, size_t err_len);
+
 /* ---- A whole expert layer on unquantised weights, for a few tokens ----
  * The reference's MoE block (nano_ktrans/models/mixtral.py:212-218) with
  * GPU-resident bf16 / fp16 experts (layers/hybrid_moe.py:3321-3329, :3442-3533)

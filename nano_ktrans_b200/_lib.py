@@ -17,6 +17,7 @@ MOE_OK, MOE_EINVAL, MOE_ECUDA, MOE_ENOWEIGHTS, MOE_ERANGE, MOE_EDEVICE = range(6
 K_ROUTE, K_PERMUTE, K_GATEUP, K_DOWN, K_COMBINE, K_DECODE_FUSED = range(1, 7)
 DTYPE_BF16, DTYPE_FP16 = 0, 1
 DENSE_MAX_TOKENS = 16
+LINEAR_KERNELS = ("none", "generic", "stream", "split", "pair")
 ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 OPT_DECODE_FUSED, OPT_TRACE, OPT_GEMM, OPT_GEMM_TILE, OPT_STREAM, OPT_HOST_IO = 1, 2, 3, 4, 5, 6
 
@@ -39,6 +40,11 @@ class MoeLinearDesc(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x_dev", "w_dev", "w_up_dev", "bias_dev", "residual_dev", "out_dev")]
                 + [(n, ctypes.c_int64) for n in ("ldx", "ldw", "ldw_up", "ldr", "ldo")]
                 + [(n, ctypes.c_int32) for n in ("m", "n", "k", "dtype", "activation")])
+
+
+class MoeLinearPlan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "rows", "splits", "slices", "width", "stages", "smem_bytes",
+                                              "tmem_columns")]
 
 
 class MoeDenseDesc(ctypes.Structure):
@@ -101,6 +107,7 @@ SIGNATURES = {
     "moe_ep_group_close_peers": (_i32, [_vp]),
     "moe_ep_group_destroy": (_i32, [_vp]),
     "moe_linear": (_i32, [ctypes.POINTER(MoeLinearDesc), _vp, _cp, _sz]),
+    "moe_linear_query": (_i32, [ctypes.POINTER(MoeLinearDesc), ctypes.POINTER(MoeLinearPlan), _cp, _sz]),
     "moe_dense_workspace": (_i32, [ctypes.POINTER(MoeDenseDesc), ctypes.POINTER(ctypes.c_int64), _cp, _sz]),
     "moe_dense_forward": (_i32, [ctypes.POINTER(MoeDenseDesc), _vp, _cp, _sz]),
     "moe_dense_read_status": (_i32, [ctypes.POINTER(_i32), _vp, _cp, _sz]),

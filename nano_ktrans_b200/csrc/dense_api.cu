@@ -41,23 +41,28 @@ int sm_count(int* device = nullptr) {
 }
 
 // A few tokens are bound by the weights' bytes (streaming kernel); more go to
-// the tensor-core GEMMs.  Rows that no 16-byte load can take, to the generic
-// kernel.
+// the tensor-core GEMMs (NONE here: which of them goes by their plans).  Rows that
+// no 16-byte load can take, to the generic kernel.
+int kernel_of(const LinearArgs& a) {
+  if (!moe::dense::wide_rows(a)) return MOE_LINEAR_GENERIC;
+  return a.m <= moe::dense::kStreamTokens ? MOE_LINEAR_STREAM : MOE_LINEAR_NONE;
+}
+
 cudaError_t launch_linear(const LinearArgs& a, int dtype, cudaStream_t st) {
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms < 1) return cudaErrorInvalidDevice;
-  if (!moe::dense::wide_rows(a)) return moe::dense::launch_generic(a, dtype, st);
-  if (a.m <= moe::dense::kStreamTokens) return moe::dense::launch_stream_linear(a, dtype, sms, st);
-  return moe::dense::launch_gemm(a, dtype, dev, sms, st);
+  switch (kernel_of(a)) {
+    case MOE_LINEAR_GENERIC: return moe::dense::launch_generic(a, dtype, st);
+    case MOE_LINEAR_STREAM: return moe::dense::launch_stream_linear(a, dtype, sms, st);
+    default: return moe::dense::launch_gemm(a, dtype, dev, sms, st);
+  }
 }
 
-}  // namespace
+constexpr int kB200Sms = 148;  // for the checks of a call on a host without a device
 
-extern "C" {
-
-int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len) {
-  const char* me = "moe_linear";
+// The description of a projection, checked; what it says, in `a`.
+int read_linear(const char* me, const moe_linear_desc* d, LinearArgs& a, char* err, size_t err_len) {
   if (d == nullptr) return refuse(err, err_len, MOE_EINVAL, "%s: null argument", me);
   if (d->dtype != MOE_DTYPE_BF16 && d->dtype != MOE_DTYPE_FP16)
     return refuse(err, err_len, MOE_EINVAL, "%s: dtype must be MOE_DTYPE_BF16 or MOE_DTYPE_FP16", me);
@@ -87,7 +92,6 @@ int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len
       (d->bias_dev && meet(out, span(d->bias_dev, 1, d->n, d->n))) ||
       (d->residual_dev && !in_place && meet(out, span(d->residual_dev, d->m, d->n, d->ldr))))
     return refuse(err, err_len, MOE_EINVAL, "%s: out overlaps an input (only residual may be out itself)", me);
-  LinearArgs a{};
   a.x = static_cast<const uint16_t*>(d->x_dev);
   a.w = static_cast<const uint16_t*>(d->w_dev);
   a.w_up = static_cast<const uint16_t*>(d->w_up_dev);
@@ -103,15 +107,42 @@ int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len
   a.n = d->n;
   a.k = d->k;
   a.act = d->activation;
-  const cudaError_t e = launch_linear(a, d->dtype, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "%s: %s", me, cudaGetErrorString(e));
   return MOE_OK;
 }
 
+}  // namespace
+
+extern "C" {
+
+int moe_linear(const moe_linear_desc* d, void* stream, char* err, size_t err_len) {
+  LinearArgs a{};
+  const int rc = read_linear("moe_linear", d, a, err, err_len);
+  if (rc != MOE_OK || a.m == 0) return rc;
+  const cudaError_t e = launch_linear(a, d->dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return refuse(err, err_len, MOE_ECUDA, "moe_linear: %s", cudaGetErrorString(e));
+  return MOE_OK;
+}
+
+int moe_linear_query(const moe_linear_desc* d, moe_linear_plan* plan, char* err, size_t err_len) {
+  if (plan == nullptr) return refuse(err, err_len, MOE_EINVAL, "moe_linear_query: null argument");
+  LinearArgs a{};
+  const int rc = read_linear("moe_linear_query", d, a, err, err_len);
+  if (rc != MOE_OK) return rc;
+  *plan = {};
+  if (a.m == 0) return MOE_OK;
+  int dev = -1;
+  int sms = sm_count(&dev);
+  if (sms < 1) {
+    cudaGetLastError();
+    dev = -1;
+    sms = kB200Sms;
+  }
+  plan->kernel = kernel_of(a);
+  if (plan->kernel == MOE_LINEAR_NONE) moe::dense::plan_gemm(a, dev, sms, *plan);
+  return MOE_OK;
+}
 
 namespace {
-
-constexpr int kB200Sms = 148;  // for the checks of a call on a host without a device
 
 struct MoeSpace {
   size_t bar, open, logits, partial, bytes;

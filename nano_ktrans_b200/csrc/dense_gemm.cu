@@ -503,6 +503,7 @@ struct SplitPlan {
   int box_x;    // token rows loaded per stage
   int stages;
   int smem;
+  int tmem;     // columns of tensor memory
   int wide;     // out and residual rows allow 16-byte accesses
 };
 constexpr int kQThreads = 320;  // producer, MMA, 8 epilogue warps
@@ -594,8 +595,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
   const int cols = GATED ? 2 * p.width : p.width;  // the MMA's N
   const int row_tiles = (valid + 127) / 128;
   const int x_bytes = p.box_x * 128, stage_bytes = x_bytes + cols * 128;
-  const uint32_t need = static_cast<uint32_t>((p.rows / 128) * cols);
-  const uint32_t tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+  const uint32_t tmem_cols = static_cast<uint32_t>(p.tmem);
 
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -905,7 +905,8 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
         const double t = real_waves * (steps * (load > mma ? load : mma) + join + 3000.0);
         if (t < clocks) {
           clocks = t;
-          best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem), 0};
+          const int need = rows / 128 * cols, tmem = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+          best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem), tmem, 0};
         }
       }
     }
@@ -976,15 +977,21 @@ cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, pair_gemm_kernel<T, GATED>, tx, tw, tu, a, wide);
 }
 
-template <typename T, bool GATED>
-cudaError_t gemm(const LinearArgs& a, int dev, int sms, cudaStream_t st) {
+// Whether the split kernel takes a projection, and then its plan.
+bool takes_split(const LinearArgs& a, int dev, int sms, SplitPlan& p) {
   double split_clocks = 0;
-  const SplitPlan p = plan_split(a, dev, sms, split_clocks);
-  const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
+  p = plan_split(a, dev, sms, split_clocks);
+  const int wide = a.w_up != nullptr ? 128 : 256;
+  const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + wide - 1) / wide);
   const int pairs = sms / 2, nk = (a.k + kBK - 1) / kBK;
   const double pair_clocks = static_cast<double>((tiles + pairs - 1) / pairs) * nk * 600.0 + 8000.0;
-  if (split_clocks < pair_clocks) return launch_split<T, GATED>(a, p, st);
-  return launch_pair<T, GATED>(a, sms, st);
+  return split_clocks < pair_clocks;
+}
+
+template <typename T, bool GATED>
+cudaError_t gemm(const LinearArgs& a, int dev, int sms, cudaStream_t st) {
+  SplitPlan p;
+  return takes_split(a, dev, sms, p) ? launch_split<T, GATED>(a, p, st) : launch_pair<T, GATED>(a, sms, st);
 }
 
 }  // namespace
@@ -992,6 +999,15 @@ cudaError_t gemm(const LinearArgs& a, int dev, int sms, cudaStream_t st) {
 cudaError_t launch_gemm(const LinearArgs& a, int dtype, int dev, int sms, cudaStream_t st) {
   if (dtype == MOE_DTYPE_FP16) return a.w_up ? gemm<Fp16, true>(a, dev, sms, st) : gemm<Fp16, false>(a, dev, sms, st);
   return a.w_up ? gemm<Bf16, true>(a, dev, sms, st) : gemm<Bf16, false>(a, dev, sms, st);
+}
+
+void plan_gemm(const LinearArgs& a, int dev, int sms, moe_linear_plan& out) {
+  SplitPlan p;
+  if (takes_split(a, dev, sms, p)) {
+    out = {MOE_LINEAR_SPLIT, p.rows, p.splits, p.slices, p.width, p.stages, p.smem, p.tmem};
+  } else {
+    out = {MOE_LINEAR_PAIR, 256, 1, 1, a.w_up != nullptr ? 128 : 256, kPStages, static_cast<int>(kPSmem), 512};
+  }
 }
 
 cudaError_t read_gemm_status(int* status, cudaStream_t st) {
