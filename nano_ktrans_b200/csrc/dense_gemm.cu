@@ -37,6 +37,13 @@ namespace {
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kBK = 64;                 // K elements per stage: one 128-byte swizzled row
 constexpr size_t kSmemLimit = 232448;
+// A block of a cluster holds tensor memory while it waits for the cluster's
+// other blocks, so it must never wait for some itself: two such blocks of two
+// clusters could wait for each other for good.  It therefore takes shared memory
+// in proportion, 512 columns all of it, and the blocks of clusters that an SM can
+// hold never come to more than its 512 columns, whatever calls they belong to.
+// (Blocks without a cluster may have to wait, but nothing waits in them.)
+constexpr size_t kTmemShare = (kSmemLimit - 512) / 512;  // bytes a column
 
 MOE_DEV uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 MOE_DEV void mbar_init(uint32_t bar, uint32_t count) {
@@ -227,7 +234,8 @@ constexpr int kPTurnOff = kPBarOff + 8 * (2 * kPStages + 4) + 16;  // 32 rows x 
 constexpr int kPTurnRow = 17;
 constexpr size_t kPSmem = kPTurnOff + 4 * 32 * kPTurnRow * sizeof(float) + 1024;
 constexpr int kPThreads = 256;
-static_assert(kPSmem <= kSmemLimit, "shared-memory plan");
+constexpr size_t kPTake = 512 * kTmemShare;  // what a block asks for
+static_assert(kPSmem <= kPTake && kPTake <= kSmemLimit, "shared-memory plan");
 
 // Residual of 64 columns of a row, read well ahead of the sums it joins: a read
 // per 16 columns when they are stored waits out a memory latency each time
@@ -898,7 +906,7 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
         if (stages > 16) stages = 16;
         if (stages > steps) stages = steps;
         if (stages < steps && stages < 3) continue;
-        const int64_t smem = static_cast<int64_t>(stages) * stage + part + kQTail;
+        int64_t smem = static_cast<int64_t>(stages) * stage + part + kQTail;
         const double load = stage / 50.0, mma = 2.0 * cols * (box > 128 ? 2 : 1);
         const double items = (valid + 31) / 32 * ((width + 7) / 8) * mul / 8.0;  // 32 rows x 8 columns a warp
         const double join = splits > 1 ? 2500.0 + 90.0 * items + 60.0 * items : 110.0 * items;
@@ -906,6 +914,7 @@ SplitPlan plan_split(const LinearArgs& a, int dev, int sms, double& clocks) {
         if (t < clocks) {
           clocks = t;
           const int need = rows / 128 * cols, tmem = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+          if (splits > 1 && smem < static_cast<int64_t>(tmem * kTmemShare)) smem = static_cast<int64_t>(tmem * kTmemShare);
           best = SplitPlan{rows, splits, slices, width, box, stages, static_cast<int>(smem), tmem, 0};
         }
       }
@@ -961,13 +970,13 @@ cudaError_t launch_pair(const LinearArgs& a, int sms, cudaStream_t st) {
                       row_stride(GATED ? a.ldwu : a.ldw, a.n, a.k), 128))
     return cudaErrorInvalidValue;
   const void* kern = reinterpret_cast<const void*>(pair_gemm_kernel<T, GATED>);
-  if (!ensure_dynamic_smem(kern, kPSmem, kPThreads)) return cudaErrorInvalidConfiguration;
+  if (!ensure_dynamic_smem(kern, kPTake, kPThreads)) return cudaErrorInvalidConfiguration;
   const int wide = wide_output(a);
   const int64_t tiles = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + (GATED ? 127 : 255)) / (GATED ? 128 : 256));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < sms / 2 ? tiles : sms / 2));
   cfg.blockDim = dim3(kPThreads);
-  cfg.dynamicSmemBytes = kPSmem;
+  cfg.dynamicSmemBytes = kPTake;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1006,7 +1015,7 @@ void plan_gemm(const LinearArgs& a, int dev, int sms, moe_linear_plan& out) {
   if (takes_split(a, dev, sms, p)) {
     out = {MOE_LINEAR_SPLIT, p.rows, p.splits, p.slices, p.width, p.stages, p.smem, p.tmem};
   } else {
-    out = {MOE_LINEAR_PAIR, 256, 1, 1, a.w_up != nullptr ? 128 : 256, kPStages, static_cast<int>(kPSmem), 512};
+    out = {MOE_LINEAR_PAIR, 256, 1, 1, a.w_up != nullptr ? 128 : 256, kPStages, static_cast<int>(kPTake), 512};
   }
 }
 

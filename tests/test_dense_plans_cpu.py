@@ -41,3 +41,45 @@ def test_refusals():
     assert L.moe_linear_query(ctypes.byref(d), ctypes.byref(out), err, 256) == _lib.MOE_EINVAL and b"n and k" in err.value
     assert L.moe_linear_query(ctypes.byref(d), None, err, 256) == _lib.MOE_EINVAL
     assert L.moe_linear_query(None, ctypes.byref(out), None, 0) == _lib.MOE_EINVAL
+
+
+# An SM's shared memory; what a block is charged beside its dynamic part: 1024 reserved, and static variables
+SM_BYTES, BLOCK_BYTES = 233472, 1024 + 256
+
+
+def clusters():
+    """Plans whose blocks wait for one another, over the whole range of sizes."""
+    ms = [33, 40, 64, 80, 100, 128, 129, 136, 200, 256, 257, 333, 600, 1024, 3000]
+    ns = [1, 16, 24, 100, 256, 330, 768, 1001, 1408, 2048, 4096, 5000, 9738, 17326, 151936]
+    ks = [40, 72, 128, 200, 264, 512, 520, 1024, 1408, 2048, 4096, 14336]
+    out = {}
+    for gated in (False, True):
+        for m in ms:
+            for n in ns:
+                for k in ks:
+                    p = dp.plan(m, n, k, gated)
+                    if p["kernel"] == "pair" or (p["kernel"] == "split" and p["splits"] > 1):
+                        out[(p["tmem_columns"], p["smem_bytes"])] = (m, n, k, gated, p)
+    return out
+
+
+def test_blocks_that_wait_for_one_another_never_wait_for_tensor_memory():
+    """Blocks of clusters that fit an SM together by their shared memory, of the same or of different calls, ask for at
+    most the 512 columns that it has: otherwise one could hold some and wait for a block that waits for them."""
+    found = clusters()
+    assert {t for t, _ in found} == {32, 64, 128, 256, 512} and any(v[4]["kernel"] == "pair" for v in found.values())
+    for (columns, smem), case in found.items():
+        # in proportion: blocks of more than 512 columns, in steps of 32, together exceed the SM
+        assert (smem + BLOCK_BYTES) * 544 > SM_BYTES * columns, case
+        assert smem + 272 <= 232448, case
+    least = {}
+    for columns, smem in found:
+        least[columns] = min(smem, least.get(columns, smem))
+
+    def fill(columns, room):
+        for c, smem in least.items():
+            if smem + BLOCK_BYTES <= room:
+                assert columns + c <= 512, (columns, c, least)
+                fill(columns + c, room - smem - BLOCK_BYTES)
+
+    fill(0, SM_BYTES)
