@@ -23,15 +23,28 @@ int refuse(char* buf, size_t len, int code, const char* f, ...) {
   return code;
 }
 
-// Bytes [lo, hi) that `rows` rows of `cols` 16-bit elements, `ld` apart, lie in.
+// `rows` rows of `cols` 16-bit elements, `ld` elements apart: bytes [lo, hi) hold
+// them, in pieces of `row` bytes `step` apart.
 struct Span {
   uintptr_t lo, hi;
+  uintptr_t row, step;  // step 0: one piece
 };
 Span span(const void* p, int64_t rows, int64_t cols, int64_t ld) {
   const uintptr_t b = reinterpret_cast<uintptr_t>(p);
-  return {b, rows > 0 ? b + 2 * static_cast<uintptr_t>((rows - 1) * ld + cols) : b};
+  return {b, rows > 0 ? b + 2 * static_cast<uintptr_t>((rows - 1) * ld + cols) : b, 2 * static_cast<uintptr_t>(cols),
+          rows > 1 ? 2 * static_cast<uintptr_t>(ld) : 0};
 }
-bool meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Whether they have a byte in common.  Two column ranges of one buffer have not,
+// though each lies between the other's first and last byte; rows of two different
+// steps are taken to meet where their whole extents do.
+bool meet(const Span& a, const Span& b) {
+  if (!(a.lo < b.hi && b.lo < a.hi)) return false;
+  const uintptr_t step = a.step ? a.step : b.step;
+  if (step == 0 || (a.step && b.step && a.step != b.step)) return true;
+  // where b's pieces start between two of a's: they fit if they end before the next one
+  const uintptr_t off = b.lo >= a.lo ? (b.lo - a.lo) % step : (step - (a.lo - b.lo) % step) % step;
+  return off < a.row || off + b.row > step;
+}
 
 int sm_count(int* device = nullptr) {
   int dev = 0, sms = 0;
@@ -237,19 +250,20 @@ int moe_dense_forward(const moe_dense_desc* d, void* stream, char* err, size_t e
   // read no more once the first output is stored) or residual.
   const auto whole = [](const void* p, int64_t n, int64_t bytes_each) {
     const uintptr_t b = reinterpret_cast<uintptr_t>(p);
-    return p ? Span{b, b + static_cast<uintptr_t>(n * bytes_each)} : Span{0, 0};
+    const uintptr_t size = static_cast<uintptr_t>(n * bytes_each);
+    return p ? Span{b, b + size, size, 0} : Span{};
   };
   const Span x = span(d->x_dev, t, H, d->ldx), out = span(d->out_dev, t, H, d->ldo);
-  const Span res = d->residual_dev ? span(d->residual_dev, t, H, d->ldr) : Span{0, 0};
+  const Span res = d->residual_dev ? span(d->residual_dev, t, H, d->ldr) : Span{};
   const Span lg = whole(d->logits_dev, t * E, 2);
   const Span written[] = {out, whole(d->workspace_dev, ws.bytes, 1), whole(d->ids_out_dev, t * d->top_k, 8),
-                          whole(d->weights_out_dev, t * d->top_k, 2), d->router_w_dev ? lg : Span{0, 0}};
+                          whole(d->weights_out_dev, t * d->top_k, 2), d->router_w_dev ? lg : Span{}};
   const Span read[] = {x, res, whole(d->gate_dev, E * I * H, 2), whole(d->up_dev, E * I * H, 2),
                        whole(d->down_dev, E * I * H, 2), whole(shared ? d->shared_gate_dev : nullptr, S * H, 2),
                        whole(shared ? d->shared_up_dev : nullptr, S * H, 2),
                        whole(shared ? d->shared_down_dev : nullptr, S * H, 2),
                        whole(shared ? d->shared_gate_vec_dev : nullptr, H, 2), whole(d->router_w_dev, E * H, 2),
-                       d->router_w_dev ? Span{0, 0} : lg, whole(d->ids_dev, t * d->top_k, 8),
+                       d->router_w_dev ? Span{} : lg, whole(d->ids_dev, t * d->top_k, 8),
                        whole(d->weights_dev, t * d->top_k, 2), whole(d->offload_mask_dev, E, 1)};
   const bool on_x = d->out_dev == d->x_dev && (t == 1 || d->ldo == d->ldx);
   const bool on_res = d->out_dev == d->residual_dev && (t == 1 || d->ldo == d->ldr);
