@@ -505,8 +505,9 @@ typedef struct moe_dense_desc {
 int moe_dense_workspace(const moe_dense_desc* desc, int64_t* bytes, char* err, size_t err_len);
 int moe_dense_forward(const moe_dense_desc* desc, void* stream, char* err, size_t err_len);
 /* Copy the current device's status word of the dense calls (moe_linear and
- * moe_dense_forward; bits as moe_read_status) to *status and clear it;
- * synchronises `stream`. */
+ * moe_dense_forward; bits as moe_read_status) to *status and clear the bits that
+ * were read; synchronises `stream`.  The word is one for all dense calls on the
+ * device: who reads it takes every caller's reports. */
 int moe_dense_read_status(int32_t* status, void* stream, char* err, size_t err_len);
 
 #ifdef __cplusplus

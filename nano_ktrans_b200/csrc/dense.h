@@ -37,6 +37,8 @@ cudaError_t launch_stream_linear(const LinearArgs& a, int dtype, int sms, cudaSt
 cudaError_t launch_gemm(const LinearArgs& a, int dtype, int dev, int sms, cudaStream_t st);
 // Which of them, on a device of `sms` SMs (dev < 0: none at hand, every cluster is taken to fit).
 void plan_gemm(const LinearArgs& a, int dev, int sms, moe_linear_plan& out);
+// Copy a status word to the host and clear the bits that were copied; waits for `st`.
+cudaError_t take_status(const void* symbol, int* status, cudaStream_t st);
 cudaError_t read_gemm_status(int* status, cudaStream_t st);
 
 // A whole expert layer for up to kMoeTokens tokens.

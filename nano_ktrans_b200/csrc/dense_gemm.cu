@@ -1019,14 +1019,20 @@ void plan_gemm(const LinearArgs& a, int dev, int sms, moe_linear_plan& out) {
   }
 }
 
-cudaError_t read_gemm_status(int* status, cudaStream_t st) {
+__global__ void clear_bits_kernel(int* word, int bits) { atomicAnd(word, ~bits); }
+
+// Only what was read is cleared: a kernel of another stream may set a bit meanwhile.
+cudaError_t take_status(const void* symbol, int* status, cudaStream_t st) {
   void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, g_gemm_status);
+  cudaError_t e = cudaGetSymbolAddress(&p, symbol);
   if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  return e;
+  if (e != cudaSuccess || *status == 0) return e;
+  clear_bits_kernel<<<1, 1, 0, st>>>(static_cast<int*>(p), *status);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
 }
+cudaError_t read_gemm_status(int* status, cudaStream_t st) { return take_status(&g_gemm_status, status, st); }
 
 }  // namespace dense
 }  // namespace moe

@@ -772,14 +772,7 @@ cudaError_t launch_dense_moe(MoeArgs a, int dtype, int sms, cudaStream_t st) {
   return dtype == MOE_DTYPE_FP16 ? moe_both<Fp16>(a, sms, st) : moe_both<Bf16>(a, sms, st);
 }
 
-cudaError_t read_dense_status(int* status, cudaStream_t st) {
-  void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, g_dense_status);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  return e;
-}
+cudaError_t read_dense_status(int* status, cudaStream_t st) { return take_status(&g_dense_status, status, st); }
 
 }  // namespace dense
 }  // namespace moe
