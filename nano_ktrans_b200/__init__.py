@@ -8,7 +8,7 @@ Public API (mirrors the reference's names):
 * ``HybridMoE`` — the MoE layer using it
 * ``MoeLayer`` — direct access to the C-ABI handle (route / experts / fused forward)
 * ``linear``, ``gated_linear``, ``DenseMLP`` — unquantised (bf16 / fp16) projections with their
-  bias, activation, gating and residual in the same kernel
+  bias, activation, gating and residual in the same kernel; ``read_dense_status``
 * ``DenseMoeLayer`` — a whole expert layer on unquantised weights for a few tokens: router
   projection, routing, experts, shared expert and residual in two kernels
 * ``EpMoeLayer``, ``plan_placement``, ``shard_layer``, ``TorchDistComm``,
@@ -23,6 +23,7 @@ __all__ = [
     "quantize_symmetric", "stack_layer", "CudaMoEBackend", "HybridMoE", "MoeLayer",
     "EpMoeLayer", "plan_placement", "shard_layer", "TorchDistComm", "PeerExchange",
     "linear", "gated_linear", "DenseMLP", "DenseMoeLayer", "stack_expert_modules",
+    "read_dense_status",
 ]
 
 
@@ -31,7 +32,7 @@ _MODULES = {
     "EpMoeLayer": "expert_parallel", "plan_placement": "expert_parallel", "shard_layer": "expert_parallel",
     "TorchDistComm": "expert_parallel", "PeerExchange": "expert_parallel",
     "linear": "dense", "gated_linear": "dense", "DenseMLP": "dense", "DenseMoeLayer": "dense_moe",
-    "stack_expert_modules": "dense_moe",
+    "stack_expert_modules": "dense_moe", "read_dense_status": "dense",
 }
 
 

@@ -35,8 +35,6 @@ def _moe_linear():
     return _entry
 
 
-
-
 def _err_buffer():
     buf = getattr(_tls, "err", None)
     if buf is None:
@@ -140,6 +138,21 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
                  stream=None) -> torch.Tensor:
     """``act(x @ gate_weight.T) * (x @ up_weight.T)``, rounded once: the first half of a gated MLP."""
     return _project(x, gate_weight, up_weight, None, activation, None, out, stream)
+
+
+def read_dense_status(device=None, stream=None) -> int:
+    """Status bits (as ``MoeLayer.read_status``) of the dense calls on a device (the current one) since the last read,
+    whichever operator or layer made them and whoever reads; synchronises the stream."""
+    dev = torch.device("cuda" if device is None else device) if not isinstance(device, int) else torch.device("cuda", device)
+    if dev.type != "cuda":
+        raise ValueError(f"the dense operators run on CUDA devices, not on {dev}")
+    st, err = ctypes.c_int32(0), _err_buffer()
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    with torch.cuda.device(index):
+        rc = _lib.lib().moe_dense_read_status(ctypes.byref(st), _stream_on(index, stream), err, 512)
+    if rc != _lib.MOE_OK:
+        raise _lib.MoeError(rc, err.value.decode(errors="replace"))
+    return int(st.value)
 
 
 class DenseMLP:

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .dense import _DTYPES, _empty_on, _err_buffer, _stream_on
+from .dense import _DTYPES, _empty_on, _err_buffer, _stream_on, read_dense_status
 
 MAX_TOKENS = _lib.DENSE_MAX_TOKENS
 
@@ -209,13 +209,8 @@ class DenseMoeLayer:
     __call__ = forward
 
     def read_status(self, stream=None) -> int:
-        """Status bits (as ``MoeLayer.read_status``) of the device's dense calls since the last read; synchronises."""
-        st, err = ctypes.c_int32(0), _err_buffer()
-        with torch.cuda.device(self._dev):
-            rc = _lib.lib().moe_dense_read_status(ctypes.byref(st), _stream_on(self._dev, stream), err, 512)
-        if rc != _lib.MOE_OK:
-            raise _lib.MoeError(rc, err.value.decode(errors="replace"))
-        return int(st.value)
+        """``read_dense_status`` of the layer's device."""
+        return read_dense_status(self._dev, stream)
 
 
 def _version(t: torch.Tensor) -> int:

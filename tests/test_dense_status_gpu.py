@@ -35,3 +35,17 @@ def test_nothing_is_lost_to_a_read_at_the_same_time(cuda_device):
         lost += (seen | layer.read_status()) != 1
     assert lost == 0, f"{lost} of 4000 reports lost"
     assert layer.read_status() == 0
+
+
+def test_read_without_a_layer(cuda_device):
+    from nano_ktrans_b200 import read_dense_status
+
+    layer, x, w = small_layer(cuda_device)
+    assert read_dense_status() == 0
+    layer.experts_forward(x, torch.full((1, 1), 5, device=cuda_device), w)
+    assert read_dense_status(cuda_device) == 1 and read_dense_status(torch.device("cuda")) == 0
+    side = torch.cuda.Stream()
+    layer.experts_forward(x, torch.full((1, 1), 5, device=cuda_device), w, stream=side)
+    assert read_dense_status(cuda_device, stream=side) == 1 and layer.read_status() == 0
+    with pytest.raises(ValueError, match="CUDA"):
+        read_dense_status(torch.device("cpu"))
