@@ -398,8 +398,9 @@ int moe_decode_noalloc(const moe_layer_desc* desc, const moe_weights* w, const u
  * elements from row to row; bias and residual may be NULL.  Sums are fp32,
  * the result is rounded once.  residual_dev == out_dev (same ldr) adds in
  * place; any other overlap of out with an input is refused.  m == 0 is a
- * no-op.  Any alignment of 2 bytes is accepted; rows on 16-byte boundaries
- * with k a multiple of 8 take the fast kernels. */
+ * no-op.  m, n and k are at most 2^31 - 256.  Any alignment of 2 bytes is
+ * accepted; rows on 16-byte boundaries with k a multiple of 8 take the fast
+ * kernels. */
 enum moe_dtype { MOE_DTYPE_BF16 = 0, MOE_DTYPE_FP16 = 1 };
 enum moe_activation {
   MOE_ACT_NONE = 0,

@@ -83,6 +83,10 @@ int read_linear(const char* me, const moe_linear_desc* d, LinearArgs& a, char* e
     return refuse(err, err_len, MOE_EINVAL, "%s: unknown activation %d", me, d->activation);
   if (d->m < 0 || d->n < 1 || d->k < 1)
     return refuse(err, err_len, MOE_EINVAL, "%s: m must be >= 0, n and k >= 1 (got %d, %d, %d)", me, d->m, d->n, d->k);
+  // a tile's last row and column number, up to 255 beyond the tensor's, have to fit 32 bits
+  const int32_t most = INT32_MAX - 255;
+  if (d->m > most || d->n > most || d->k > most)
+    return refuse(err, err_len, MOE_EINVAL, "%s: m, n and k are at most 2^31 - 256 (got %d, %d, %d)", me, d->m, d->n, d->k);
   if (d->m == 0) return MOE_OK;
   if (d->x_dev == nullptr || d->w_dev == nullptr || d->out_dev == nullptr)
     return refuse(err, err_len, MOE_EINVAL, "%s: null device pointer", me);

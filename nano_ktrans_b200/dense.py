@@ -21,6 +21,7 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
+_MOST = 2 ** 31 - 256  # the description's sizes are 32 bits: a larger one would arrive as another
 _tls = threading.local()
 _Desc = _lib.MoeLinearDesc
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -92,6 +93,8 @@ def _project(x, weight, up, bias, activation, residual, out, stream) -> torch.Te
     ldw = _row_stride(weight, "weight" if up is None else "gate_weight", n, k, dtype, dev)
     if n < 1 or k < 1:
         raise ValueError(f"empty weight {tuple(weight.shape)}")
+    if m > _MOST or n > _MOST or k > _MOST:
+        raise ValueError(f"m, n and k are at most {_MOST}, got {m}, {n}, {k}")
     up_ptr = bias_ptr = res_ptr = None
     ldu = ldr = 0
     if up is not None:

@@ -145,7 +145,8 @@ class DenseMoeLayer:
         ldx = self._rows(x, "x", None, self.hidden_size)
         t = x.shape[0]
         d = _lib.MoeDenseDesc.from_buffer_copy(self._layer_bytes)
-        d.x_dev, d.ldx, d.num_tokens, d.add_shared = x.data_ptr(), ldx, t, add_shared
+        # a count above the limit is refused, whatever its low 32 bits
+        d.x_dev, d.ldx, d.num_tokens, d.add_shared = x.data_ptr(), ldx, min(t, MAX_TOKENS + 1), add_shared
         if router is not None:
             d.router_w_dev = self._exact(router, "router_weight", (self.num_experts, self.hidden_size), self.dtype)
         if logits is not None:

@@ -83,3 +83,22 @@ def test_blocks_that_wait_for_one_another_never_wait_for_tensor_memory():
                 fill(columns + c, room - smem - BLOCK_BYTES)
 
     fill(0, SM_BYTES)
+
+
+MOST = (1 << 31) - 256
+
+
+@pytest.mark.parametrize("name", ["m", "n", "k"])
+def test_sizes_whose_tiles_leave_32_bits(name):
+    """Row and column numbers are 32 bits in the kernels, a tile's last ones beyond the tensor's end included."""
+    from nano_ktrans_b200 import _lib
+
+    L, err, out = _lib.lib(), ctypes.create_string_buffer(256), _lib.MoeLinearPlan()
+    for size, code in ((MOST, _lib.MOE_OK), (MOST + 1, _lib.MOE_EINVAL), ((1 << 31) - 1, _lib.MOE_EINVAL)):
+        d = dict(m=1, n=8, k=8, x_dev=1 << 50, w_dev=1 << 51, out_dev=1 << 52)
+        d[name] = size
+        d.update(ldx=d["k"], ldw=d["k"], ldo=d["n"])
+        for rows in (1, 33) if name != "m" else (size,):
+            d["m"] = rows
+            assert L.moe_linear_query(ctypes.byref(_lib.MoeLinearDesc(**d)), ctypes.byref(out), err, 256) == code, err.value
+            assert code == _lib.MOE_OK or b"2^31 - 256" in err.value
