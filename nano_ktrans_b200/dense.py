@@ -24,7 +24,7 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _MOST = 2 ** 31 - 256  # the description's sizes are 32 bits: a larger one would arrive as another
 _tls = threading.local()
 _Desc = _lib.MoeLinearDesc
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a torch built without CUDA has none
 _entry = None
 
 
@@ -45,14 +45,14 @@ def _err_buffer():
 
 def _stream_on(device_index: int, stream) -> int:
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device_index)
+        return _raw_stream(device_index)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _empty_on(shape, dtype, device, stream) -> torch.Tensor:
     """A new tensor that belongs to the stream the kernels run on: allocated for another
     stream, its memory could be handed out again while they still write it."""
-    if stream is None or _stream_on(device.index, stream) == torch._C._cuda_getCurrentRawStream(device.index):
+    if stream is None or _stream_on(device.index, stream) == _raw_stream(device.index):
         return torch.empty(shape, dtype=dtype, device=device)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
