@@ -51,10 +51,15 @@ def stack_expert_modules(modules) -> tuple:
         raise ValueError("the experts differ in size, type or device: one stack cannot hold them")
     if len({id(w) for ws in weights for w in ws}) < 3 * len(weights):
         raise ValueError("two experts share a weight: it cannot be a view of two places")
-    stacks = tuple(torch.stack([ws[j].detach() for ws in weights]).contiguous() for j in range(3))
-    for e, ws in enumerate(weights):
-        for j in range(3):
-            ws[j].data = stacks[j][e]
+    # Copies that autocast leaves alone, into tensors that autograd may use: the parameters become views of them.
+    with torch.inference_mode(False), torch.no_grad():
+        stacks = tuple(torch.empty(len(weights), *w.shape, dtype=w.dtype, device=w.device) for w in weights[0])
+        for e, ws in enumerate(weights):
+            for stack, w in zip(stacks, ws):
+                stack[e].copy_(w)
+        for e, ws in enumerate(weights):
+            for stack, w in zip(stacks, ws):
+                w.data = stack[e]
     return stacks
 
 
@@ -233,8 +238,9 @@ def _shows_silu(module, layers) -> bool:
     down = torch.eye(hidden, inter, dtype=w.dtype, device=w.device)
     x = torch.zeros(3, hidden, dtype=w.dtype, device=w.device)
     x[0, 0], x[1, 0] = 1.0, -1.0
-    with torch.no_grad():
-        out = torch.func.functional_call(module, {f"{names[p]}.weight": v for p, v in zip(layers, (gate, up, down))}, (x,))
+    probe = {f"{names[p]}.weight": v for p, v in zip(layers, (gate, up, down))}
+    with torch.no_grad(), torch.autocast(w.device.type, enabled=False):
+        out = torch.func.functional_call(module, probe, (x,))
     n = min(hidden, inter)
     g, u = gate[:n, 0].double(), up[:n, 0].double()
     want = torch.zeros(3, hidden, dtype=torch.float64, device=w.device)

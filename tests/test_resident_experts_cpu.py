@@ -277,3 +277,29 @@ def test_hooks(where, before):
     h.remove()
     holds(res, mods)
     assert not seen
+
+
+@pytest.mark.parametrize("at", ["built", "stacked anew"])
+def test_stacking_in_inference_mode(at):
+    """It leaves the parameters what they were: usable by autograd afterwards."""
+    mods = torch.nn.ModuleDict({str(n): Expert(n) for n in (1, 4, 7)})
+    if at == "built":
+        with torch.inference_mode():
+            res = ResidentExperts(mods, mask_of((1, 4, 7)), 2, torch.device("cpu"), make_layer=Stacks)
+    else:
+        res = ResidentExperts(mods, mask_of((1, 4, 7)), 2, torch.device("cpu"), make_layer=Stacks)
+        with torch.inference_mode():
+            data(mods)
+            res.current(mods, mask_of((1, 4, 7)))
+    holds(res, mods)
+    assert not any(p.is_inference() for p in mods["1"].parameters())
+    mods["1"](torch.ones(2, H, dtype=torch.bfloat16)).sum().backward()
+    assert mods["1"].w1.weight.grad is not None
+    holds(res, mods)
+
+
+def test_stacking_under_autocast():
+    mods = torch.nn.ModuleDict({str(n): Expert(n) for n in (1, 4, 7)})
+    with torch.autocast("cpu", dtype=torch.float16):
+        res = ResidentExperts(mods, mask_of((1, 4, 7)), 2, torch.device("cpu"), make_layer=Stacks)
+    holds(res, mods)
