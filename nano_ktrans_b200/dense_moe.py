@@ -240,7 +240,10 @@ def _shows_silu(module, layers) -> bool:
     x[0, 0], x[1, 0] = 1.0, -1.0
     probe = {f"{names[p]}.weight": v for p, v in zip(layers, (gate, up, down))}
     with torch.no_grad(), torch.autocast(w.device.type, enabled=False):
-        out = torch.func.functional_call(module, probe, (x,))
+        try:
+            out = torch.func.functional_call(module, probe, (x,))
+        except Exception:  # whatever a module makes of a call that it does not take
+            return False
     n = min(hidden, inter)
     g, u = gate[:n, 0].double(), up[:n, 0].double()
     want = torch.zeros(3, hidden, dtype=torch.float64, device=w.device)

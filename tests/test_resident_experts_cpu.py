@@ -303,3 +303,15 @@ def test_stacking_under_autocast():
     with torch.autocast("cpu", dtype=torch.float16):
         res = ResidentExperts(mods, mask_of((1, 4, 7)), 2, torch.device("cpu"), make_layer=Stacks)
     holds(res, mods)
+
+
+def test_a_module_that_takes_no_such_call():
+    def fails(m, x):
+        raise RuntimeError("not like this")
+
+    mods = torch.nn.ModuleDict({"1": Expert(1), "4": Another(fails)})
+    with pytest.raises(ValueError, match="silu"):
+        ResidentExperts(mods, mask_of((1, 4)), 2, torch.device("cpu"), make_layer=Stacks)
+    mods, res = make()
+    mods["4"] = Another(fails)
+    assert res.current(mods, mask_of((1, 4, 7))) is None
