@@ -123,7 +123,8 @@ class DenseMoeLayer:
                 if rc != _lib.MOE_OK:
                     raise _lib.MoeError(rc, err.value.decode(errors="replace"))
                 space.append(n.value)
-        self._at, self._space, self._layer_bytes = at, space, bytes(desc)
+        self._space, self._layer_bytes = space, bytes(desc)
+        self._at = at  # last: what another thread compares before it uses the others
 
     # ------------------------------------------------------------------
     def _rows(self, t: torch.Tensor, name: str, rows: Optional[int], cols: int) -> int:

@@ -79,3 +79,24 @@ def test_a_weight_whose_memory_is_gone(cuda_device):
     storage.resize_(size)
     bank.gate.data.copy_(keep)
     assert torch.equal(layer.forward_x(x, wr), want)
+
+
+def test_two_threads_while_a_weight_moves(cuda_device):
+    """What a call compares is set after what it then uses, so that a call of another thread meets a whole description."""
+    from nano_ktrans_b200 import DenseMoeLayer
+
+    order = []
+
+    class Seen(DenseMoeLayer):
+        def __setattr__(self, name, value):
+            order.append(name)
+            super().__setattr__(name, value)
+
+    bank = Bank(1)
+    layer = Seen(bank.gate, bank.up, bank.down, top_k=K)
+    x, wr = inputs(2)
+    bank.up.data = bank.up.data.clone()
+    order.clear()
+    out = layer.forward_x(x, wr)
+    assert order[-1] == "_at" and {"_space", "_layer_bytes", "dtype"} <= set(order)
+    assert torch.equal(out, DenseMoeLayer(bank.gate, bank.up, bank.down, top_k=K).forward_x(x, wr))
