@@ -100,7 +100,8 @@ class CudaMoEBackend(ExpertOffloadBackend):
             raise ValueError("CudaMoEBackend.submit_forward needs CUDA hidden states")
         x = flat if flat.dtype == torch.bfloat16 else flat.to(torch.bfloat16)
         stream = cuda_stream if cuda_stream is not None else torch.cuda.current_stream(flat.device).cuda_stream
-        out = self.layer.experts_forward(x, topk_ids.view(x.shape[0], -1), topk_weights.view(x.shape[0], -1),
+        shape = (x.shape[0], -1 if x.shape[0] else self.top_k)  # nothing tells the last dimension of no elements
+        out = self.layer.experts_forward(x, topk_ids.view(shape), topk_weights.view(shape),
                                          offload_mask=self._offload_mask_dev, stream=stream)
         self.last_launches = self.layer.last_launch_count()
         ev = torch.cuda.Event()

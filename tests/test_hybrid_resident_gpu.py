@@ -236,3 +236,23 @@ def test_hidden_states_at_any_alignment(codes, cuda_device):
         wide = torch.zeros(5, width, dtype=BF16, device=cuda_device)
         wide[:, off:off + H] = x
         assert torch.equal(moe(wide[:, off:off + H], lg), want)
+
+
+@pytest.mark.parametrize("resident", ["dense", "modules", "kernels"])
+def test_no_tokens(resident, codes, cuda_device):
+    moe = build(codes, modules(cuda_device), resident=resident)
+    x, lg = inputs(3)
+    assert moe(x[:0], lg[:0]).shape == (0, H)
+
+
+def test_in_inference_mode(codes, cuda_device):
+    """Weights that change and are stacked anew there stay usable by autograd outside."""
+    moe = build(codes, modules(cuda_device))
+    with torch.inference_mode():
+        check(moe, 5)
+        moe.gpu_experts["4"].w3.weight.data = Expert(900, cuda_device).w3.weight.data
+        check(moe, 5)
+    check(moe, 5)
+    moe.gpu_experts["4"](inputs(2)[0]).sum().backward()
+    assert moe.gpu_experts["4"].w3.weight.grad is not None
+    check(moe, 5)
