@@ -61,7 +61,7 @@ MOE_DEV float activate(float v) {
   if constexpr (ACT == MOE_ACT_GELU_TANH) {
     // (1 + tanh y) / 2 = 1 / (1 + e^-2y), the exponential of the negative side on both, which cannot overflow
     const float y = 0.79788456080286536f * (v + 0.044715f * v * v * v), e = expf(-2.0f * fabsf(y));
-    return v * ((y < 0.0f ? e : 1.0f) / (1.0f + e));
+    return v * __fdividef(y < 0.0f ? e : 1.0f, 1.0f + e);  // of 1 .. 2: within 2 units
   }
   if constexpr (ACT == MOE_ACT_RELU) return v < 0.0f ? 0.0f : v;  // NaN stays NaN
   return v;
