@@ -473,6 +473,9 @@ int moe_linear_query(const moe_linear_desc* desc, moe_linear_plan* plan, char* e
  * workspace_dev: moe_dense_workspace bytes, 256-byte aligned, for this call
  * alone until its kernels have run (calls in flight at once, and graphs
  * replayed at once, each need their own).  Its contents need no preparation.
+ * It holds 4 bytes x tokens x hidden_size for each piece of the split, about
+ * (SMs + routed experts) and up to several times the SMs where their rows do not
+ * fit the SMs at once: 56 MB for 16 tokens of 128 experts of 2048 x 768.
  * Nothing else is kept between calls. */
 #define MOE_DENSE_MAX_TOKENS 16
 typedef struct moe_dense_desc {

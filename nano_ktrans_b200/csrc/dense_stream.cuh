@@ -71,7 +71,8 @@ constexpr int kSlots = 4;  // of a warp's ring
 // of a tile that does not exist is a copy less in flight (2048 x 2048, one token:
 // 4.0 us, with slots for four tiles where there is one 5.0); and two where a
 // round of four would be over after two steps (128 x 768 experts, hidden 2048,
-// 16 tokens: 149 us with two, 164 with four; 8 x 14336, hidden 4096: 439 and 424).
+// 16 tokens: 149 us with two, 164 with four; 8 x 14336, hidden 4096: 439 and 424;
+// sizes between were not measured).
 constexpr int kLongK = 2 * 64 * kSW + 1;
 template <int NT>
 inline int tiles_at_once(int tiles, int k) {

@@ -4,8 +4,8 @@ its argument, and each of its own bits has to be right, not only its distance on
 The arguments are made exactly: a zero product plus a bias, or one product by 1.  Bounds, relative to the result, of an
 fp32 evaluation at an exact argument v (a unit is 2^-23, an operation half a unit, expf 2 units, erfcf 4):
 gelu = v/2 erfc(z), z = -v/sqrt 2 off by a unit, which erfc magnifies by at most 2 z^2 + 2 = v^2 + 2; two products:
-(v^2 + 8) units.  gelu_tanh = v s(2 y): 2 y off by 3 units, which exp magnifies by |2 y|; exp 2, sum, quotient and
-product 3 halves: (6 |y| + 6) units.  Then one rounding to the type."""
+(v^2 + 8) units.  gelu_tanh = v s(2 y): 2 y off by 3 units, which exp magnifies by |2 y|; exp 2, quotient 2, sum and
+product 2 halves: (6 |y| + 6) units.  Then one rounding to the type."""
 import math
 
 import pytest
