@@ -140,6 +140,8 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
                  activation: Optional[str] = "silu", out: Optional[torch.Tensor] = None,
                  stream=None) -> torch.Tensor:
     """``act(x @ gate_weight.T) * (x @ up_weight.T)``, rounded once: the first half of a gated MLP."""
+    if up_weight is None:
+        raise ValueError("up_weight is missing: linear is the product with one weight")
     return _project(x, gate_weight, up_weight, None, activation, None, out, stream)
 
 
