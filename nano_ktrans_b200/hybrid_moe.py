@@ -81,7 +81,7 @@ class HybridMoE(nn.Module):
         self.hidden_act = hidden_act
         if resident_experts not in ("kernels", "modules", "dense"):
             raise ValueError("resident_experts must be 'kernels', 'modules' or 'dense'")
-        if resident_experts == "dense" and hidden_act not in ("silu", "swish"):
+        if resident_experts == "dense" and str(hidden_act).lower() not in ("silu", "swish"):
             raise ValueError(f"resident_experts='dense' runs gated SiLU experts, not hidden_act {hidden_act!r}")
         self.resident_experts = resident_experts
         self.has_cpu_experts = bool((~gpu_experts_mask.bool()).any().item())

@@ -169,6 +169,11 @@ def test_experts_of_another_kind_are_refused(codes, cuda_device):
         build(codes, modules(cuda_device, dtype=torch.float32))
 
 
+@pytest.mark.parametrize("name", ["silu", "SiLU", "swish"])
+def test_names_of_the_activation(name, codes, cuda_device):
+    check(build(codes, modules(cuda_device), hidden_act=name), 3)
+
+
 @pytest.mark.parametrize("where", ["expert", "linear"])
 @pytest.mark.parametrize("when", ["before", "after"])
 def test_hooks_are_run(when, where, codes, cuda_device):
